@@ -101,6 +101,55 @@ int mq_fp8_block_quant_pow2(const void* w, int dtype, int64_t ldw, void* q, floa
  *   w [rows,K] contiguous, K % 32 == 0; q [rows,K] e4m3fn; scale [rows,K/32] E8M0 bytes */
 int mq_mxfp8_quant(const void* w, int dtype, void* q, uint8_t* scale, int64_t rows, int64_t K, void* stream);
 
+/* The way back (no counterpart in the reference, whose MXFP8 tensors are read by the rollout engine): y = code x 2^(e - 127),
+ *   rounded once to y's dtype; a finite value that fp16 cannot hold becomes +-65504.  q [rows,K] e4m3fn, scale [rows,K/32],
+ *   y [rows,K] contiguous and 16-byte aligned. */
+int mq_mxfp8_dequant(const void* q, const uint8_t* scale, void* y, int dtype, int64_t rows, int64_t K, void* stream);
+
+/* Layer norm and RMS norm (no counterpart in the reference, which takes them from its trainer's libraries).
+ *   mean = sum(x)/n (rms != 0: 0), rstd = 1/sqrt(sum((x-mean)^2)/n + eps), xhat = (x-mean) rstd, y = xhat weight + bias
+ * x [rows,n] dtype, rows ldx elements apart, from any element boundary; weight, bias [n] of type wdtype (dtype or MQ_F32), either may
+ * be NULL; y [rows,n] contiguous.  Kept for the backward pass where the pointer is not NULL: mean, rstd [rows] fp32; xhat8 /
+ * xhat8_scale: xhat as MXFP8 (e4m3 codes [rows,n], exponent bytes [rows,n/32]; n a multiple of 32; 8-byte aligned).
+ * y8 / y8_scale: the MXFP8 copy of y itself, what mq_mxfp8_quant makes of it, for a layer that y goes into. */
+int mq_norm_forward(const void* x, int dtype, int64_t ldx, const void* weight, const void* bias, int wdtype, void* y, void* xhat8,
+                    uint8_t* xhat8_scale, void* y8, uint8_t* y8_scale, float* mean, float* rstd, int64_t rows, int64_t n,
+                    float eps, int rms, void* stream);
+/* Its backward pass: g = dy weight, dx = rstd (g - mean(g) [not rms] - xhat mean(g xhat)), dweight = sum over rows of dy xhat,
+ * dbias = sum over rows of dy (both of type wdtype).  x and mean are the forward pass's, or x holds the codes of xhat8 and
+ * xhat8_scale is not NULL (mean is then not read).  dx, dweight and dbias may each be NULL.
+ * ws: mq_norm_backward_parts(rows, n) * n floats of scratch for each of dweight and dbias that is wanted.  The rows' sums are added
+ * in an order that depends on the sizes alone. */
+int mq_norm_backward(const void* dy, int dtype, int64_t lddy, const void* x, int64_t ldx, const uint8_t* xhat8_scale, const float* mean,
+                     const float* rstd, const void* weight, int wdtype, void* dx, void* dweight, void* dbias, float* ws,
+                     int64_t rows, int64_t n, int rms, void* stream);
+int mq_norm_backward_parts(int64_t rows, int64_t n);
+
+/* Linear layers with bias, activation and residual in the product's epilogue (no counterpart in the reference).  All tensors of one
+ * dtype, MQ_BF16 or MQ_F16; sums in fp32.
+ *   z = x weight^T + bias, y = act(z) + residual;  x [M,K], weight [N,K], residual [M,N] with rows ldx, ldw, ldr elements apart,
+ *   bias [N] and residual may be NULL; y [M,N] contiguous.
+ *   Kept for the backward pass where the pointer is not NULL: z [M,N] contiguous, or z8 / z8_scale: z as MXFP8 ([M,N], [M,N/32];
+ *   N a multiple of 32; 4-byte aligned).
+ * Backward: mq_activation_backward makes dz = dy act'(z) (z, or z8 with z8_scale not NULL) [M,N] contiguous and dbias = sum over rows
+ *   of dz; with MQ_ACT_NONE z is not read and dz may be NULL.  Its ws: mq_activation_backward_parts(M, N) * N floats where dbias
+ *   is wanted.  mq_linear_input_grad: dx [M,K] = dz weight.  mq_linear_weight_grad: dweight [N,K] = dz^T x, x as above or
+ *   its MXFP8 copy (x_scale not NULL, K a multiple of 32, codes contiguous and 16-byte aligned), which is not restored in memory.
+ * ws of the products: mq_linear_workspace's floats (0: ws may be NULL), 16-byte aligned.  Sums are added in an order that depends on
+ *   the sizes, the alignment and the row strides alone. */
+enum { MQ_ACT_NONE = 0, MQ_ACT_RELU = 1, MQ_ACT_SILU = 2, MQ_ACT_GELU = 3, MQ_ACT_GELU_TANH = 4 };
+enum { MQ_LINEAR_FORWARD = 0, MQ_LINEAR_INPUT_GRAD = 1, MQ_LINEAR_WEIGHT_GRAD = 2 };
+int mq_linear_workspace(int product, int64_t M, int64_t N, int64_t K, int64_t* floats);
+int mq_linear_forward(const void* x, int dtype, int64_t ldx, const void* weight, int64_t ldw, const void* bias, int act, const void* residual,
+                      int64_t ldr, void* y, void* z, void* z8, uint8_t* z8_scale, int64_t M, int64_t N, int64_t K, float* ws, void* stream);
+int mq_activation_backward(const void* dy, int dtype, int64_t lddy, const void* z, const uint8_t* z8_scale, int act, void* dz, void* dbias,
+                           float* ws, int64_t M, int64_t N, void* stream);
+int mq_activation_backward_parts(int64_t M, int64_t N);
+int mq_linear_input_grad(const void* dz, int dtype, int64_t lddz, const void* weight, int64_t ldw, void* dx, int64_t M, int64_t N, int64_t K,
+                         float* ws, void* stream);
+int mq_linear_weight_grad(const void* dz, int dtype, int64_t lddz, const void* x, int64_t ldx, const uint8_t* x_scale, void* dweight,
+                          int64_t M, int64_t N, int64_t K, float* ws, void* stream);
+
 /* FP8 128x128 block-scaled source -> MXFP8           tools/convert_hf_to_mxfp8.py:56-102,180-195
  * A source tensor is e4m3fn codes x [M,K] with one scale per 128x128 tile: a grid of at least ceil(M/128) rows and
  * ceil(K/128) columns whose rows are lds elements apart (the reference crops a larger grid, :79,:91).

@@ -6,6 +6,7 @@ fallback: if the shared object is missing or does not load, every quantizer rais
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -29,6 +30,16 @@ SIGNATURES = {
     "mq_ue8m0_pack_scales": [_vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp],
     "mq_fp8_block_dequant": [_vp, _vp, _vp, _i64, _i64, _i32, _vp],
     "mq_mxfp8_quant": [_vp, _i32, _vp, _vp, _i64, _i64, _vp],
+    "mq_mxfp8_dequant": [_vp, _vp, _vp, _i32, _i64, _i64, _vp],
+    "mq_norm_forward": [_vp, _i32, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _i32, _vp],
+    "mq_norm_backward": [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp],
+    "mq_norm_backward_parts": [_i64, _i64],
+    "mq_linear_workspace": [_i32, _i64, _i64, _i64, _vp],
+    "mq_linear_forward": [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp],
+    "mq_activation_backward": [_vp, _i32, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _vp],
+    "mq_activation_backward_parts": [_i64, _i64],
+    "mq_linear_input_grad": [_vp, _i32, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp],
+    "mq_linear_weight_grad": [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp],
     "mq_e8m0_bytes_to_f32": [_vp, _vp, _i64, _vp],
     "mq_fp8_scales_pow2_flag": [_vp, _i64, _i64, _i64, _vp, _vp],
     "mq_e8m0_expand_tile_scales": [_vp, _i32, _i64, _vp, _i64, _i64, _vp],
@@ -130,6 +141,16 @@ def stream_ptr(device: torch.device | None = None) -> int:
             raise ValueError(f"Expected a cuda device, but got: {device}")
         index = torch.cuda.current_device() if device is None or device.index is None else device.index
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """The block in which `device` is the current one: kernels are launched on the current device."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 def require_gpu(t: torch.Tensor, what: str) -> None:

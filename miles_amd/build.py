@@ -14,6 +14,8 @@ import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -21,7 +23,8 @@ LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libmiles_quant.so")
 PROBES_LIB_PATH = os.path.join(LIB_DIR, "libmq_probes.so")
 
-SOURCES = ["mq_core.hip", "mq_fp8_block.hip", "mq_mxfp8.hip", "mq_rescale.hip", "mq_mxfp4.hip", "mq_fake_quant.hip", "mq_int4.hip", "mq_nvfp4.hip", "mq_fp8_tensor.hip", "mq_sync.hip"]
+SOURCES = ["mq_core.hip", "mq_fp8_block.hip", "mq_mxfp8.hip", "mq_rescale.hip", "mq_mxfp4.hip", "mq_fake_quant.hip", "mq_int4.hip", "mq_nvfp4.hip", "mq_fp8_tensor.hip", "mq_sync.hip",
+           "mq_norm.hip", "mq_linear.hip", "mq_gemm_forward.hip", "mq_gemm_input_grad.hip", "mq_gemm_weight_grad.hip"]
 HOST_LIB_PATH = os.path.join(LIB_DIR, "mq_host.so")
 HOST_SOURCE = os.path.join(CSRC, "host", "mq_host.cpp")
 PROBE_SOURCES = ["mq_selftest.hip", "mq_probe.hip"]
@@ -31,7 +34,6 @@ FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-ffp-contract=off",
     "-fno-fast-math",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
@@ -40,8 +42,7 @@ FLAGS = [
 ]
 
 
-def _link(target: str, sources: list[str], verbose: bool, libraries: tuple[str, ...] = ()) -> None:
-    cmd = ["hipcc", *FLAGS, "-o", target, *(os.path.join(CSRC, s) for s in sources), *libraries]
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd))
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
@@ -50,6 +51,16 @@ def _link(target: str, sources: list[str], verbose: bool, libraries: tuple[str, 
         raise RuntimeError(f"hipcc failed:\n{out}")
     if verbose and out.strip():
         print(out)
+
+
+def _link(target: str, sources: list[str], verbose: bool, libraries: tuple[str, ...] = ()) -> None:
+    """Every source compiled by itself, several at a time, and the objects linked."""
+    with tempfile.TemporaryDirectory() as objects:
+        paths = [os.path.join(objects, s + ".o") for s in sources]
+        with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+            for _ in pool.map(lambda s, o: _run(["hipcc", *FLAGS, "-c", "-o", o, os.path.join(CSRC, s)], verbose), sources, paths):
+                pass
+        _run(["hipcc", "--offload-arch=gfx950", "-fPIC", "-shared", "-o", target, *paths, *libraries], verbose)
 
 
 def _link_host(verbose: bool) -> None:

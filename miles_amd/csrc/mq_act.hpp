@@ -1,0 +1,71 @@
+// Activations of the linear layers and their slopes, in fp32.
+#pragma once
+#include <type_traits>
+
+#include "mq_api_internal.hpp"
+#include "mq_common.hpp"
+
+namespace mq {
+
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+
+// exp(-z^2 / 2) and Phi(z), the normal distribution's share below z, by formula 7.1.26 of Abramowitz and Stegun (1964), whose error
+// is at most 1.5e-7 for erf, a hundred-thousandth of a step of the 16-bit results; the side of small shares is computed itself and
+// not as 1 minus the other.
+__device__ __forceinline__ void normal_share(float z, float& bell, float& share) {
+    const float x = __builtin_fabsf(z) * 0.7071067811865476f;
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
+    float p = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+    p = __builtin_fmaf(t, p, 1.421413741f);
+    p = __builtin_fmaf(t, p, -0.284496736f);
+    p = __builtin_fmaf(t, p, 0.254829592f);
+    bell = fast_exp(-x * x);
+    const float tail = 0.5f * t * p * bell;
+    share = z < 0.0f ? tail : 1.0f - tail;
+}
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z)); }
+
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if (ACT == MQ_ACT_RELU) return z < 0.0f ? 0.0f : z;          // (a NaN stays)
+    if (ACT == MQ_ACT_SILU) return z * sigmoid(z);
+    if (ACT == MQ_ACT_GELU) {
+        float bell, share;
+        normal_share(z, bell, share);
+        return z * share;
+    }
+    // 0.5 z (1 + tanh(u)) = z sigmoid(2 u), u = sqrt(2/pi) (z + 0.044715 z^3)
+    if (ACT == MQ_ACT_GELU_TANH) return z * sigmoid(1.5957691216057308f * z * __builtin_fmaf(0.044715f, z * z, 1.0f));
+    return z;
+}
+// the slope of the activation at z
+template <int ACT>
+__device__ __forceinline__ float slope(float z) {
+    if (ACT == MQ_ACT_RELU) return z > 0.0f ? 1.0f : z == z ? 0.0f : z;
+    if (ACT == MQ_ACT_SILU) {
+        const float s = sigmoid(z);
+        return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
+    }
+    if (ACT == MQ_ACT_GELU) {
+        float bell, share;
+        normal_share(z, bell, share);
+        return __builtin_fmaf(z * 0.3989422804014327f, bell, share);
+    }
+    if (ACT == MQ_ACT_GELU_TANH) {
+        const float s = sigmoid(1.5957691216057308f * z * __builtin_fmaf(0.044715f, z * z, 1.0f));
+        return s * __builtin_fmaf(1.5957691216057308f * z * __builtin_fmaf(0.134145f, z * z, 1.0f), 1.0f - s, 1.0f);
+    }
+    return 1.0f;
+}
+
+// the activation as a template argument
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+    if (act == MQ_ACT_GELU) f(std::integral_constant<int, MQ_ACT_GELU>{});
+    else if (act == MQ_ACT_SILU) f(std::integral_constant<int, MQ_ACT_SILU>{});
+    else if (act == MQ_ACT_RELU) f(std::integral_constant<int, MQ_ACT_RELU>{});
+    else if (act == MQ_ACT_GELU_TANH) f(std::integral_constant<int, MQ_ACT_GELU_TANH>{});
+    else f(std::integral_constant<int, MQ_ACT_NONE>{});
+}
+
+}  // namespace mq

@@ -10,6 +10,7 @@
 #include "mq_api_internal.hpp"
 #include "mq_common.hpp"
 #include "mq_group.hpp"
+#include "mq_rows.hpp"
 
 namespace mq {
 
@@ -160,6 +161,43 @@ __global__ __launch_bounds__(256) void mxfp8_generic_kernel(const void* __restri
     }
 }
 
+// The way back: code x 2^(e - 127), rounded once to the output's type (for bf16 and fp32 there is nothing to round outside
+// the subnormals).  A finite value that fp16 cannot hold becomes its largest: the code above 65504 stands for a value below it.
+// A lane stores 16 bytes per unit, from one load of eight (16-bit outputs) or four codes, all loads before the first use.
+constexpr int kMxBackUnits = 2;
+template <int D>
+__global__ __launch_bounds__(256) void mxfp8_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale, char* __restrict__ y,
+                                                            int64_t units) {
+    constexpr int V = kVec<D>;
+    const int64_t base = (int64_t)blockIdx.x * (256 * kMxBackUnits) + threadIdx.x;
+    u32x2 c[kMxBackUnits];
+    uint32_t e[kMxBackUnits];
+#pragma unroll
+    for (int i = 0; i < kMxBackUnits; i++) {
+        const int64_t u = base + i * 256;
+        c[i] = u32x2{0u, 0u};
+        e[i] = 0;
+        if (u < units) {
+            if (D == MQ_F32) c[i].x = *(const u32_at1*)(q + u * 4);
+            else c[i] = ld8_at1(q + u * 8);
+            e[i] = scale[u * V / 32];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kMxBackUnits; i++) {
+        const int64_t u = base + i * 256;
+        const float s = e8m0_value(e[i]);
+        float f[8];
+        kept_values4(c[i].x, s, f);
+        if (D != MQ_F32) kept_values4(c[i].y, s, f + 4);
+        if (D == MQ_F16) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] = clamp_keep_nan(f[j], -65504.0f, 65504.0f);
+        }
+        if (u < units) st16(y + u * 16, pack<D>(f));
+    }
+}
+
 }  // namespace mq
 
 using namespace mq;
@@ -214,4 +252,20 @@ extern "C" int mq_mxfp8_quant(const void* w, int dtype, void* q, uint8_t* scale,
     hipLaunchKernelGGL(mxfp8_generic_kernel, dim3((unsigned)blocks), dim3(256), 0, st, w, dtype, (uint8_t*)q, scale,
                        groups);
     return mq_check_launch("mxfp8 quant");
+}
+
+extern "C" int mq_mxfp8_dequant(const void* q, const uint8_t* scale, void* y, int dtype, int64_t rows, int64_t K, void* stream) {
+    if ((!q || !scale || !y) && rows != 0 && K != 0) return mq_fail(MQ_ERR_ARG, "null pointer");
+    if (dtype < MQ_BF16 || dtype > MQ_F32 || rows < 0 || K < 0) return mq_fail(MQ_ERR_ARG, "bad argument");
+    if (K % 32 != 0) return mq_fail(MQ_ERR_ARG, "Last dim must be divisible by 32 for MXFP8.");
+    if ((uintptr_t)y % 16) return mq_fail(MQ_ERR_ARG, "the output starts at a multiple of 16 bytes");
+    if (rows == 0 || K == 0) return MQ_OK;
+    const int64_t units = rows * (K / (dtype == MQ_F32 ? 4 : 8)), blocks = (units + 256 * kMxBackUnits - 1) / (256 * kMxBackUnits);
+    if (blocks > 0x7FFFFFF0) return mq_fail(MQ_ERR_ARG, "tensor too large");
+    const dim3 grid((unsigned)blocks), blk(256);
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == MQ_F32) hipLaunchKernelGGL(mxfp8_dequant_kernel<MQ_F32>, grid, blk, 0, st, (const uint8_t*)q, scale, (char*)y, units);
+    else if (dtype == MQ_F16) hipLaunchKernelGGL(mxfp8_dequant_kernel<MQ_F16>, grid, blk, 0, st, (const uint8_t*)q, scale, (char*)y, units);
+    else hipLaunchKernelGGL(mxfp8_dequant_kernel<MQ_BF16>, grid, blk, 0, st, (const uint8_t*)q, scale, (char*)y, units);
+    return mq_check_launch("mxfp8 dequant");
 }

@@ -1,0 +1,129 @@
+// Row access shared by the norm kernels and the linear layers' epilogues: elements of any of the three types as floats, sums
+// over lanes, and the 8-bit copies (e4m3 codes, one E8M0 exponent byte per 32 columns) that stand for an activation.
+#pragma once
+#include "mq_api_internal.hpp"
+#include "mq_common.hpp"
+
+namespace mq {
+
+// elements of one 16-byte access
+template <int D>
+constexpr int kVec = D == MQ_F32 ? 4 : 8;
+template <int D>
+constexpr int kElem = D == MQ_F32 ? 4 : 2;
+
+template <int D>
+__device__ __forceinline__ float one_elem(const void* p, int64_t i) { return load_f32(p, i, D); }
+
+// kVec elements from any element boundary
+template <int D>
+__device__ __forceinline__ void unpack(u32x4 v, float* f) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (D == MQ_F32) f[i] = u2f(u[i]);
+        else {
+            f[2 * i] = elem_lo<D == MQ_F16>(u[i]);
+            f[2 * i + 1] = elem_hi<D == MQ_F16>(u[i]);
+        }
+    }
+}
+// two floats as two 16-bit elements, rounded to nearest even
+template <int D>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if (D == MQ_F16) {
+        const _Float16 x = (_Float16)a, y = (_Float16)b;
+        return (uint32_t)__builtin_bit_cast(uint16_t, x) | ((uint32_t)__builtin_bit_cast(uint16_t, y) << 16);
+    }
+    return hw_bf16x2(a, b);
+}
+template <int D>
+__device__ __forceinline__ u32x4 pack(const float* f) {
+    if (D == MQ_F32) return u32x4{f2u(f[0]), f2u(f[1]), f2u(f[2]), f2u(f[3])};
+    return u32x4{pack2<D>(f[0], f[1]), pack2<D>(f[2], f[3]), pack2<D>(f[4], f[5]), pack2<D>(f[6], f[7])};
+}
+// the kVec elements of a row from column c on, zero from column n on
+template <int D>
+__device__ __forceinline__ u32x4 ld_row(const void* row, int64_t c, int64_t n) {
+    constexpr int V = kVec<D>;
+    if (c + V <= n) return ld16_at2((const char*)row + c * kElem<D>);
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (c < n) {
+        uint32_t u[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            if (c + j < n) {
+                if (D == MQ_F32) u[j & 3] = ((const uint32_t*)row)[c + j];
+                else u[j / 2] |= (uint32_t)((const uint16_t*)row)[c + j] << (16 * (j & 1));
+            }
+        }
+        v = u32x4{u[0], u[1], u[2], u[3]};
+    }
+    return v;
+}
+template <int D>
+__device__ __forceinline__ void st_row(void* row, int64_t c, int64_t n, u32x4 v) {
+    constexpr int V = kVec<D>;
+    if (c + V <= n) {
+        st16_at2((char*)row + c * kElem<D>, v);
+        return;
+    }
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        if (c + j < n) {
+            if (D == MQ_F32) ((uint32_t*)row)[c + j] = u[j & 3];
+            else ((uint16_t*)row)[c + j] = (uint16_t)(u[j / 2] >> (16 * (j & 1)));
+        }
+    }
+}
+// V elements of a vector that is fp32 (WF32) or of type D, zero from n on
+template <int D, int WF32>
+__device__ __forceinline__ void ld_vector(const void* p, int64_t c, int64_t n, float* f) {
+    constexpr int V = kVec<D>;
+    if (WF32) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) unpack<MQ_F32>(ld_row<MQ_F32>(p, c + j, n), f + j);
+    } else {
+        unpack<D>(ld_row<D>(p, c, n), f);
+    }
+}
+
+// ---- sums over lanes ---------------------------------------------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v) { return u2f(dpp_u32<CTRL>(f2u(v))); }
+// the same order of additions in every lane, so that a result does not depend on which lane reads it
+__device__ __forceinline__ float wave_sum(float v) {
+    v += dpp_f32<kDppQuadXor1>(v);
+    v += dpp_f32<kDppQuadXor2>(v);
+    v += dpp_f32<kDppRowHalfMirror>(v);
+    v += dpp_f32<kDppRowMirror>(v);
+    const float a = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(v), 0)), b = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(v), 16));
+    const float c = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(v), 32)), d = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(v), 48));
+    return (a + b) + (c + d);
+}
+
+// ---- 8-bit copies --------------------------------------------------------------------------------------------------------
+// 2^(e - 127)
+__device__ __forceinline__ float e8m0_value(uint32_t e) { return e ? u2f(e == 255 ? 0x7FC00000u : e << 23) : u2f(0x00400000u); }
+// a magnitude's part in the group maximum: a NaN has none (the arithmetic of mxfp8_quantize)
+__device__ __forceinline__ uint32_t keep_magnitude(float v) {
+    const uint32_t a = f2u(v) & 0x7FFFFFFFu;
+    return a > 0x7F800000u ? 0u : a;
+}
+// four values over the group's power of two: the clamp takes infinities to 448, a NaN goes through
+__device__ __forceinline__ uint32_t keep_codes4(float a, float b, float c, float d, float inv) {
+    return hw_e4m3x4(clamp_keep_nan(a * inv, -kFp8Max, kFp8Max), clamp_keep_nan(b * inv, -kFp8Max, kFp8Max),
+                     clamp_keep_nan(c * inv, -kFp8Max, kFp8Max), clamp_keep_nan(d * inv, -kFp8Max, kFp8Max));
+}
+__device__ __forceinline__ uint32_t keep_exponent(uint32_t group_magnitude) { return e8m0_ceil(u2f(group_magnitude) * u2f(0x3B124925u)); }
+// four codes as floats: exact, a power of two away from three bits of mantissa
+__device__ __forceinline__ void kept_values4(uint32_t codes, float scale, float* f) {
+    const f32x2 lo = hw_e4m3x2_decode<false>(codes), hi = hw_e4m3x2_decode<true>(codes);
+    f[0] = lo.x * scale;
+    f[1] = lo.y * scale;
+    f[2] = hi.x * scale;
+    f[3] = hi.y * scale;
+}
+
+}  // namespace mq

@@ -57,6 +57,28 @@ def mxfp8_quantize(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
                           (torch.uint8, *w.shape[:-1], k // MXFP8_GROUP_SIZE))
 
 
+def mxfp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """(float8_e4m3fn codes [..., K], uint8 E8M0 scales [..., K/32]) of `mxfp8_quantize` -> the values they stand for, `code x
+    2^(scale - 127)` rounded once to bf16, fp16 or fp32 (in fp16 a finite value beyond +-65504 becomes +-65504)."""
+    _lib.require_gpu(codes, "mxfp8_dequantize")
+    _lib.require_gpu(scales, "mxfp8_dequantize")
+    if codes.dtype not in (torch.float8_e4m3fn, torch.uint8) or scales.dtype != torch.uint8:
+        raise ValueError(f"expected float8_e4m3fn codes and uint8 scales, got {codes.dtype} and {scales.dtype}")
+    if dtype not in _lib.DTYPE_CODE:
+        raise ValueError(f"MXFP8 values are returned as bfloat16, float16 or float32, not {dtype}")
+    if codes.dim() == 0 or codes.shape[-1] % MXFP8_GROUP_SIZE or scales.shape != (*codes.shape[:-1], codes.shape[-1] // MXFP8_GROUP_SIZE):
+        raise ValueError(f"scales {tuple(scales.shape)} are not those of codes {tuple(codes.shape)}, one for each {MXFP8_GROUP_SIZE} of a row")
+    if codes.device != scales.device:
+        raise ValueError(f"codes on {codes.device}, scales on {scales.device}")
+    q, s, k = codes.contiguous(), scales.contiguous(), codes.shape[-1]
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    launch.note_direct_call()
+    with _lib.on_device(q.device):
+        _lib.check(_lib.load().mq_mxfp8_dequant(q.data_ptr(), s.data_ptr(), out.data_ptr(), _lib.DTYPE_CODE[dtype],
+                                                q.numel() // k if k else 0, k, _lib.stream_ptr(q.device)))
+    return out
+
+
 # ---- FP8 128x128 block-scaled sources (tools/convert_hf_to_mxfp8.py:56-102,180-195) ---------------------------------
 SOURCE_FP8_TILE = 128
 
