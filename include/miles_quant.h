@@ -135,20 +135,23 @@ int mq_norm_backward_parts(int64_t rows, int64_t n);
  *   of dz; with MQ_ACT_NONE z is not read and dz may be NULL.  Its ws: mq_activation_backward_parts(M, N) * N floats where dbias
  *   is wanted.  mq_linear_input_grad: dx [M,K] = dz weight.  mq_linear_weight_grad: dweight [N,K] = dz^T x, x as above or
  *   its MXFP8 copy (x_scale not NULL, K a multiple of 32, codes contiguous and 16-byte aligned), which is not restored in memory.
- * ws of the products: mq_linear_workspace's floats (0: ws may be NULL), 16-byte aligned.  Sums are added in an order that depends on
- *   the sizes, the alignment and the row strides alone. */
+ * ws of the products: mq_linear_workspace's bytes (0: ws may be NULL), 16-byte aligned, for partial sums and for copies of operands
+ *   whose rows do not begin and end at multiples of 16 bytes.  a and b: the operands as they are passed to the product, x or dz and
+ *   weight or x, with their row strides; kept8: z8 is wanted, or x is an 8-bit copy.  Sums are added in an order that depends on
+ *   the sizes, kept8 and, for MQ_LINEAR_FORWARD, on whether M is at most 16. */
 enum { MQ_ACT_NONE = 0, MQ_ACT_RELU = 1, MQ_ACT_SILU = 2, MQ_ACT_GELU = 3, MQ_ACT_GELU_TANH = 4 };
 enum { MQ_LINEAR_FORWARD = 0, MQ_LINEAR_INPUT_GRAD = 1, MQ_LINEAR_WEIGHT_GRAD = 2 };
-int mq_linear_workspace(int product, int64_t M, int64_t N, int64_t K, int64_t* floats);
+int mq_linear_workspace(int product, const void* a, int64_t lda, const void* b, int64_t ldb, int kept8, int64_t M, int64_t N, int64_t K,
+                        int64_t* bytes);
 int mq_linear_forward(const void* x, int dtype, int64_t ldx, const void* weight, int64_t ldw, const void* bias, int act, const void* residual,
-                      int64_t ldr, void* y, void* z, void* z8, uint8_t* z8_scale, int64_t M, int64_t N, int64_t K, float* ws, void* stream);
+                      int64_t ldr, void* y, void* z, void* z8, uint8_t* z8_scale, int64_t M, int64_t N, int64_t K, void* ws, void* stream);
 int mq_activation_backward(const void* dy, int dtype, int64_t lddy, const void* z, const uint8_t* z8_scale, int act, void* dz, void* dbias,
                            float* ws, int64_t M, int64_t N, void* stream);
 int mq_activation_backward_parts(int64_t M, int64_t N);
 int mq_linear_input_grad(const void* dz, int dtype, int64_t lddz, const void* weight, int64_t ldw, void* dx, int64_t M, int64_t N, int64_t K,
-                         float* ws, void* stream);
+                         void* ws, void* stream);
 int mq_linear_weight_grad(const void* dz, int dtype, int64_t lddz, const void* x, int64_t ldx, const uint8_t* x_scale, void* dweight,
-                          int64_t M, int64_t N, int64_t K, float* ws, void* stream);
+                          int64_t M, int64_t N, int64_t K, void* ws, void* stream);
 
 /* FP8 128x128 block-scaled source -> MXFP8           tools/convert_hf_to_mxfp8.py:56-102,180-195
  * A source tensor is e4m3fn codes x [M,K] with one scale per 128x128 tile: a grid of at least ceil(M/128) rows and

@@ -34,7 +34,7 @@ SIGNATURES = {
     "mq_norm_forward": [_vp, _i32, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _i32, _vp],
     "mq_norm_backward": [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp],
     "mq_norm_backward_parts": [_i64, _i64],
-    "mq_linear_workspace": [_i32, _i64, _i64, _i64, _vp],
+    "mq_linear_workspace": [_i32, _vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp],
     "mq_linear_forward": [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp],
     "mq_activation_backward": [_vp, _i32, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _vp],
     "mq_activation_backward_parts": [_i64, _i64],

@@ -4,13 +4,13 @@
 //   forward          P = W [N][K], Q = x [M][K]          both with k along the rows
 //   input gradient   P = W [N][K] read as (k of W, n), Q = dz [M][N]
 //   weight gradient  P = x [M][K] or its 8-bit copy, Q = dz [M][N], both with the sum going down the rows
-// A workgroup computes a BP x BQ tile of the output in steps of 64 along k, through two buffers in shared memory: while the matrix
-// cores work on one, the next step's operands go into the other.
+// A workgroup computes a BP x BQ tile of the output in steps of 64 along k: the operands of a step lie in shared memory while those
+// of the next steps are on their way.
 //
-// Operands with k along the rows lie in shared memory as rows of 64 elements (eight 16-byte slots; slot s of row r holds the
-// row's piece s ^ (r & 7), so that the 16 rows of a fragment read from all banks); a lane's eight k are one 16-byte read.  Operands
-// whose sum goes down the rows lie as 64 rows of BP or BQ elements (32-byte slots, slot c of row k holds piece c ^ swizzle(k)); a
-// lane's eight k come by two transposing reads of four rows by 16 columns for each 16 lanes.
+// Operands with k along the rows lie in shared memory as rows of 64 elements, a cache line of memory each (eight 16-byte slots; slot s
+// of row r holds the row's piece s ^ (r / 2 & 7), so that the rows of a fragment are read from all banks); a lane's eight k are
+// one 16-byte read.  Operands whose sum goes down the rows lie as 64 rows of BP or BQ elements (32-byte slots, slot c of row k holds
+// piece c ^ swizzle(k)); a lane's eight k come by two transposing reads of four rows by 16 columns for each 16 lanes.
 // The P operand is the first of v_mfma_f32_16x16x32: a lane's four results are neighbours along p, the rows of the output.
 #pragma once
 #include "mq_act.hpp"
@@ -20,9 +20,10 @@ namespace mq {
 
 constexpr int kStep = 64;                 // k of a step
 
-// how an operand is staged: k along its rows or down them; straight into shared memory (16-byte aligned rows, sizes a multiple of
-// eight), through registers with every bound checked, or from an 8-bit copy (then 16-bit values are made on the way)
-enum { kRowsDirect = 0, kRowsAny = 1, kDownDirect = 2, kDownAny = 3, kDownKept = 4 };
+// How an operand is staged: k along its rows or down them, straight into shared memory; or from an 8-bit copy, whose 16-bit values are
+// made on the way.  Rows begin at multiples of 16 bytes, and the last piece of eight of a row is read whole: what lies behind the
+// operand's end along k has to be zero there (an operand that is not like that is copied first).
+enum { kRows = 0, kDown = 1, kDownKept = 2 };
 
 struct GemmArgs {
     const char* p;
@@ -36,12 +37,15 @@ struct GemmArgs {
     int64_t ldr;
     char* z;                              // what the activation is applied to, in the output's type, null: not kept
     uint8_t *zq, *zs;                     // the same in 8 bits, null: not kept
-    float* ws;                            // partial sums [splits][nq][round up np to 4], null: one split
-    int64_t k_split;                      // k of a split, a multiple of the step
-    int tiles_p, tiles_q, act;
+    // Tiles from `whole` on are cut along k into `splits` parts of k_split (a multiple of the step); part s of tile t leaves its sums
+    // at ws + ((t - whole) splits + s) BP BQ, row by row.
+    float* ws;
+    int64_t k_split;
+    int tiles_p, tiles_q, whole, splits, act;
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -51,6 +55,13 @@ template <int D>
 __device__ __forceinline__ f32x4 mfma(u32x4 p, u32x4 q, f32x4 c) {
     if (D == MQ_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+}
+
+// 32 x 32 outputs, 16 k
+template <int D>
+__device__ __forceinline__ f32x16 mfma(u32x4 p, u32x4 q, f32x16 c) {
+    if (D == MQ_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
 }
 
 // 16 bytes from memory straight into shared memory: lane i's go to `lds` + 16 i (lds uniform), from rsrc's base + offset, zeros where
@@ -70,6 +81,17 @@ __device__ __forceinline__ u32x4 buffer_of(const char* base) {
     return r;
 }
 
+// the same into registers, and one byte
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource_of(const void* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00027000);
+}
+__device__ __forceinline__ u32x4 read16(const void* base, uint32_t offset) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(resource_of(base), (int)offset, 0, 0));
+}
+__device__ __forceinline__ uint32_t read1(const void* base, uint32_t offset) {
+    return __builtin_amdgcn_raw_buffer_load_b8(resource_of(base), (int)offset, 0, 0);
+}
+
 // piece order of row k of an operand that lies down the rows, 32-byte pieces, B elements to a row
 template <int B>
 __device__ __forceinline__ int down_swizzle(int k) { return ((k & 3) | ((k >> 1) & 4)) & (B / 16 - 1); }
@@ -77,9 +99,9 @@ __device__ __forceinline__ int down_swizzle(int k) { return ((k & 3) | ((k >> 1)
 // One operand's way into shared memory.  A buffer is B x 64 elements; thread t's unit u is the 16 bytes at (t + u THREADS) 16.
 template <int MODE, int D, int B, int THREADS>
 struct Stage {
-    static constexpr bool kDirect = MODE == kRowsDirect || MODE == kDownDirect;
-    static constexpr bool kDown = MODE >= kDownDirect;
+    static constexpr bool kAcross = MODE == kRows;
     static constexpr bool kKept = MODE == kDownKept;
+    static constexpr bool kDirect = !kKept;
     static constexpr int kUnits = B * 8 / THREADS;
     static constexpr int kPieces = kKept ? kUnits / 2 : kUnits;       // accesses to memory: 16 codes fill two units
     static_assert(B * 8 % (THREADS * (kKept ? 2 : 1)) == 0, "whole units");
@@ -87,11 +109,12 @@ struct Stage {
     const char* base;                     // the tile's first element at the next step's first k
     const uint8_t* scales;
     int64_t ld, n;                        // n: outputs from the tile's first on
-    int64_t advance;
+    int64_t step_bytes;
     uint32_t offset[kPieces];
     u32x4 v[kPieces];
     uint32_t e[kPieces];
 
+    static __device__ __forceinline__ int row_piece(int at) { return (at & 7) ^ (at >> 4 & 7); }
     static __device__ __forceinline__ int down_k(int at) { return at / (B / 8); }
     static __device__ __forceinline__ int down_col(int at) {
         const int unit = at % (B / 8);
@@ -102,113 +125,73 @@ struct Stage {
         ld = ld_;
         n = count - first;
         constexpr int kSize = kKept ? 1 : 2;
-        base = op + (kDown ? k0 * ld + first : first * ld + k0) * kSize;
-        advance = (kDown ? kStep * ld : kStep) * kSize;
+        base = op + (kAcross ? first * ld + k0 : k0 * ld + first) * kSize;
+        step_bytes = (kAcross ? kStep : kStep * ld) * kSize;
         if (kKept) scales = s + k0 * (ld / 32) + first / 32;
         if (kDirect) {
 #pragma unroll
             for (int u = 0; u < kUnits; u++) {
                 const int at = (int)threadIdx.x + u * THREADS;
-                if (kDown) {
+                if (kAcross) {
+                    const int row = at >> 3, c = row_piece(at);
+                    offset[u] = (uint32_t)((row < n ? row : n - 1) * ld * 2 + c * 16);
+                } else {
                     const int k = down_k(at), c = down_col(at);
                     offset[u] = (uint32_t)((int64_t)k * ld * 2 + (c < n ? c : 0) * 2);
-                } else {
-                    const int row = at >> 3, c = (at & 7) ^ (row & 7);
-                    offset[u] = (uint32_t)((row < n ? row : n - 1) * ld * 2 + c * 16);
                 }
             }
         }
     }
-    // the next step's operand: on its way to `lds` (direct), or into registers; left: k that are left from the step's first on
-    __device__ __forceinline__ void fetch(uint32_t lds, int64_t left) {
+    // The next step's operand, piece by piece: on its way to `lds` (direct), or into registers.  left: k that are left from the step's
+    // first on, from zero down for a step behind the last, whose operands are zeros.  All pieces of a step, then `advance`.
+    __device__ __forceinline__ void fetch_piece(int u, uint32_t lds, int left) {
         if (kDirect) {
-            const u32x4 rsrc = buffer_of(base);
             const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave) * (kWave * 16);
-            if (left >= kStep) {
-#pragma unroll
-                for (int u = 0; u < kUnits; u++) direct16(lds + wave + u * (THREADS * 16), rsrc, offset[u]);
-            } else {
-#pragma unroll
-                for (int u = 0; u < kUnits; u++) {
-                    const int at = (int)threadIdx.x + u * THREADS;
-                    const int k = kDown ? down_k(at) : ((at & 7) ^ ((at >> 3) & 7)) * 8;
-                    direct16(lds + wave + u * (THREADS * 16), rsrc, k < left ? offset[u] : kNowhere);
-                }
-            }
-        } else if (kKept) {
-#pragma unroll
-            for (int i = 0; i < kPieces; i++) {
-                const int at = ((int)threadIdx.x + i * THREADS) * 2, k = down_k(at), c = down_col(at);
-                v[i] = u32x4{0u, 0u, 0u, 0u};
-                e[i] = 0;
-                if (k < left && c < n) {
-                    v[i] = *(const u32x4*)(base + k * ld + c);
-                    e[i] = scales[k * (ld / 32) + c / 32];
-                }
-            }
-            scales += kStep * (ld / 32);
+            const int at = (int)threadIdx.x + u * THREADS, k = kAcross ? row_piece(at) * 8 : down_k(at);
+            direct16(lds + wave + u * (THREADS * 16), buffer_of(base), k < left ? offset[u] : kNowhere);
         } else {
-#pragma unroll
-            for (int u = 0; u < kUnits; u++) {
-                const int at = (int)threadIdx.x + u * THREADS;
-                v[u] = u32x4{0u, 0u, 0u, 0u};
-                if (kDown) {
-                    const int k = down_k(at), c = down_col(at);
-                    if (k < left) v[u] = ld_row<MQ_BF16>(base + (int64_t)k * ld * 2, c, n);
-                } else {
-                    const int row = at >> 3, c = ((at & 7) ^ (row & 7)) * 8;
-                    if (row < n) v[u] = ld_row<MQ_BF16>(base + (int64_t)row * ld * 2, c, left);
-                }
-            }
+            const int at = ((int)threadIdx.x + u * THREADS) * 2, k = down_k(at), c = down_col(at);
+            const bool inside = k < left && c < n;
+            v[u] = read16(base, inside ? (uint32_t)(k * ld + c) : kNowhere);
+            e[u] = read1(scales, inside ? (uint32_t)(k * (ld / 32) + c / 32) : kNowhere);
         }
-        base += advance;
     }
-    // what came through registers, into shared memory
-    __device__ __forceinline__ void put(MQ_LDS char* lds) {
+    __device__ __forceinline__ void advance() {
+        base += step_bytes;
+        if (kKept) scales += kStep * (ld / 32);
+    }
+    // a quarter, four values, of an 8-bit piece that came through registers, into shared memory
+    __device__ __forceinline__ void put_part(int u, int part, MQ_LDS char* lds) {
         if (kDirect) return;
-        if (kKept) {
+        float f[4];
+        kept_values4(part == 0 ? v[u].x : part == 1 ? v[u].y : part == 2 ? v[u].z : v[u].w, e8m0_value(e[u]), f);
+        if (D == MQ_F16)
 #pragma unroll
-            for (int i = 0; i < kPieces; i++) {
-                const float s = e8m0_value(e[i]);
-                const uint32_t c[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                float f[16];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    kept_values4(c[j], s, f + 4 * j);
-                    if (D == MQ_F16)
-                        for (int m = 0; m < 4; m++) f[4 * j + m] = clamp_keep_nan(f[4 * j + m], -65504.0f, 65504.0f);
-                }
-                MQ_LDS u32x4* to = (MQ_LDS u32x4*)(lds + ((int)threadIdx.x + i * THREADS) * 32);
-                to[0] = pack<D>(f);
-                to[1] = pack<D>(f + 8);
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < kUnits; u++) *(MQ_LDS u32x4*)(lds + ((int)threadIdx.x + u * THREADS) * 16) = v[u];
-        }
+            for (int m = 0; m < 4; m++) f[m] = clamp_keep_nan(f[m], -65504.0f, 65504.0f);
+        *(MQ_LDS u32x2*)(lds + ((int)threadIdx.x + u * THREADS) * 32 + part * 8) = u32x2{pack2<D>(f[0], f[1]), pack2<D>(f[2], f[3])};
     }
 };
 
 // Addresses of a wavefront's fragments of an operand in shared memory: F fragments of 16 outputs from `first` on
 template <int MODE, int B, int F>
 struct Fragments {
-    static constexpr bool kDown = MODE >= kDownDirect;
-    uint32_t at[kDown ? F : 2];
+    static constexpr bool kAcross = MODE == kRows;
+    uint32_t at[kAcross ? 2 : F];
 
     __device__ __forceinline__ void init(int first) {
         const int lane = threadIdx.x & (kWave - 1), j = lane & 15, g = lane >> 4;
-        if (kDown) {
+        if (!kAcross) {
             const int k = g * 8 + (j >> 2);
 #pragma unroll
             for (int f = 0; f < F; f++) at[f] = (uint32_t)(k * (B * 2) + ((first / 16 + f) ^ down_swizzle<B>(k)) * 32 + (j & 3) * 8);
         } else {
 #pragma unroll
-            for (int s = 0; s < 2; s++) at[s] = (uint32_t)((first + j) * 128 + ((g + 4 * s) ^ (j & 7)) * 16);
+            for (int s = 0; s < 2; s++) at[s] = (uint32_t)((first + j) * 128 + ((g + 4 * s) ^ (j >> 1 & 7)) * 16);
         }
     }
     // fragment f of the 32 k from 32 s on
     __device__ __forceinline__ u32x4 get(MQ_LDS char* lds, int s, int f) const {
-        if (kDown) {
+        if (!kAcross) {
             MQ_LDS char* from = lds + at[f] + s * (32 * B * 2);
             const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MQ_LDS s16x4*)from);
             const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MQ_LDS s16x4*)(from + 4 * B * 2));
@@ -216,6 +199,38 @@ struct Fragments {
             return u32x4{x.x, x.y, y.x, y.y};
         }
         return *(MQ_LDS const u32x4*)(lds + at[s] + f * 2048);
+    }
+};
+
+// The same for fragments of 32 outputs and 16 k, four of them along k in a step
+template <int MODE, int B, int F>
+struct WideFragments {
+    static constexpr bool kAcross = MODE == kRows;
+    uint32_t at[4];
+    static_assert(F == 4, "addresses for fragments, or for the parts of a step");
+
+    __device__ __forceinline__ void init(int first) {
+        const int lane = threadIdx.x & (kWave - 1);
+        if (!kAcross) {
+            const int j = lane & 15, g = lane >> 4, k = (g >> 1) * 8 + (j >> 2);
+#pragma unroll
+            for (int f = 0; f < F; f++) at[f] = (uint32_t)(k * (B * 2) + ((first / 16 + f * 2 + (g & 1)) ^ down_swizzle<B>(k)) * 32 + (j & 3) * 8);
+        } else {
+            const int j = lane & 31, g = lane >> 5;
+#pragma unroll
+            for (int h = 0; h < 4; h++) at[h] = (uint32_t)((first + j) * 128 + ((g + 2 * h) ^ (j >> 1 & 7)) * 16);
+        }
+    }
+    // fragment f of the 16 k from 16 h on
+    __device__ __forceinline__ u32x4 get(MQ_LDS char* lds, int h, int f) const {
+        if (!kAcross) {
+            MQ_LDS char* from = lds + at[f] + h * (16 * B * 2);
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MQ_LDS s16x4*)from);
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MQ_LDS s16x4*)(from + 4 * B * 2));
+            const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
+            return u32x4{x.x, x.y, y.x, y.y};
+        }
+        return *(MQ_LDS const u32x4*)(lds + at[h] + f * 4096);
     }
 };
 
@@ -265,172 +280,310 @@ __device__ __forceinline__ void add_bias4(const GemmArgs& a, int64_t col, float*
     z[3] += elem_hi<D == MQ_F16>(b.y);
 }
 
-// the tile of a workgroup: the eight XCDs take turns on the ids, so each is given a run of tiles of its own, and a run goes down four
-// tiles of q before it goes on along p, so that the 32 tiles that an XCD works on share their operands in its L2
-__device__ __forceinline__ void tile_of(const GemmArgs& a, int& tp, int& tq, int& split) {
-    const int tiles = a.tiles_p * a.tiles_q, total = (int)gridDim.x, id = (int)blockIdx.x;
-    const int xcd = id & 7, nth = id >> 3, per = total >> 3, more = total & 7;
-    int t = xcd * per + (xcd < more ? xcd : more) + nth;
-    split = t / tiles;
-    t -= split * tiles;
+// Where tile t lies: down four tiles of q before it goes on along p, so that the 32 tiles that an XCD works on share their operands
+// in its L2.
+__device__ __forceinline__ void place_of(const GemmArgs& a, int t, int& tp, int& tq) {
     const int band = 4 * a.tiles_p, b = t / band, in = t - b * band;
     const int high = a.tiles_q - b * 4 < 4 ? a.tiles_q - b * 4 : 4;
     tp = in / high;
     tq = b * 4 + in - tp * high;
 }
+// the tile and part of a workgroup: whole tiles first; the eight XCDs take turns on the ids, so each is given a run of tiles of its own
+__device__ __forceinline__ void tile_of(const GemmArgs& a, int& tile, int& part) {
+    const int id = (int)blockIdx.x, tail = id >= a.whole, total = tail ? (int)gridDim.x - a.whole : a.whole, mine = tail ? id - a.whole : id;
+    const int xcd = mine & 7, nth = mine >> 3, per = total >> 3, more = total & 7;
+    const int t = xcd * per + (xcd < more ? xcd : more) + nth;
+    tile = tail ? a.whole + t / a.splits : t;
+    part = tail ? t % a.splits : -1;
+}
+
+// every wavefront of the workgroup has come this far, with its reads and writes of shared memory done; nothing is moved across
+__device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
+// What follows the sums, from shared memory: 64 columns of ROWS rows of one wavefront, in fp32, four columns at position
+// (column / 4) ^ (row & 15) of a row's sixteen.  A lane has eight columns, so that eight lanes store whole lines.
+__device__ __forceinline__ int stage_at(int row, int four) { return row * 256 + ((four ^ (row & 15)) * 16); }
+
+template <int D, bool EPILOGUE, int ROWS>
+__device__ __forceinline__ void finish_block(const GemmArgs& a, float* sums, int pitch, int64_t row0, int64_t col0, MQ_LDS const char* stage) {
+    const int lane = threadIdx.x & (kWave - 1), mine = lane & 7;
+    const int64_t col = col0 + mine * 8;
+    if (!EPILOGUE || sums) {                               // sums: where a part's go, rows `pitch` apart
+        for (int r = lane >> 3; r < ROWS; r += 8) {
+            const int64_t row = row0 + r;
+            if (row >= a.nq) break;
+            const f32x4 lo = *(MQ_LDS const f32x4*)(stage + stage_at(r, 2 * mine)), hi = *(MQ_LDS const f32x4*)(stage + stage_at(r, 2 * mine + 1));
+            if (sums) {
+                f32x4* to = (f32x4*)(sums + r * pitch + mine * 8);
+                to[0] = lo;
+                to[1] = hi;
+            } else {
+                const float z[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                st_row<D>(a.out + row * a.np * 2, col, a.np, pack<D>(z));
+            }
+        }
+        return;
+    }
+    float bias[8];
+    if (a.bias) {
+        unpack<D>(ld_row<D>(a.bias, col, a.np), bias);
+    } else {
+#pragma unroll
+        for (int x = 0; x < 8; x++) bias[x] = 0.0f;
+    }
+    with_activation(a.act, [&](auto kind) {
+        constexpr int ACT = decltype(kind)::value;
+        for (int r = lane >> 3; r < ROWS; r += 8) {
+            const int64_t row = row0 + r;
+            if (row >= a.nq) break;                        // (the four lanes of 32 columns have one row)
+            const f32x4 lo = *(MQ_LDS const f32x4*)(stage + stage_at(r, 2 * mine)), hi = *(MQ_LDS const f32x4*)(stage + stage_at(r, 2 * mine + 1));
+            float z[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+            for (int x = 0; x < 8; x++) z[x] += bias[x];
+            if (a.zq) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int x = 0; x < 8; x++) m = umax(m, keep_magnitude(z[x]));
+                m = group_max4(m);
+                const uint32_t e = keep_exponent(m);
+                const float inv = e8m0_inverse(e);
+                if (col < a.np) {
+                    uint32_t* to = (uint32_t*)(a.zq + row * a.np + col);
+                    to[0] = keep_codes4(z[0], z[1], z[2], z[3], inv);
+                    to[1] = keep_codes4(z[4], z[5], z[6], z[7], inv);
+                    if ((lane & 3) == 0) a.zs[row * (a.np / 32) + col / 32] = (uint8_t)e;
+                }
+            }
+            if (a.z) st_row<D>(a.z + row * a.np * 2, col, a.np, pack<D>(z));
+#pragma unroll
+            for (int x = 0; x < 8; x++) z[x] = activate<ACT>(z[x]);
+            if (a.res) {
+                float f[8];
+                unpack<D>(ld_row<D>(a.res + row * a.ldr * 2, col, a.np), f);
+#pragma unroll
+                for (int x = 0; x < 8; x++) z[x] += f[x];
+            }
+            st_row<D>(a.out + row * a.np * 2, col, a.np, pack<D>(z));
+        }
+    });
+}
 
 template <int D, int PM, int QM, int BP, int BQ, int WP, int WQ, bool EPILOGUE>
-__global__ __launch_bounds__(WP* WQ* kWave) void gemm_kernel(const GemmArgs a) {
+__global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1))) void gemm_kernel(const GemmArgs a) {
     constexpr int kThreads = WP * WQ * kWave, TP = BP / WP, TQ = BQ / WQ, FP = TP / 16, FQ = TQ / 16;
     constexpr int kPBytes = BP * kStep * 2, kQBytes = BQ * kStep * 2, kBuffer = kPBytes + kQBytes;
-    __shared__ __attribute__((aligned(1024))) char shared[2 * kBuffer];
+    __shared__ __attribute__((aligned(1024))) char shared[BP == 256 ? 5 * kPBytes : 2 * kBuffer];
     MQ_LDS char* lds = (MQ_LDS char*)shared;
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
-    int tp, tq, split;
-    tile_of(a, tp, tq, split);
-    const int64_t p0 = (int64_t)tp * BP, q0 = (int64_t)tq * BQ, k0 = split * a.k_split;
-    const int64_t k1 = k0 + a.k_split < a.k ? k0 + a.k_split : a.k;
+    int tile, part, tp, tq;
+    tile_of(a, tile, part);
+    place_of(a, tile, tp, tq);
+    const int64_t p0 = (int64_t)tp * BP, q0 = (int64_t)tq * BQ, k0 = part < 0 ? 0 : part * a.k_split;
+    const int64_t k1 = part >= 0 && k0 + a.k_split < a.k ? k0 + a.k_split : a.k;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), wp = wave % WP, wq = wave / WP;
+    float* sums = part < 0 ? nullptr : a.ws + ((int64_t)(tile - a.whole) * a.splits + part) * (BP * BQ) + wq * TQ * BP + wp * TP;
     const int lane = threadIdx.x & (kWave - 1);
 
     Stage<PM, D, BP, kThreads> sp;
     Stage<QM, D, BQ, kThreads> sq;
     sp.init(a.p, a.ps, a.ldp, p0, a.np, k0);
     sq.init(a.q, nullptr, a.ldq, q0, a.nq, k0);
-    Fragments<PM, BP, FP> fp;
-    Fragments<QM, BQ, FQ> fq;
-    fp.init(wp * TP);
-    fq.init(wq * TQ);
-
-    f32x4 acc[FP][FQ];
+    const int steps = (int)((k1 - k0 + kStep - 1) / kStep);
+    const int span = (int)(k1 - k0);
+    auto left_of = [&](int t) { return span - t * kStep; };
+    // A step's pieces of one operand, on their way to buffer `to`.  The same number of accesses for every step, also behind the last
+    // (there they read nothing), so that a wavefront knows by counting which have arrived.
+    auto fetch_p = [&](int t, uint32_t to) {
+        const int left = left_of(t);
 #pragma unroll
-    for (int i = 0; i < FP; i++)
+        for (int u = 0; u < sp.kPieces; u++) sp.fetch_piece(u, to, left);
+        sp.advance();
+    };
+    auto fetch_q = [&](int t, uint32_t to) {
+        const int left = left_of(t);
 #pragma unroll
-        for (int j = 0; j < FQ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    if (k0 < k1) {
-        sp.fetch(lds0, k1 - k0);
-        sq.fetch(lds0 + kPBytes, k1 - k0);
-        sp.put(lds);
-        sq.put(lds + kPBytes);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    int now = 0;
-    for (int64_t k = k0; k < k1; k += kStep) {
-        const int next = now ^ kBuffer;                  // (the buffers lie at 0 and kBuffer)
-        const bool more = k + kStep < k1;
-        if (more) {
-            sp.fetch(lds0 + next, k1 - k - kStep);
-            sq.fetch(lds0 + next + kPBytes, k1 - k - kStep);
+        for (int u = 0; u < sq.kPieces; u++) sq.fetch_piece(u, to, left);
+        sq.advance();
+    };
+    auto put_p = [&](MQ_LDS char* to) {
+#pragma unroll
+        for (int u = 0; u < sp.kPieces; u++)
+#pragma unroll
+            for (int part = 0; part < 4; part++) sp.put_part(u, part, to);
+    };
+    constexpr bool kPDirect = PM != kDownKept;
+    static_assert(QM != kDownKept, "the first operand may be an 8-bit copy");
+    if constexpr (BP == 256) {
+        // One wavefront on each SIMD, 128 x 128 outputs each: four of them read half of what eight would from shared memory.  The
+        // next 16 k's fragments are read between the products of these.  Halfway through a step every wavefront has the rest of its
+        // fragments, so that its buffer is free for the step after the next three, and has seen its part of the next step arrive.
+        constexpr int F = 4;
+        WideFragments<PM, BP, F> fp;
+        WideFragments<QM, BQ, F> fq;
+        fp.init(wp * TP);
+        fq.init(wq * TQ);
+        f32x16 acc[F][F];
+#pragma unroll
+        for (int i = 0; i < F; i++)
+#pragma unroll
+            for (int j = 0; j < F; j++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) acc[i][j][x] = 0.0f;
+        // Five buffers of one operand of one step each, P and Q of the steps in turn: those of step t and t + 1, and P of step t + 2.
+        constexpr uint32_t kFifth = kPBytes, kAll = 5 * kFifth;
+        auto after = [&](uint32_t buffer, uint32_t by) { return buffer + by * kFifth >= kAll ? buffer + by * kFifth - kAll : buffer + by * kFifth; };
+        static_assert(BP == BQ && sq.kPieces == 8 && sp.kPieces == (kPDirect ? 8 : 4), "buffers of one size, a piece for every other product");
+        fetch_p(0, lds0);
+        put_p(lds);
+        fetch_q(0, lds0 + kFifth);
+        fetch_p(1, lds0 + 2 * kFifth);
+        put_p(lds + 2 * kFifth);
+        fetch_q(1, lds0 + 3 * kFifth);
+        if (kPDirect) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(sp.kUnits + sq.kUnits) : "memory");
+        else {
+            fetch_p(2, 0);                                  // (into registers)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
+        meet();
+        u32x4 p[2][F], q[2][F];
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            u32x4 p[FP], q[FQ];
-#pragma unroll
-            for (int i = 0; i < FP; i++) p[i] = fp.get(lds + now, s, i);
-#pragma unroll
-            for (int j = 0; j < FQ; j++) q[j] = fq.get(lds + now + kPBytes, s, j);
-#pragma unroll
-            for (int i = 0; i < FP; i++)
-#pragma unroll
-                for (int j = 0; j < FQ; j++) acc[i][j] = mfma<D>(p[i], q[j], acc[i][j]);
+        for (int i = 0; i < F; i++) {
+            p[0][i] = fp.get(lds, 0, i);
+            q[0][i] = fq.get(lds + kFifth, 0, i);
         }
-        if (more) {
-            sp.put(lds + next);
-            sq.put(lds + next + kPBytes);
-        }
-        // the next step's operands have arrived, and every wavefront is done with this step's, whose buffer is filled next
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        now = next;
-    }
-
-    const int64_t row0 = q0 + wq * TQ + (lane & 15), col0 = p0 + wp * TP + (lane >> 4) * 4;
-    if (a.ws) {
-        const int64_t ldw = (a.np + 3) / 4 * 4;
+        uint32_t at = 0;                                    // the buffer of P of step t
+        for (int t = 0; t < steps; t++) {
+            const uint32_t next = after(at, 2), third = after(at, 4);
+            const int left = left_of(t + 2), left_kept = left_of(t + 3);
+            // A wavefront issues an instruction in about four cycles and its product takes 32: what goes between two products is kept
+            // short, and the reads come first, so that they are back when the products that need them are due.
 #pragma unroll
-        for (int j = 0; j < FQ; j++) {
-            const int64_t row = row0 + j * 16;
-            if (row >= a.nq) continue;
-            float* to = a.ws + ((int64_t)split * a.nq + row) * ldw;
-#pragma unroll
-            for (int i = 0; i < FP; i++) {
-                const int64_t col = col0 + i * 16;
-                if (col < a.np) *(f32x4*)(to + col) = acc[i][j];
-            }
-        }
-        return;
-    }
-    if (!EPILOGUE) {
-#pragma unroll
-        for (int j = 0; j < FQ; j++) {
-            const int64_t row = row0 + j * 16;
-            if (row >= a.nq) continue;
-#pragma unroll
-            for (int i = 0; i < FP; i++)
-                st4_row(a.out + row * a.np * 2, col0 + i * 16, a.np, u32x2{pack2<D>(acc[i][j][0], acc[i][j][1]), pack2<D>(acc[i][j][2], acc[i][j][3])});
-        }
-        return;
-    }
-    with_activation(a.act, [&](auto kind) {
-        constexpr int ACT = decltype(kind)::value;
-#pragma unroll
-        for (int i = 0; i < FP; i += 2) {
-#pragma unroll
-            for (int j = 0; j < FQ; j++) {
-                const int64_t row = row0 + j * 16;
-                float z[2][4];
-                uint32_t m = 0;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-#pragma unroll
-                    for (int x = 0; x < 4; x++) z[h][x] = acc[i + h][j][x];
-                    add_bias4<D>(a, col0 + (i + h) * 16, z[h]);
-#pragma unroll
-                    for (int x = 0; x < 4; x++) m = umax(m, keep_magnitude(z[h][x]));
+            for (int h = 0; h < 4; h++) {
+                if (h == 3) {
+                    // this step's fragments are all in registers and so its buffers are free; the next step's operands have arrived,
+                    // whose last pieces were asked for a step ago (P of step t + 2 may still be on its way)
+                    if (kPDirect) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(sp.kUnits) : "memory");
+                    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    meet();
                 }
-                if (a.zq) {                              // 32 columns: two fragments of the four lanes with this row
-                    m = umax(m, (uint32_t)__shfl_xor((int)m, 16));
-                    m = umax(m, (uint32_t)__shfl_xor((int)m, 32));
-                    const uint32_t e = keep_exponent(m);
-                    const float inv = e8m0_inverse(e);
-                    if (row < a.nq && col0 + i * 16 < a.np) {
-                        uint8_t* to = a.zq + row * a.np + col0 + i * 16;
-                        *(uint32_t*)to = keep_codes4(z[0][0], z[0][1], z[0][2], z[0][3], inv);
-                        *(uint32_t*)(to + 16) = keep_codes4(z[1][0], z[1][1], z[1][2], z[1][3], inv);
-                        if (lane < 16) a.zs[row * (a.np / 32) + (col0 + i * 16) / 32] = (uint8_t)e;
+                MQ_LDS char* fromp = lds + (h == 3 ? next : at);
+                MQ_LDS char* fromq = lds + (h == 3 ? after(next, 1) : after(at, 1));
+#pragma unroll
+                for (int m = 0; m < F * F; m++) {
+                    acc[m / F][m % F] = mfma<D>(p[h & 1][m / F], q[h & 1][m % F], acc[m / F][m % F]);
+                    if (m < F) p[h & 1 ^ 1][m] = fp.get(fromp, h + 1 & 3, m);
+                    else if (m < 2 * F) q[h & 1 ^ 1][m - F] = fq.get(fromq, h + 1 & 3, m - F);
+                    else if (kPDirect && h < 2) {            // P of step t + 2, eight pieces in two parts of this step
+                        if (m % 2 == 0) sp.fetch_piece((m - 8) / 2 + h * 4, lds0 + third, left);
+                    } else if (!kPDirect && h < 2) {         // or its registers are written out, in sixteen parts
+                        sp.put_part((m - 8) / 4 + h * 2, m % 4, lds + third);
+                    } else if (h == 3) {
+                        sq.fetch_piece(m - 8, lds0 + at, left);
                     }
-                }
-                if (row < a.nq) {
-                    finish4<D, ACT>(a, row, col0 + i * 16, z[0]);
-                    finish4<D, ACT>(a, row, col0 + (i + 1) * 16, z[1]);
+                    if (!kPDirect && h == 3 && m < 8 && m % 2 == 0) sp.fetch_piece(m / 2, 0, left_kept);      // and filled again
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
+            sp.advance();
+            sq.advance();
+            at = next;
         }
-    });
+        // nothing may reach this shared memory when it is another workgroup's
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        meet();
+        MQ_LDS char* stage = lds + wave * (TQ * 256);
+        const int row = lane & 31, four = lane >> 5;        // a lane has sixteen columns of a row, fours that are eight apart
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < F; j++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const f32x16& c = acc[2 * half + i][j];
+                        *(MQ_LDS f32x4*)(stage + stage_at(j * 32 + row, i * 8 + x * 2 + four)) = f32x4{c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3]};
+                    }
+            finish_block<D, EPILOGUE, TQ>(a, sums ? sums + half * 64 : nullptr, BP, q0 + wq * TQ, p0 + wp * TP + half * 64, stage);
+        }
+    } else {
+        Fragments<PM, BP, FP> fp;
+        Fragments<QM, BQ, FQ> fq;
+        fp.init(wp * TP);
+        fq.init(wq * TQ);
+        f32x4 acc[FP][FQ];
+#pragma unroll
+        for (int i = 0; i < FP; i++)
+#pragma unroll
+            for (int j = 0; j < FQ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        // Several workgroups on a compute unit, two buffers each.  While step t is worked on, step t + 1 is on its way; what goes through
+        // registers was loaded a step earlier.
+        fetch_p(0, lds0);
+        fetch_q(0, lds0 + kPBytes);
+        put_p(lds);
+        if (!kPDirect) fetch_p(1, 0);
+        for (int t = 0; t < steps; t++) {
+            MQ_LDS char* from = lds + (t & 1) * kBuffer;
+            const uint32_t next = (uint32_t)(t + 1 & 1) * kBuffer;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            meet();
+            fetch_q(t + 1, lds0 + next + kPBytes);
+            if (kPDirect) {
+                fetch_p(t + 1, lds0 + next);
+            } else {
+                put_p(lds + next);
+                fetch_p(t + 2, 0);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                u32x4 p[FP], q[FQ];
+#pragma unroll
+                for (int i = 0; i < FP; i++) p[i] = fp.get(from, h, i);
+#pragma unroll
+                for (int j = 0; j < FQ; j++) q[j] = fq.get(from + kPBytes, h, j);
+#pragma unroll
+                for (int i = 0; i < FP; i++)
+#pragma unroll
+                    for (int j = 0; j < FQ; j++) acc[i][j] = mfma<D>(p[i], q[j], acc[i][j]);
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // (as above)
+        meet();
+        MQ_LDS char* stage = lds + wave * (TQ * 256);
+        static_assert(TP == 64, "one block of columns");
+#pragma unroll
+        for (int i = 0; i < FP; i++)
+#pragma unroll
+            for (int j = 0; j < FQ; j++) *(MQ_LDS f32x4*)(stage + stage_at(j * 16 + (lane & 15), i * 4 + (lane >> 4))) = acc[i][j];
+        finish_block<D, EPILOGUE, TQ>(a, sums, BP, q0 + wq * TQ, p0 + wp * TP, stage);
+    }
 }
 
 // ---- the host's side ---------------------------------------------------------------------------------------------------------
 enum { kTileLarge = 0, kTileMiddle = 1, kTileLow = 2 };       // 256 x 256, 128 x 128, 128 (p) x 64 (q)
 struct GemmPlan {
-    int tile, splits;
+    int tile, tiles_p, tiles_q, whole, splits;
     int64_t k_split;
 };
+constexpr int kTileP[3] = {256, 128, 128}, kTileQ[3] = {256, 128, 64};
 
 template <int D, int PM, int QM, bool EPILOGUE>
 int gemm_launch(GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
-    a.ws = plan.splits > 1 ? ws : nullptr;
+    a.ws = ws;
     a.k_split = plan.k_split;
-    const int bp = plan.tile == kTileLarge ? 256 : 128, bq = plan.tile == kTileLarge ? 256 : plan.tile == kTileMiddle ? 128 : 64;
-    a.tiles_p = (int)((a.np + bp - 1) / bp);
-    a.tiles_q = (int)((a.nq + bq - 1) / bq);
-    const dim3 grid((unsigned)((int64_t)a.tiles_p * a.tiles_q * plan.splits));
-    constexpr bool kBounded = PM == kRowsAny || PM == kDownAny || QM == kRowsAny || QM == kDownAny;
-    if constexpr (kBounded) {
-        hipLaunchKernelGGL((gemm_kernel<D, PM, QM, 128, 128, 2, 2, EPILOGUE>), grid, dim3(256), 0, st, a);
-    } else if (plan.tile == kTileLarge) {
-        hipLaunchKernelGGL((gemm_kernel<D, PM, QM, 256, 256, 2, 4, EPILOGUE>), grid, dim3(512), 0, st, a);
+    a.tiles_p = plan.tiles_p;
+    a.tiles_q = plan.tiles_q;
+    a.whole = plan.whole;
+    a.splits = plan.splits;
+    const dim3 grid((unsigned)(plan.whole + (plan.tiles_p * plan.tiles_q - plan.whole) * plan.splits));
+    if (plan.tile == kTileLarge) {
+        hipLaunchKernelGGL((gemm_kernel<D, PM, QM, 256, 256, 2, 2, EPILOGUE>), grid, dim3(256), 0, st, a);
     } else if (plan.tile == kTileMiddle) {
         hipLaunchKernelGGL((gemm_kernel<D, PM, QM, 128, 128, 2, 2, EPILOGUE>), grid, dim3(256), 0, st, a);
     } else {
@@ -442,6 +595,6 @@ int gemm_launch(GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
 }  // namespace mq
 
 // the three products, each in a file of its own: launched as planned, the partial sums of several splits left in ws
-int mq_gemm_forward(int dtype, bool bounded, mq::GemmArgs& a, const mq::GemmPlan& plan, float* ws, hipStream_t st);
-int mq_gemm_input_grad(int dtype, bool bounded, mq::GemmArgs& a, const mq::GemmPlan& plan, float* ws, hipStream_t st);
-int mq_gemm_weight_grad(int dtype, bool bounded, mq::GemmArgs& a, const mq::GemmPlan& plan, float* ws, hipStream_t st);
+int mq_gemm_forward(int dtype, mq::GemmArgs& a, const mq::GemmPlan& plan, float* ws, hipStream_t st);
+int mq_gemm_input_grad(int dtype, mq::GemmArgs& a, const mq::GemmPlan& plan, float* ws, hipStream_t st);
+int mq_gemm_weight_grad(int dtype, mq::GemmArgs& a, const mq::GemmPlan& plan, float* ws, hipStream_t st);

@@ -3,10 +3,6 @@
 
 using namespace mq;
 
-template <int D>
-static int forward(bool bounded, GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
-    return bounded ? gemm_launch<D, kRowsAny, kRowsAny, true>(a, plan, ws, st) : gemm_launch<D, kRowsDirect, kRowsDirect, true>(a, plan, ws, st);
-}
-int mq_gemm_forward(int dtype, bool bounded, GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
-    return dtype == MQ_F16 ? forward<MQ_F16>(bounded, a, plan, ws, st) : forward<MQ_BF16>(bounded, a, plan, ws, st);
+int mq_gemm_forward(int dtype, GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
+    return dtype == MQ_F16 ? gemm_launch<MQ_F16, kRows, kRows, true>(a, plan, ws, st) : gemm_launch<MQ_BF16, kRows, kRows, true>(a, plan, ws, st);
 }

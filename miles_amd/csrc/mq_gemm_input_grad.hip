@@ -3,10 +3,6 @@
 
 using namespace mq;
 
-template <int D>
-static int input_grad(bool bounded, GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
-    return bounded ? gemm_launch<D, kDownAny, kRowsAny, false>(a, plan, ws, st) : gemm_launch<D, kDownDirect, kRowsDirect, false>(a, plan, ws, st);
-}
-int mq_gemm_input_grad(int dtype, bool bounded, GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
-    return dtype == MQ_F16 ? input_grad<MQ_F16>(bounded, a, plan, ws, st) : input_grad<MQ_BF16>(bounded, a, plan, ws, st);
+int mq_gemm_input_grad(int dtype, GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
+    return dtype == MQ_F16 ? gemm_launch<MQ_F16, kDown, kRows, false>(a, plan, ws, st) : gemm_launch<MQ_BF16, kDown, kRows, false>(a, plan, ws, st);
 }

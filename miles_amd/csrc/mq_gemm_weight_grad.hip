@@ -5,10 +5,9 @@
 using namespace mq;
 
 template <int D>
-static int weight_grad(bool bounded, GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
-    if (a.ps) return bounded ? gemm_launch<D, kDownKept, kDownAny, false>(a, plan, ws, st) : gemm_launch<D, kDownKept, kDownDirect, false>(a, plan, ws, st);
-    return bounded ? gemm_launch<D, kDownAny, kDownAny, false>(a, plan, ws, st) : gemm_launch<D, kDownDirect, kDownDirect, false>(a, plan, ws, st);
+static int weight_grad(GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
+    return a.ps ? gemm_launch<D, kDownKept, kDown, false>(a, plan, ws, st) : gemm_launch<D, kDown, kDown, false>(a, plan, ws, st);
 }
-int mq_gemm_weight_grad(int dtype, bool bounded, GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
-    return dtype == MQ_F16 ? weight_grad<MQ_F16>(bounded, a, plan, ws, st) : weight_grad<MQ_BF16>(bounded, a, plan, ws, st);
+int mq_gemm_weight_grad(int dtype, GemmArgs& a, const GemmPlan& plan, float* ws, hipStream_t st) {
+    return dtype == MQ_F16 ? weight_grad<MQ_F16>(a, plan, ws, st) : weight_grad<MQ_BF16>(a, plan, ws, st);
 }

@@ -5,18 +5,21 @@ int mq_column_sum_launch(const float* p0, void* out0, const float* p1, void* out
 
 namespace mq {
 
-// The sums of a product's splits, in their order, and what follows them.  Four columns a lane; the eight lanes of 32 columns are
-// neighbours, because a row's units are counted in fours of eight.
+// The sums of the parts of the tiles that were cut along k, in the parts' order, and what follows them.  Four columns a lane; the eight
+// lanes of 32 columns are neighbours.
 template <int D>
-__global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs a, int splits) {
-    const int64_t per_row = (a.np + 31) / 32 * 8, ldw = (a.np + 3) / 4 * 4;
-    const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, row = unit / per_row, col = (unit - row * per_row) * 4;
+__global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs a, int bp, int bq) {
+    const int units = bp * bq / 4, blocks = units / 256, nth = (int)blockIdx.x / blocks, unit = ((int)blockIdx.x - nth * blocks) * 256 + (int)threadIdx.x;
+    int tp, tq;
+    place_of(a, a.whole + nth, tp, tq);
+    const int r = unit / (bp / 4), c = (unit - r * (bp / 4)) * 4;
+    const int64_t row = (int64_t)tq * bq + r, col = (int64_t)tp * bp + c;
     const bool inside = row < a.nq && col < a.np;
     float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (inside) {
-        const float* from = a.ws + row * ldw + col;
-        for (int s = 0; s < splits; s++) {
-            const f32x4 v = *(const f32x4*)(from + (int64_t)s * a.nq * ldw);
+        const float* from = a.ws + (int64_t)nth * a.splits * bp * bq + r * bp + c;
+        for (int s = 0; s < a.splits; s++) {
+            const f32x4 v = *(const f32x4*)(from + (int64_t)s * bp * bq);
 #pragma unroll
             for (int i = 0; i < 4; i++) z[i] += v[i];
         }
@@ -34,6 +37,82 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs a, int sp
         }
     }
     if (inside) with_activation(a.act, [&](auto kind) { finish4<D, decltype(kind)::value>(a, row, col, z); });
+}
+
+// Operands whose rows do not begin at multiples of 16 bytes, or do not end with a whole piece of eight elements, copied so that they do,
+// zeros behind a row's end; blockIdx.y: which of the two.
+struct PadArgs {
+    const char* from[2];
+    char* to[2];
+    int64_t rows[2], cols[2], ld[2];
+};
+__global__ __launch_bounds__(256) void pad_rows_kernel(const PadArgs a) {
+    const int which = blockIdx.y;
+    if (!a.to[which]) return;
+    const int64_t per_row = (a.cols[which] + 7) / 8, units = a.rows[which] * per_row;
+    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += (int64_t)gridDim.x * 256) {
+        const int64_t row = u / per_row, c = (u - row * per_row) * 8;
+        *(u32x4*)(a.to[which] + u * 16) = ld_row<MQ_BF16>(a.from[which] + row * a.ld[which] * 2, c, a.cols[which]);
+    }
+}
+
+// A few tokens (nq <= 16): what counts is reading the weight once, as fast as memory gives it.  A wavefront has 16 rows of the weight and
+// a share of k; its loads go straight into the operands of the matrix instruction (a lane's 16 elements of each 64 are neighbours, in
+// both operands, so that one load touches whole lines), and the eight wavefronts' sums meet in shared memory.
+struct FewArgs {
+    GemmArgs g;
+    int64_t k_wave;            // k of a wavefront, a multiple of 64
+};
+constexpr int kFewWaves = 8;
+template <int D>
+__global__ __launch_bounds__(kFewWaves * kWave) void few_rows_kernel(const FewArgs f) {
+    const GemmArgs& a = f.g;
+    __shared__ float sums[kFewWaves][16][17];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, j = lane & 15, g = lane >> 4;
+    const int64_t p0 = (int64_t)blockIdx.x * 16;
+    const int64_t k0 = wave * f.k_wave < a.k ? wave * f.k_wave : a.k, k1 = k0 + f.k_wave < a.k ? k0 + f.k_wave : a.k;
+    const char* p = a.p + (p0 + j < a.np ? p0 + j : a.np - 1) * a.ldp * 2;
+    const char* q = a.q + (j < a.nq ? j : a.nq - 1) * a.ldq * 2;
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    int64_t k = k0;
+    constexpr int kAhead = 4;                              // loads of 64 k at once
+    for (; k + 64 * kAhead <= k1; k += 64 * kAhead) {
+        u32x4 vp[kAhead][2], vq[kAhead][2];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                vp[i][h] = ld16_at2(p + (k + i * 64 + g * 16 + h * 8) * 2);
+                vq[i][h] = ld16_at2(q + (k + i * 64 + g * 16 + h * 8) * 2);
+            }
+#pragma unroll
+        for (int i = 0; i < kAhead; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) acc = mfma<D>(vp[i][h], vq[i][h], acc);
+    }
+    for (; k < k1; k += 64) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int64_t c = k + g * 16 + h * 8;
+            acc = mfma<D>(ld_row<D>(p, c, k1), ld_row<D>(q, c, k1), acc);
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < 4; x++) sums[wave][j][g * 4 + x] = acc[x];
+    __syncthreads();
+    const int row = threadIdx.x / 16, c = threadIdx.x % 16;
+    if (row < a.nq && p0 + c < a.np) {                     // (rows 16 and on are no rows)
+        float z = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kFewWaves; w++) z += sums[w][row][c];
+        const int64_t at = row * a.np + p0 + c;
+        if (a.bias) z += one_elem<D>(a.bias, p0 + c);
+        if (a.z) store_dtype(a.z, at, z, D);
+        float y = z;
+        with_activation(a.act, [&](auto kind) { y = activate<decltype(kind)::value>(z); });
+        if (a.res) y += one_elem<D>(a.res, row * a.ldr + p0 + c);
+        store_dtype(a.out, at, y, D);
+    }
 }
 
 struct ActGradArgs {
@@ -101,130 +180,192 @@ __global__ __launch_bounds__(256) void activation_bwd_kernel(const ActGradArgs a
 
 using namespace mq;
 
-// How a product of np columns, nq rows and k runs: the tile, and into how many splits k is cut so that every compute unit has work.
-// Each candidate's time is estimated from the rounds of workgroups that it takes and the bytes of its partial sums.
-static GemmPlan gemm_plan(int64_t np, int64_t nq, int64_t k, bool bounded) {
-    struct Tile {
-        int bp, bq, per_cu;
-        double step_us;                                   // of one step of one workgroup, with per_cu of them on a compute unit
+// How a product of np columns, nq rows and k runs: the tile, and which tiles are cut along k.  Tiles that fill every place on the card
+// run whole, round by round; those of a last round that would leave places empty (all of them, of a small product) are cut into as
+// many parts as fill it.  Each candidate's time is estimated from its rounds and the bytes of its partial sums; the constants were
+// fitted to 40 products measured with every tile and up to ten numbers of parts, where the choice loses 2 % against the best.
+static GemmPlan gemm_plan(int64_t np, int64_t nq, int64_t k) {
+    struct Cost {
+        int per_cu;
+        double least_us, step_us, tile_us;                // of a step, of a step for each workgroup on the compute unit, and besides the steps
     };
-    static const Tile tiles[3] = {{256, 256, 1, 1.25}, {128, 128, 2, 0.85}, {128, 64, 3, 0.7}};
-    const int64_t steps = (k + kStep - 1) / kStep;
-    GemmPlan best{kTileMiddle, 1, (steps > 0 ? steps : 1) * kStep};
+    static const Cost costs[3] = {{1, 0.79, 0.93, 8.5}, {2, 0.68, 0.48, 3.2}, {3, 0.49, 0.34, 1.6}};
+    const int64_t steps = k > 0 ? (k + kStep - 1) / kStep : 1;
+    GemmPlan best{};
     double best_us = 1e30;
-    for (int t = bounded ? kTileMiddle : kTileLarge; t <= (bounded ? kTileMiddle : kTileLow); t++) {
-        const Tile& tile = tiles[t];
-        const double count = (double)((np + tile.bp - 1) / tile.bp) * (double)((nq + tile.bq - 1) / tile.bq);
-        for (int splits = 1; splits <= 64; splits = splits < 4 ? splits + 1 : splits + splits / 2) {
+    for (int t = kTileLarge; t <= kTileLow; t++) {
+        const Cost& cost = costs[t];
+        const int64_t tiles_p = (np + kTileP[t] - 1) / kTileP[t], tiles_q = (nq + kTileQ[t] - 1) / kTileQ[t];
+        const int64_t tiles = tiles_p * tiles_q, places = 256 * cost.per_cu, rest = tiles % places;
+        auto round_us = [&](int64_t count, int64_t n_steps) {      // so many workgroups at once, of so many steps
+            const double step = cost.step_us * (double)((count + 255) / 256);
+            return (double)n_steps * (step > cost.least_us ? step : cost.least_us) + cost.tile_us;
+        };
+        const double whole_us = (double)(tiles / places) * round_us(places, steps);
+        for (int64_t splits = 1; splits <= 64; splits++) {
             const int64_t per = (steps + splits - 1) / splits;
-            const int real = per > 0 ? (int)((steps + per - 1) / per) : 1;
-            if (splits > 1 && (real != splits || per < 4)) continue;
-            const double slots = 256.0 * tile.per_cu, rounds = (double)(int64_t)((count * real + slots - 1) / slots);
-            double us = 3.0 + rounds * ((double)per * tile.step_us + 3.0);
-            if (real > 1) us += 4.0 + (double)real * np * nq * 8 / 4e6;
+            if (splits > 1 && (rest == 0 || per < 2 || (steps + per - 1) / per != splits)) continue;
+            const int64_t parts = rest * splits;
+            double us = whole_us + (double)(parts / places) * round_us(places, per);
+            if (parts % places) us += round_us(parts % places, per);
+            if (splits > 1) us += 2.5 + (double)parts * kTileP[t] * (double)(nq < kTileQ[t] ? nq : kTileQ[t]) * 8 / 6.4e6;
             if (us < best_us) {
                 best_us = us;
-                best = GemmPlan{t, real, per * kStep};
+                best = GemmPlan{t, (int)tiles_p, (int)tiles_q, (int)(splits > 1 ? tiles - rest : tiles), (int)splits, per * kStep};
             }
         }
     }
     return best;
 }
+static int64_t partial_floats(const GemmPlan& plan) {
+    return (int64_t)(plan.tiles_p * plan.tiles_q - plan.whole) * plan.splits * kTileP[plan.tile] * kTileQ[plan.tile];
+}
 
 static bool direct_ok(const void* p, int64_t ld, int64_t cols) {
     return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && cols % 8 == 0 && ld < (1 << 22);
 }
-static int check_sizes(int dtype, int64_t M, int64_t N, int64_t K) {
-    if (dtype != MQ_BF16 && dtype != MQ_F16) return mq_fail(MQ_ERR_ARG, "linear: bf16 or fp16");
-    if (M < 0 || N < 0 || K < 0) return mq_fail(MQ_ERR_ARG, "linear: bad argument");
-    if (M > 0x7FFFFF00 || N > 0x7FFFFF00 || K > 0x7FFFFF00) return mq_fail(MQ_ERR_ARG, "linear: tensor too large");
-    return MQ_OK;
-}
-static int check_rows(int64_t rows, int64_t cols, int64_t ld) {
-    return rows > 1 && ld < cols ? mq_fail(MQ_ERR_ARG, "linear: rows overlap") : MQ_OK;
-}
-static int check_grid(const GemmPlan& plan, int64_t np, int64_t nq) {
-    return ((np + 127) / 128) * ((nq + 63) / 64) * plan.splits > 0x7FFFFFF0 ? mq_fail(MQ_ERR_ARG, "linear: tensor too large") : MQ_OK;
-}
-// joins the splits, if there are any
+// joins the parts, if there are any
 static int join(int dtype, const GemmArgs& a, const GemmPlan& plan, hipStream_t st) {
-    if (plan.splits > 1) {
-        const int64_t blocks = (a.nq * ((a.np + 31) / 32 * 8) + 255) / 256;
-        if (dtype == MQ_F16) hipLaunchKernelGGL(gemm_join_kernel<MQ_F16>, dim3((unsigned)blocks), dim3(256), 0, st, a, plan.splits);
-        else hipLaunchKernelGGL(gemm_join_kernel<MQ_BF16>, dim3((unsigned)blocks), dim3(256), 0, st, a, plan.splits);
+    const int cut = plan.tiles_p * plan.tiles_q - plan.whole, bp = kTileP[plan.tile], bq = kTileQ[plan.tile];
+    if (cut > 0) {
+        const dim3 grid((unsigned)(cut * (bp * bq / 1024)));
+        if (dtype == MQ_F16) hipLaunchKernelGGL(gemm_join_kernel<MQ_F16>, grid, dim3(256), 0, st, a, bp, bq);
+        else hipLaunchKernelGGL(gemm_join_kernel<MQ_BF16>, grid, dim3(256), 0, st, a, bp, bq);
     }
     return mq_check_launch("linear");
 }
 
-extern "C" int mq_linear_workspace(int product, int64_t M, int64_t N, int64_t K, int64_t* floats) {
-    if (!floats || product < MQ_LINEAR_FORWARD || product > MQ_LINEAR_WEIGHT_GRAD || M < 0 || N < 0 || K < 0) return mq_fail(MQ_ERR_ARG, "linear: bad argument");
-    const int64_t np = product == MQ_LINEAR_FORWARD ? N : K, nq = product == MQ_LINEAR_WEIGHT_GRAD ? N : M;
-    const int64_t k = product == MQ_LINEAR_FORWARD ? K : product == MQ_LINEAR_INPUT_GRAD ? N : M;
-    *floats = 0;
-    for (int bounded = 0; bounded < 2; bounded++) {
-        const GemmPlan plan = gemm_plan(np, nq, k, bounded != 0);
-        const int64_t need = plan.splits > 1 ? plan.splits * nq * ((np + 3) / 4 * 4) : 0;
-        if (need > *floats) *floats = need;
+// A product as it is run: sizes and operands (P the first, p_rows x p_cols in memory), and what of the workspace is whose.
+struct Product {
+    const void *p, *q;
+    int64_t ldp, ldq, p_rows, p_cols, q_rows, q_cols, np, nq, k;
+    bool kept, few;
+    GemmPlan plan;
+    int64_t p_at, q_at, bytes;     // where the operands' copies are, -1 for none
+
+    Product(int product, const void* a, int64_t lda, const void* b, int64_t ldb, bool kept_, bool few_, int64_t M, int64_t N, int64_t K)
+        : p(b), q(a), ldp(ldb), ldq(lda), kept(kept_), few(few_) {
+        const bool weight_grad = product == MQ_LINEAR_WEIGHT_GRAD, forward = product == MQ_LINEAR_FORWARD;
+        p_rows = weight_grad ? M : N, p_cols = K;
+        q_rows = M, q_cols = forward ? K : N;
+        np = forward ? N : K, nq = weight_grad ? N : M, k = forward ? K : weight_grad ? M : N;
+        plan = few ? GemmPlan{} : gemm_plan(np, nq, k);
+        bytes = few ? 0 : partial_floats(plan) * 4;
+        p_at = few || kept ? -1 : copy_at(p, ldp, p_rows, p_cols);
+        q_at = few ? -1 : copy_at(q, ldq, q_rows, q_cols);
     }
+    int64_t copy_at(const void* at, int64_t ld, int64_t rows, int64_t cols) {
+        if (direct_ok(at, rows > 1 ? ld : 8, cols)) return -1;
+        const int64_t here = bytes;
+        bytes += rows * ((cols + 7) / 8 * 8) * 2;          // (a multiple of 16)
+        return here;
+    }
+    // the arguments, with the operands copied into the workspace where that is needed
+    int arguments(GemmArgs& a, char* ws, hipStream_t st) const {
+        if (bytes > 0 && (!ws || (uintptr_t)ws % 16)) return mq_fail(MQ_ERR_ARG, "linear: a 16-byte aligned workspace is needed");
+        a.p = (const char*)p, a.q = (const char*)q, a.ldp = ldp, a.ldq = ldq, a.np = np, a.nq = nq, a.k = k;
+        PadArgs pad{};
+        int64_t units = 0;
+        auto copy = [&](int i, const char*& operand, int64_t& ld, int64_t at, int64_t rows, int64_t cols) {
+            if (at < 0) return;
+            pad.from[i] = operand, pad.ld[i] = ld, pad.rows[i] = rows, pad.cols[i] = cols, pad.to[i] = ws + at;
+            operand = ws + at, ld = (cols + 7) / 8 * 8;
+            const int64_t n = rows * (ld / 8);
+            if (n > units) units = n;
+        };
+        copy(0, a.p, a.ldp, p_at, p_rows, p_cols);
+        copy(1, a.q, a.ldq, q_at, q_rows, q_cols);
+        if (units > 0) {
+            const int64_t blocks = (units + 255) / 256;
+            hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), 2), dim3(256), 0, st, pad);
+        }
+        return MQ_OK;
+    }
+};
+// few tokens, and nothing that needs 32 columns at once
+static bool few_rows(int product, int64_t M, bool z8) { return product == MQ_LINEAR_FORWARD && M <= 16 && !z8; }
+
+static int check_product(int product, const void* a, int64_t lda, const void* b, int64_t ldb, bool kept, int64_t M, int64_t N, int64_t K) {
+    if (M < 0 || N < 0 || K < 0) return mq_fail(MQ_ERR_ARG, "linear: bad argument");
+    // (a lane's offsets into 256 rows of an operand are 32-bit numbers)
+    if (M > 0x7FFFFF00 || N >= 1 << 22 || K >= 1 << 22) return mq_fail(MQ_ERR_ARG, "linear: tensor too large");
+    const bool forward = product == MQ_LINEAR_FORWARD, weight_grad = product == MQ_LINEAR_WEIGHT_GRAD;
+    if ((M > 1 && lda < (forward ? K : N)) || (!kept && (weight_grad ? M : N) > 1 && ldb < K)) return mq_fail(MQ_ERR_ARG, "linear: rows overlap");
+    const int64_t np = forward ? N : K, nq = weight_grad ? N : M;
+    if (((np + 127) / 128) * ((nq + 63) / 64) > 0x7FFFFF) return mq_fail(MQ_ERR_ARG, "linear: tensor too large");
+    return MQ_OK;
+}
+static int check_dtype(int dtype) { return dtype != MQ_BF16 && dtype != MQ_F16 ? mq_fail(MQ_ERR_ARG, "linear: bf16 or fp16") : MQ_OK; }
+
+extern "C" int mq_linear_workspace(int product, const void* a, int64_t lda, const void* b, int64_t ldb, int kept8, int64_t M, int64_t N, int64_t K,
+                                   int64_t* bytes) {
+    if (!bytes || product < MQ_LINEAR_FORWARD || product > MQ_LINEAR_WEIGHT_GRAD) return mq_fail(MQ_ERR_ARG, "linear: bad argument");
+    const bool kept = product == MQ_LINEAR_WEIGHT_GRAD && kept8;
+    if (const int rc = check_product(product, a, lda, b, ldb, kept, M, N, K)) return rc;
+    *bytes = 0;
+    if ((product != MQ_LINEAR_WEIGHT_GRAD && M == 0) || (product != MQ_LINEAR_INPUT_GRAD && N == 0) || (product != MQ_LINEAR_FORWARD && K == 0)) return MQ_OK;
+    *bytes = Product(product, a, lda, b, ldb, kept, few_rows(product, M, kept8 != 0), M, N, K).bytes;
     return MQ_OK;
 }
 
 extern "C" int mq_linear_forward(const void* x, int dtype, int64_t ldx, const void* weight, int64_t ldw, const void* bias, int act,
                                  const void* residual, int64_t ldr, void* y, void* z, void* z8, uint8_t* z8_scale, int64_t M, int64_t N,
-                                 int64_t K, float* ws, void* stream) {
-    if (const int rc = check_sizes(dtype, M, N, K)) return rc;
+                                 int64_t K, void* ws, void* stream) {
+    if (const int rc = check_dtype(dtype)) return rc;
+    if (const int rc = check_product(MQ_LINEAR_FORWARD, x, ldx, weight, ldw, false, M, N, K)) return rc;
     if (act < MQ_ACT_NONE || act > MQ_ACT_GELU_TANH) return mq_fail(MQ_ERR_ARG, "linear: unknown activation");
-    if (check_rows(M, K, ldx) || check_rows(N, K, ldw) || (residual && check_rows(M, N, ldr))) return MQ_ERR_ARG;
+    if (residual && M > 1 && ldr < N) return mq_fail(MQ_ERR_ARG, "linear: rows overlap");
     if (M == 0 || N == 0) return MQ_OK;
     if (!y || (K > 0 && (!x || !weight)) || !z8 != !z8_scale) return mq_fail(MQ_ERR_ARG, "linear: null pointer");
     if (z8 && (N % 32 != 0 || (uintptr_t)z8 % 4)) return mq_fail(MQ_ERR_ARG, "linear: columns kept in 8 bits are a multiple of 32, 4-byte aligned");
-    const bool bounded = !direct_ok(x, M > 1 ? ldx : 8, K) || !direct_ok(weight, N > 1 ? ldw : 8, K);
-    const GemmPlan plan = gemm_plan(N, M, K, bounded);
-    if (const int rc = check_grid(plan, N, M)) return rc;
-    if (plan.splits > 1 && (!ws || (uintptr_t)ws % 16)) return mq_fail(MQ_ERR_ARG, "linear: a 16-byte aligned workspace is needed");
-    GemmArgs a{};
-    a.p = (const char*)weight, a.q = (const char*)x, a.ldp = ldw, a.ldq = ldx, a.np = N, a.nq = M, a.k = K;
+    const hipStream_t st = (hipStream_t)stream;
+    const Product product(MQ_LINEAR_FORWARD, x, ldx, weight, ldw, false, few_rows(MQ_LINEAR_FORWARD, M, z8 != nullptr), M, N, K);
+    FewArgs few{};
+    GemmArgs& a = few.g;
+    if (const int rc = product.arguments(a, (char*)ws, st)) return rc;
     a.out = (char*)y, a.bias = (const char*)bias, a.res = (const char*)residual, a.ldr = ldr;
     a.z = (char*)z, a.zq = (uint8_t*)z8, a.zs = z8_scale, a.act = act;
-    const hipStream_t st = (hipStream_t)stream;
-    if (const int rc = mq_gemm_forward(dtype, bounded, a, plan, ws, st)) return rc;
-    return join(dtype, a, plan, st);
+    if (product.few) {
+        few.k_wave = (K + kFewWaves * 64 - 1) / (kFewWaves * 64) * 64;
+        const dim3 grid((unsigned)((N + 15) / 16));
+        if (dtype == MQ_F16) hipLaunchKernelGGL(few_rows_kernel<MQ_F16>, grid, dim3(kFewWaves * kWave), 0, st, few);
+        else hipLaunchKernelGGL(few_rows_kernel<MQ_BF16>, grid, dim3(kFewWaves * kWave), 0, st, few);
+        return mq_check_launch("linear");
+    }
+    if (const int rc = mq_gemm_forward(dtype, a, product.plan, (float*)ws, st)) return rc;
+    return join(dtype, a, product.plan, st);
 }
 
 extern "C" int mq_linear_input_grad(const void* dz, int dtype, int64_t lddz, const void* weight, int64_t ldw, void* dx, int64_t M, int64_t N,
-                                    int64_t K, float* ws, void* stream) {
-    if (const int rc = check_sizes(dtype, M, N, K)) return rc;
-    if (check_rows(M, N, lddz) || check_rows(N, K, ldw)) return MQ_ERR_ARG;
+                                    int64_t K, void* ws, void* stream) {
+    if (const int rc = check_dtype(dtype)) return rc;
+    if (const int rc = check_product(MQ_LINEAR_INPUT_GRAD, dz, lddz, weight, ldw, false, M, N, K)) return rc;
     if (M == 0 || K == 0) return MQ_OK;
     if (!dx || (N > 0 && (!dz || !weight))) return mq_fail(MQ_ERR_ARG, "linear: null pointer");
-    const bool bounded = !direct_ok(dz, M > 1 ? lddz : 8, N) || !direct_ok(weight, N > 1 ? ldw : 8, K);
-    const GemmPlan plan = gemm_plan(K, M, N, bounded);
-    if (const int rc = check_grid(plan, K, M)) return rc;
-    if (plan.splits > 1 && (!ws || (uintptr_t)ws % 16)) return mq_fail(MQ_ERR_ARG, "linear: a 16-byte aligned workspace is needed");
-    GemmArgs a{};
-    a.p = (const char*)weight, a.q = (const char*)dz, a.ldp = ldw, a.ldq = lddz, a.np = K, a.nq = M, a.k = N, a.out = (char*)dx;
     const hipStream_t st = (hipStream_t)stream;
-    if (const int rc = mq_gemm_input_grad(dtype, bounded, a, plan, ws, st)) return rc;
-    return join(dtype, a, plan, st);
+    const Product product(MQ_LINEAR_INPUT_GRAD, dz, lddz, weight, ldw, false, false, M, N, K);
+    GemmArgs a{};
+    if (const int rc = product.arguments(a, (char*)ws, st)) return rc;
+    a.out = (char*)dx;
+    if (const int rc = mq_gemm_input_grad(dtype, a, product.plan, (float*)ws, st)) return rc;
+    return join(dtype, a, product.plan, st);
 }
 
 extern "C" int mq_linear_weight_grad(const void* dz, int dtype, int64_t lddz, const void* x, int64_t ldx, const uint8_t* x_scale, void* dweight,
-                                     int64_t M, int64_t N, int64_t K, float* ws, void* stream) {
-    if (const int rc = check_sizes(dtype, M, N, K)) return rc;
-    if (check_rows(M, N, lddz) || (!x_scale && check_rows(M, K, ldx))) return MQ_ERR_ARG;
+                                     int64_t M, int64_t N, int64_t K, void* ws, void* stream) {
+    if (const int rc = check_dtype(dtype)) return rc;
+    if (x_scale) ldx = K;
+    if (const int rc = check_product(MQ_LINEAR_WEIGHT_GRAD, dz, lddz, x, ldx, x_scale != nullptr, M, N, K)) return rc;
     if (N == 0 || K == 0) return MQ_OK;
     if (!dweight || (M > 0 && (!dz || !x))) return mq_fail(MQ_ERR_ARG, "linear: null pointer");
     if (x_scale && (K % 32 != 0 || (uintptr_t)x % 16)) return mq_fail(MQ_ERR_ARG, "linear: an 8-bit copy has a multiple of 32 columns and is 16-byte aligned");
-    const bool bounded = !direct_ok(dz, M > 1 ? lddz : 8, N) || (!x_scale && !direct_ok(x, M > 1 ? ldx : 8, K));
-    const GemmPlan plan = gemm_plan(K, N, M, bounded);
-    if (const int rc = check_grid(plan, K, N)) return rc;
-    if (plan.splits > 1 && (!ws || (uintptr_t)ws % 16)) return mq_fail(MQ_ERR_ARG, "linear: a 16-byte aligned workspace is needed");
-    GemmArgs a{};
-    a.p = (const char*)x, a.ps = x_scale, a.q = (const char*)dz, a.ldp = x_scale ? K : ldx, a.ldq = lddz, a.np = K, a.nq = N, a.k = M;
-    a.out = (char*)dweight;
     const hipStream_t st = (hipStream_t)stream;
-    if (const int rc = mq_gemm_weight_grad(dtype, bounded, a, plan, ws, st)) return rc;
-    return join(dtype, a, plan, st);
+    const Product product(MQ_LINEAR_WEIGHT_GRAD, dz, lddz, x, ldx, x_scale != nullptr, false, M, N, K);
+    GemmArgs a{};
+    if (const int rc = product.arguments(a, (char*)ws, st)) return rc;
+    a.ps = x_scale, a.out = (char*)dweight;
+    if (const int rc = mq_gemm_weight_grad(dtype, a, product.plan, (float*)ws, st)) return rc;
+    return join(dtype, a, product.plan, st);
 }
 
 static int64_t act_parts(int64_t M, int64_t N) {
@@ -237,9 +378,11 @@ extern "C" int mq_activation_backward_parts(int64_t M, int64_t N) { return (int)
 
 extern "C" int mq_activation_backward(const void* dy, int dtype, int64_t lddy, const void* z, const uint8_t* z8_scale, int act, void* dz,
                                       void* dbias, float* ws, int64_t M, int64_t N, void* stream) {
-    if (const int rc = check_sizes(dtype, M, N, 0)) return rc;
+    if (const int rc = check_dtype(dtype)) return rc;
+    if (M < 0 || N < 0) return mq_fail(MQ_ERR_ARG, "linear: bad argument");
+    if (M > 0x7FFFFF00 || N > 0x7FFFFF00) return mq_fail(MQ_ERR_ARG, "linear: tensor too large");
     if (act < MQ_ACT_NONE || act > MQ_ACT_GELU_TANH) return mq_fail(MQ_ERR_ARG, "linear: unknown activation");
-    if (check_rows(M, N, lddy)) return MQ_ERR_ARG;
+    if (M > 1 && lddy < N) return mq_fail(MQ_ERR_ARG, "linear: rows overlap");
     if (N == 0 || (M == 0 && !dbias)) return MQ_OK;
     if ((M > 0 && (!dy || (act != MQ_ACT_NONE && !z))) || (dbias && !ws)) return mq_fail(MQ_ERR_ARG, "linear: null pointer");
     if (z8_scale && (N % 32 != 0 || (uintptr_t)z % 8)) return mq_fail(MQ_ERR_ARG, "linear: an 8-bit copy has a multiple of 32 columns and is 8-byte aligned");

@@ -22,10 +22,11 @@ ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}      # 
 _FORWARD, _INPUT_GRAD, _WEIGHT_GRAD = 0, 1, 2                                   # MQ_LINEAR_*
 
 
-def _workspace(product: int, m: int, n: int, k: int, device) -> torch.Tensor | None:
-    floats = ctypes.c_int64()
-    _lib.check(_lib.load().mq_linear_workspace(product, m, n, k, ctypes.addressof(floats)))
-    return torch.empty(floats.value, dtype=torch.float32, device=device) if floats.value else None
+def _workspace(product: int, a: torch.Tensor, b: torch.Tensor, kept8: bool, m: int, n: int, k: int) -> torch.Tensor | None:
+    """Scratch memory of a product of two matrices as they are passed to it, or None."""
+    size = ctypes.c_int64()
+    _lib.check(_lib.load().mq_linear_workspace(product, a.data_ptr(), pitch(a), b.data_ptr(), pitch(b), int(kept8), m, n, k, ctypes.addressof(size)))
+    return torch.empty(size.value, dtype=torch.uint8, device=a.device) if size.value else None
 
 
 def _forward(x2, weight, bias, act, residual2, keep_z, keep8_z):
@@ -38,7 +39,7 @@ def _forward(x2, weight, bias, act, residual2, keep_z, keep8_z):
         z = torch.empty((m, n), dtype=torch.float8_e4m3fn if keep8_z else x2.dtype, device=device)
         scales = torch.empty((m, n // MXFP8_GROUP_SIZE), dtype=torch.uint8, device=device) if keep8_z else None
     launch.note_direct_call()
-    ws = _workspace(_FORWARD, m, n, k, device)
+    ws = _workspace(_FORWARD, x2, weight, keep_z and keep8_z, m, n, k)
     with _lib.on_device(device):
         _lib.check(_lib.load().mq_linear_forward(
             x2.data_ptr(), _lib.DTYPE_CODE[x2.dtype], pitch(x2), weight.data_ptr(), pitch(weight), address(bias), act, address(residual2),
@@ -88,13 +89,13 @@ class _Linear(torch.autograd.Function):
             if need_x:
                 w2 = rows(weight)
                 dx = torch.empty(ctx.x_shape, dtype=ctx.dtype, device=device)
-                ws = _workspace(_INPUT_GRAD, m, n, k, device)
+                ws = _workspace(_INPUT_GRAD, dz, w2, False, m, n, k)
                 _lib.check(lib.mq_linear_input_grad(dz.data_ptr(), dtype, pitch(dz), w2.data_ptr(), pitch(w2), dx.data_ptr(), m, n, k,
                                                     address(ws), stream))
             if need_w:
                 x2 = kept if x_scales is not None else rows(kept)
                 dw = torch.empty((n, k), dtype=ctx.dtype, device=device)
-                ws = _workspace(_WEIGHT_GRAD, m, n, k, device)
+                ws = _workspace(_WEIGHT_GRAD, dz, x2, x_scales is not None, m, n, k)
                 _lib.check(lib.mq_linear_weight_grad(dz.data_ptr(), dtype, pitch(dz), x2.data_ptr(), pitch(x2), address(x_scales),
                                                      dw.data_ptr(), m, n, k, address(ws), stream))
         return dx, dw, db, dy if need_r else None, None, None, None, None

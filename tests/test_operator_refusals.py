@@ -96,15 +96,24 @@ def test_c_entries_of_the_linear_layers():
     _refused(forward(K=1 << 31, ldx=1 << 31, ldw=1 << 31), "too large")
     assert forward(M=0) == 0 and forward(N=0) == 0
 
-    floats = ctypes.c_int64(-1)
-    _refused(lib.mq_linear_workspace(3, 1, 1, 1, ctypes.addressof(floats)), "bad argument")
-    _refused(lib.mq_linear_workspace(0, 1, 1, 1, None), "bad argument")
+    size = ctypes.c_int64(-1)
+
+    def workspace(product=0, a=P, lda=64, b=P, ldb=64, kept=0, M=4, N=32, K=64, out=ctypes.addressof(size)):
+        return lib.mq_linear_workspace(product, a, lda, b, ldb, kept, M, N, K, out)
+
+    _refused(workspace(product=3), "bad argument")
+    _refused(workspace(out=None), "bad argument")
+    _refused(workspace(lda=60), "overlap")
     for product in range(3):
-        assert lib.mq_linear_workspace(product, 1, 512, 8192, ctypes.addressof(floats)) == 0 and floats.value >= 0
-    # a long sum over few outputs is split, and then the partial sums need their memory
-    assert lib.mq_linear_workspace(0, 48, 512, 8192, ctypes.addressof(floats)) == 0 and floats.value > 0
-    _refused(forward(M=48, N=512, K=8192, ldx=8192, ldw=8192, ldr=512, ws=None), "workspace")
-    _refused(forward(M=48, N=512, K=8192, ldx=8192, ldw=8192, ldr=512, ws=P + 4), "workspace")
+        assert workspace(product, lda=8192, ldb=8192, M=300, N=512, K=8192) == 0 and size.value >= 0
+    # a long sum over few outputs is cut, and then the partial sums need their memory; rows off 16 bytes are copied
+    long = dict(M=48, N=512, K=8192)
+    assert workspace(lda=8192, ldb=8192, **long) == 0 and size.value > 0
+    partial = size.value
+    assert workspace(a=P + 2, lda=8192, ldb=8192, **long) == 0 and size.value == partial + 48 * 8192 * 2
+    assert workspace(lda=8192, ldb=8195, **long) == 0 and size.value == partial + 512 * 8192 * 2
+    _refused(forward(**long, ldx=8192, ldw=8192, ldr=512, ws=None), "workspace")
+    _refused(forward(**long, ldx=8192, ldw=8192, ldr=512, ws=P + 4), "workspace")
 
     def weight_grad(dz=P, lddz=32, x=P, ldx=64, xs=None, dw=P, M=4, N=32, K=64):
         return lib.mq_linear_weight_grad(dz, 0, lddz, x, ldx, xs, dw, M, N, K, P, None)
