@@ -108,8 +108,9 @@ int mq_mxfp8_dequant(const void* q, const uint8_t* scale, void* y, int dtype, in
 
 /* Layer norm and RMS norm (no counterpart in the reference, which takes them from its trainer's libraries).
  *   mean = sum(x)/n (rms != 0: 0), rstd = 1/sqrt(sum((x-mean)^2)/n + eps), xhat = (x-mean) rstd, y = xhat weight + bias
- * x [rows,n] dtype, rows ldx elements apart, from any element boundary; weight, bias [n] of type wdtype (dtype or MQ_F32), either may
- * be NULL; y [rows,n] contiguous.  Kept for the backward pass where the pointer is not NULL: mean, rstd [rows] fp32; xhat8 /
+ * x [rows,n] dtype, rows ldx elements apart; row i of x and of y have the same address modulo 16 bytes, for every i (contiguous
+ * tensors that begin at multiples of 16 do, whatever n), and with 8-bit copies it is 0; weight, bias [n] of type wdtype (dtype or MQ_F32), either may
+ * be NULL (bias is, for RMS norm); y [rows,n] contiguous.  Kept for the backward pass where the pointer is not NULL: mean, rstd [rows] fp32; xhat8 /
  * xhat8_scale: xhat as MXFP8 (e4m3 codes [rows,n], exponent bytes [rows,n/32]; n a multiple of 32; 8-byte aligned).
  * y8 / y8_scale: the MXFP8 copy of y itself, what mq_mxfp8_quant makes of it, for a layer that y goes into. */
 int mq_norm_forward(const void* x, int dtype, int64_t ldx, const void* weight, const void* bias, int wdtype, void* y, void* xhat8,
@@ -117,7 +118,8 @@ int mq_norm_forward(const void* x, int dtype, int64_t ldx, const void* weight, c
                     float eps, int rms, void* stream);
 /* Its backward pass: g = dy weight, dx = rstd (g - mean(g) [not rms] - xhat mean(g xhat)), dweight = sum over rows of dy xhat,
  * dbias = sum over rows of dy (both of type wdtype).  x and mean are the forward pass's, or x holds the codes of xhat8 and
- * xhat8_scale is not NULL (mean is then not read).  dx, dweight and dbias may each be NULL.
+ * xhat8_scale is not NULL (mean is then not read).  Rows of dy, of x (unless it holds codes) and of dx (contiguous) have the same
+ * addresses modulo 16 bytes, 0 where x holds codes.  dx, dweight and dbias may each be NULL.
  * ws: mq_norm_backward_parts(rows, n) * n floats of scratch for each of dweight and dbias that is wanted.  The rows' sums are added
  * in an order that depends on the sizes alone. */
 int mq_norm_backward(const void* dy, int dtype, int64_t lddy, const void* x, int64_t ldx, const uint8_t* xhat8_scale, const float* mean,

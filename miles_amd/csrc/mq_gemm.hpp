@@ -347,16 +347,15 @@ __device__ __forceinline__ void finish_block(const GemmArgs& a, float* sums, int
 #pragma unroll
             for (int x = 0; x < 8; x++) z[x] += bias[x];
             if (a.zq) {
-                uint32_t m = 0;
+                float top = 0.0f;
 #pragma unroll
-                for (int x = 0; x < 8; x++) m = umax(m, keep_magnitude(z[x]));
-                m = group_max4(m);
-                const uint32_t e = keep_exponent(m);
+                for (int x = 0; x < 8; x++) top = keep_larger(top, z[x]);
+                const uint32_t m = group_max4(f2u(top)), e = keep_exponent(m);
                 const float inv = e8m0_inverse(e);
                 if (col < a.np) {
                     uint32_t* to = (uint32_t*)(a.zq + row * a.np + col);
-                    to[0] = keep_codes4(z[0], z[1], z[2], z[3], inv);
-                    to[1] = keep_codes4(z[4], z[5], z[6], z[7], inv);
+                    to[0] = keep_codes4(z[0], z[1], z[2], z[3], inv, m == kInfinity);
+                    to[1] = keep_codes4(z[4], z[5], z[6], z[7], inv, m == kInfinity);
                     if ((lane & 3) == 0) a.zs[row * (a.np / 32) + col / 32] = (uint8_t)e;
                 }
             }

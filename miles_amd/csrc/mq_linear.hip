@@ -26,13 +26,9 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs a, int bp
         add_bias4<D>(a, col, z);
     }
     if (a.zq) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) m = umax(m, keep_magnitude(z[i]));
-        m = group_max8(m);
-        const uint32_t e = keep_exponent(m);
+        const uint32_t m = group_max8(f2u(keep_larger(keep_larger(keep_larger(keep_larger(0.0f, z[0]), z[1]), z[2]), z[3]))), e = keep_exponent(m);
         if (inside) {
-            *(uint32_t*)(a.zq + row * a.np + col) = keep_codes4(z[0], z[1], z[2], z[3], e8m0_inverse(e));
+            *(uint32_t*)(a.zq + row * a.np + col) = keep_codes4(z[0], z[1], z[2], z[3], e8m0_inverse(e), m == kInfinity);
             if (col % 32 == 0) a.zs[row * (a.np / 32) + col / 32] = (uint8_t)e;
         }
     }

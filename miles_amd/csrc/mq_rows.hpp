@@ -106,16 +106,17 @@ __device__ __forceinline__ float wave_sum(float v) {
 // ---- 8-bit copies --------------------------------------------------------------------------------------------------------
 // 2^(e - 127)
 __device__ __forceinline__ float e8m0_value(uint32_t e) { return e ? u2f(e == 255 ? 0x7FC00000u : e << 23) : u2f(0x00400000u); }
-// a magnitude's part in the group maximum: a NaN has none (the arithmetic of mxfp8_quantize)
-__device__ __forceinline__ uint32_t keep_magnitude(float v) {
-    const uint32_t a = f2u(v) & 0x7FFFFFFFu;
-    return a > 0x7F800000u ? 0u : a;
+// The larger of a running maximum and a magnitude; a NaN has no part in it (the arithmetic of mxfp8_quantize).
+__device__ __forceinline__ float keep_larger(float m, float v) { return __builtin_fmaxf(m, __builtin_fabsf(v)); }
+// Four values over their group's power of two, which leaves none above 448 but an infinity, in a group whose maximum is one
+// (infinite != 0): that becomes 448.  A NaN goes through.
+__device__ __forceinline__ uint32_t keep_codes4(float a, float b, float c, float d, float inv, bool infinite) {
+    if (infinite)
+        return hw_e4m3x4(clamp_keep_nan(a * inv, -kFp8Max, kFp8Max), clamp_keep_nan(b * inv, -kFp8Max, kFp8Max),
+                         clamp_keep_nan(c * inv, -kFp8Max, kFp8Max), clamp_keep_nan(d * inv, -kFp8Max, kFp8Max));
+    return hw_e4m3x4(a * inv, b * inv, c * inv, d * inv);
 }
-// four values over the group's power of two: the clamp takes infinities to 448, a NaN goes through
-__device__ __forceinline__ uint32_t keep_codes4(float a, float b, float c, float d, float inv) {
-    return hw_e4m3x4(clamp_keep_nan(a * inv, -kFp8Max, kFp8Max), clamp_keep_nan(b * inv, -kFp8Max, kFp8Max),
-                     clamp_keep_nan(c * inv, -kFp8Max, kFp8Max), clamp_keep_nan(d * inv, -kFp8Max, kFp8Max));
-}
+constexpr uint32_t kInfinity = 0x7F800000u;
 __device__ __forceinline__ uint32_t keep_exponent(uint32_t group_magnitude) { return e8m0_ceil(u2f(group_magnitude) * u2f(0x3B124925u)); }
 // four codes as floats: exact, a power of two away from three bits of mantissa
 __device__ __forceinline__ void kept_values4(uint32_t codes, float scale, float* f) {

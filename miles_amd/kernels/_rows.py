@@ -24,3 +24,11 @@ def pitch(t: torch.Tensor) -> int:
 
 def address(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def rows_like_contiguous(t: torch.Tensor) -> torch.Tensor:
+    """`rows(t)`, copied unless every row has the address modulo 16 bytes that it has in a contiguous tensor."""
+    m = rows(t)
+    if m.data_ptr() % 16 == 0 and (m.shape[0] <= 1 or (m.stride(0) - m.shape[1]) * m.element_size() % 16 == 0):
+        return m
+    return m.clone(memory_format=torch.contiguous_format)

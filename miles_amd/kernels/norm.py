@@ -15,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from miles_amd import _lib, launch
-from miles_amd.kernels._rows import address, pitch, rows
+from miles_amd.kernels._rows import address, pitch, rows_like_contiguous
 from miles_amd.kernels.quant.act_checkpoint import MXFP8_GROUP_SIZE, ActCheckpoint, check_width
 
 
@@ -26,7 +26,7 @@ def _empty8(m: int, n: int, device) -> tuple[torch.Tensor, torch.Tensor]:
 
 def _forward(x, weight, bias, eps, rms, statistics, keep, copy):
     """(y, mean, rstd, kept xhat, its scales, copy of y, its scales), with None for what is not asked for."""
-    x2 = rows(x)
+    x2 = rows_like_contiguous(x)
     m, n = x2.shape
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     mean = torch.empty(m, dtype=torch.float32, device=x.device) if statistics and not rms and not keep else None
@@ -58,9 +58,9 @@ class _Norm(torch.autograd.Function):
     def backward(ctx, dy, *_):
         x, xs, mean, rstd, weight = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        dy2 = rows(dy)
+        dy2 = rows_like_contiguous(dy)
         m, n = dy2.shape
-        x2 = x if xs is not None else rows(x)
+        x2 = x if xs is not None else rows_like_contiguous(x)
         vector = weight.dtype if weight is not None else dy.dtype
         lib = _lib.load()
         launch.note_direct_call()

@@ -48,8 +48,8 @@ def test_c_entry_of_the_dequantizer():
 def test_c_entries_of_the_norms():
     lib = _lib.load()
 
-    def forward(x=P, dtype=0, ldx=64, w=P, b=P, wdtype=0, y=P, xq=None, xs=None, yq=None, ys=None, rows=4, n=64):
-        return lib.mq_norm_forward(x, dtype, ldx, w, b, wdtype, y, xq, xs, yq, ys, P, P, rows, n, 1e-5, 0, None)
+    def forward(x=P, dtype=0, ldx=64, w=P, b=P, wdtype=0, y=P, xq=None, xs=None, yq=None, ys=None, rows=4, n=64, rms=0):
+        return lib.mq_norm_forward(x, dtype, ldx, w, b, wdtype, y, xq, xs, yq, ys, P, P, rows, n, 1e-5, rms, None)
 
     _refused(forward(dtype=3), "bad argument")
     _refused(forward(rows=-1), "bad argument")
@@ -61,6 +61,10 @@ def test_c_entries_of_the_norms():
     _refused(forward(yq=P, ys=P, n=48), "multiple of 32")
     _refused(forward(xq=P + 4, xs=P), "8 bytes")
     _refused(forward(rows=1 << 31), "too large")
+    _refused(forward(rms=1), "no bias")
+    _refused(forward(x=P + 2), "offsets")
+    _refused(forward(ldx=66), "offsets")
+    _refused(forward(x=P + 2, y=P + 2, yq=P, ys=P), "offsets")
     assert forward(rows=0, x=None, y=None) == 0
 
     def backward(dy=P, lddy=64, x=P, ldx=64, xs=None, mean=P, rstd=P, dw=P, db=P, ws=P, rows=4, n=64, rms=0):
@@ -72,6 +76,10 @@ def test_c_entries_of_the_norms():
     _refused(backward(rstd=None), "null pointer")
     _refused(backward(ws=None), "null pointer")
     _refused(backward(xs=P, n=48), "multiple of 32")
+    _refused(backward(rms=1), "no bias")
+    _refused(backward(dy=P + 2), "offsets")
+    _refused(backward(lddy=65), "offsets")
+    _refused(backward(xs=P, x=P + 8, lddy=66), "offsets")
     _refused(backward(xs=P, x=P + 4), "8-byte")
     assert backward(n=0, ws=P) == 0
 
