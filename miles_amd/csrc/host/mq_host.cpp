@@ -647,6 +647,12 @@ PyObject* int4_fake(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+}  // namespace
+
+#include "mq_host_operators.hpp"
+
+namespace {
+
 // set_error(exception class): what a refusal by the library raises
 PyObject* set_error(PyObject*, PyObject* o) {
     Py_XSETREF(g_error, Py_NewRef(o));
@@ -674,6 +680,10 @@ PyMethodDef methods[] = {{"set_error", set_error, METH_O, nullptr},
                          {"simulate", (PyCFunction)(void*)simulate, METH_FASTCALL, nullptr},
                          {"nvfp4_images", (PyCFunction)(void*)nvfp4_images, METH_FASTCALL, nullptr},
                          {"int4_fake", (PyCFunction)(void*)int4_fake, METH_FASTCALL, nullptr},
+                         {"norm", (PyCFunction)(void*)norm, METH_FASTCALL, nullptr},
+                         {"keep8", keep8, METH_O, nullptr},
+                         {"mxfp8_dequant", (PyCFunction)(void*)mxfp8_dequant, METH_FASTCALL, nullptr},
+                         {"linear", (PyCFunction)(void*)linear, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mq_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -15,6 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from miles_amd import _lib, launch
+from miles_amd._host import native
 from miles_amd.kernels._rows import address, pitch, rows
 from miles_amd.kernels.quant.act_checkpoint import MXFP8_GROUP_SIZE, ActCheckpoint, check_width, keep8
 
@@ -110,6 +111,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     multiple of 32) in 8 bits for the backward pass; an `ActCheckpoint` of x that exists already (of a norm's output, or one
     that several projections of one input share) is kept instead of a new one."""
     what = "linear"
+    if activation in ACTIVATIONS and not torch.compiler.is_dynamo_compiling():
+        given = type(checkpoint) is ActCheckpoint
+        made = native.linear(x, weight, bias, ACTIVATIONS[activation], residual, given or checkpoint,          # ordinary tensors: graph
+                             checkpoint.codes if given else None, checkpoint.scales if given else None)        # node in native code
+        if made is not None:
+            return made
     _lib.require_gpu(x, what)
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"linear: bfloat16 or float16 tensors, got {x.dtype}")

@@ -15,6 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from miles_amd import _lib, launch
+from miles_amd._host import native
 from miles_amd.kernels._rows import address, pitch, rows_like_contiguous
 from miles_amd.kernels.quant.act_checkpoint import MXFP8_GROUP_SIZE, ActCheckpoint, check_width
 
@@ -78,6 +79,10 @@ class _Norm(torch.autograd.Function):
 
 
 def _norm(what, x, weight, bias, eps, rms, checkpoint, output_checkpoint):
+    if not torch.compiler.is_dynamo_compiling():
+        made = native.norm(x, weight, bias, eps, rms, checkpoint, output_checkpoint)      # ordinary tensors: graph node in native code
+        if made is not None:
+            return (made[0], ActCheckpoint(made[1], made[2], x.dtype)) if output_checkpoint else made
     _lib.require_gpu(x, what)
     _lib.dtype_code(x, what)
     if x.dim() == 0:

@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 
 from miles_amd import _lib, launch
+from miles_amd._host import native
 from miles_amd.utils.mxfp8 import MXFP8_GROUP_SIZE, mxfp8_dequantize
 
 
@@ -60,6 +61,9 @@ def keep8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def checkpoint_activation(x: torch.Tensor) -> ActCheckpoint:
     """x [..., K] (bf16, fp16 or fp32, K a multiple of 32) kept in 8 bits.  The copy carries no gradient."""
+    made = native.keep8(x)
+    if made is not None:
+        return ActCheckpoint(*made, x.dtype)
     _lib.require_gpu(x, "checkpoint_activation")
     _lib.dtype_code(x, "checkpoint_activation")
     if x.dim() == 0:

@@ -60,6 +60,9 @@ def mxfp8_quantize(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def mxfp8_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """(float8_e4m3fn codes [..., K], uint8 E8M0 scales [..., K/32]) of `mxfp8_quantize` -> the values they stand for, `code x
     2^(scale - 127)` rounded once to bf16, fp16 or fp32 (in fp16 a finite value beyond +-65504 becomes +-65504)."""
+    made = native.mxfp8_dequant(codes, scales, dtype)
+    if made is not None:
+        return made
     _lib.require_gpu(codes, "mxfp8_dequantize")
     _lib.require_gpu(scales, "mxfp8_dequantize")
     if codes.dtype not in (torch.float8_e4m3fn, torch.uint8) or scales.dtype != torch.uint8:

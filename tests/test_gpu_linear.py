@@ -333,3 +333,50 @@ def test_refusals():
     g = torch.autograd.grad(linear(x, w).float().square().sum(), x, create_graph=True)[0]
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), x)
+
+
+def test_native_and_python_host_layers_agree(monkeypatch):
+    """An ordinary call makes its graph node in native code, any other in Python: the same bits, and only what asks has a gradient."""
+    from miles_amd.kernels import norm as norm_mod
+    from miles_amd.kernels.norm import layer_norm
+
+    class Declines:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    x, w, b, r, dy = _random(40, 64, 96, torch.bfloat16, seed=21)
+    gamma, beta = (torch.randn(96, device=DEV).bfloat16().requires_grad_(True) for _ in range(2))
+
+    def everything():
+        out = []
+        for wanted in itertools.product((False, True), repeat=3):
+            if any(wanted):
+                gx, gw, gb = (t if want else t.detach() for t, want in zip((x, gamma, beta), wanted))
+                leaves = [t for t, want in zip((gx, gw, gb), wanted) if want]
+                for ww, bb in ((gw, gb), (gw, None), (None, gb), (None, None)):
+                    for kw in ({}, {"checkpoint": True}):
+                        y = layer_norm(gx.view(8, 5, 96), ww, bb, **kw)
+                        if y.requires_grad:
+                            out.append(y.detach())
+                            out.extend(g for g in torch.autograd.grad(y.sum(0), leaves, dy[:5, :1].expand(5, 96), allow_unused=True) if g is not None)
+        for wanted in itertools.product((False, True), repeat=4):
+            if any(wanted):
+                args = [t if want else t.detach() for t, want in zip((x, w, b, r), wanted)]
+                for bias, residual in itertools.product((args[2], None), (args[3], None)):
+                    for kw in ({}, {"checkpoint": True}, {"checkpoint": checkpoint_activation(x)}):
+                        for act in (None, "silu"):
+                            y = linear(args[0], args[1], bias, activation=act, residual=residual, **kw)
+                            if y.requires_grad:
+                                out.append(y.detach())
+                                leaves = [t for t, want in zip(args, wanted) if want]
+                                out.extend(g for g in torch.autograd.grad(y, leaves, dy, allow_unused=True) if g is not None)
+        copy = checkpoint_activation(x)
+        return out + [copy.codes.view(torch.uint8), copy.scales, copy.restore()]
+
+    ours = everything()
+    for module in (linear_module, norm_mod):
+        monkeypatch.setattr(module, "native", Declines())
+    monkeypatch.setattr("miles_amd.kernels.quant.act_checkpoint.native", Declines())
+    monkeypatch.setattr("miles_amd.utils.mxfp8.native", Declines())
+    theirs = everything()
+    assert len(ours) == len(theirs) > 100 and all(torch.equal(p, q) for p, q in zip(ours, theirs))
