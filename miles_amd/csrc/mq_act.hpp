@@ -15,12 +15,12 @@ __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp
 __device__ __forceinline__ void normal_share(float z, float& bell, float& share) {
     const float x = __builtin_fabsf(z) * 0.7071067811865476f;
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
-    float p = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
-    p = __builtin_fmaf(t, p, 1.421413741f);
-    p = __builtin_fmaf(t, p, -0.284496736f);
-    p = __builtin_fmaf(t, p, 0.254829592f);
-    bell = fast_exp(-x * x);
-    const float tail = 0.5f * t * p * bell;
+    float p = __builtin_fmaf(t, 0.5307027145f, -0.7265760135f);         // (half the formula's coefficients: half of erfc)
+    p = __builtin_fmaf(t, p, 0.7107068705f);
+    p = __builtin_fmaf(t, p, -0.142248368f);
+    p = __builtin_fmaf(t, p, 0.127414796f);
+    bell = __builtin_amdgcn_exp2f(z * z * -0.7213475204444817f);          // exp(-z^2 / 2)
+    const float tail = t * p * bell;
     share = z < 0.0f ? tail : 1.0f - tail;
 }
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z)); }

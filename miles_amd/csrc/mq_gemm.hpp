@@ -111,8 +111,8 @@ struct Stage {
     int64_t ld, n;                        // n: outputs from the tile's first on
     int64_t step_bytes;
     uint32_t offset[kPieces];
-    u32x4 v[kPieces];
-    uint32_t e[kPieces];
+    u32x4 coming[kKept ? kPieces : 1], v[kKept ? kPieces : 1];        // codes on their way, and those that have arrived
+    uint32_t coming_e[kKept ? kPieces : 1], e[kKept ? kPieces : 1];
 
     static __device__ __forceinline__ int row_piece(int at) { return (at & 7) ^ (at >> 4 & 7); }
     static __device__ __forceinline__ int down_k(int at) { return at / (B / 8); }
@@ -140,6 +140,12 @@ struct Stage {
                     offset[u] = (uint32_t)((int64_t)k * ld * 2 + (c < n ? c : 0) * 2);
                 }
             }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kPieces; u++) {
+                const int at = ((int)threadIdx.x + u * THREADS) * 2, c = down_col(at);
+                offset[u] = (uint32_t)(down_k(at) * ld + (c < n ? c : 0));
+            }
         }
     }
     // The next step's operand, piece by piece: on its way to `lds` (direct), or into registers.  left: k that are left from the step's
@@ -150,25 +156,33 @@ struct Stage {
             const int at = (int)threadIdx.x + u * THREADS, k = kAcross ? row_piece(at) * 8 : down_k(at);
             direct16(lds + wave + u * (THREADS * 16), buffer_of(base), k < left ? offset[u] : kNowhere);
         } else {
-            const int at = ((int)threadIdx.x + u * THREADS) * 2, k = down_k(at), c = down_col(at);
-            const bool inside = k < left && c < n;
-            v[u] = read16(base, inside ? (uint32_t)(k * ld + c) : kNowhere);
-            e[u] = read1(scales, inside ? (uint32_t)(k * (ld / 32) + c / 32) : kNowhere);
+            const bool inside = down_k(((int)threadIdx.x + u * THREADS) * 2) < left;
+            coming[u] = read16(base, inside ? offset[u] : kNowhere);
+            coming_e[u] = read1(scales, inside ? offset[u] / 32 : kNowhere);                  // (ld is a multiple of 32)
         }
     }
     __device__ __forceinline__ void advance() {
         base += step_bytes;
         if (kKept) scales += kStep * (ld / 32);
     }
-    // a quarter, four values, of an 8-bit piece that came through registers, into shared memory
-    __device__ __forceinline__ void put_part(int u, int part, MQ_LDS char* lds) {
+    // The codes have arrived: said where the wavefront has waited for them anyway, because a wait that the compiler put in front of
+    // their use would also wait for the accesses issued since, which it does not know of.
+    __device__ __forceinline__ void settle() {
         if (kDirect) return;
-        float f[4];
-        kept_values4(part == 0 ? v[u].x : part == 1 ? v[u].y : part == 2 ? v[u].z : v[u].w, e8m0_value(e[u]), f);
-        if (D == MQ_F16)
 #pragma unroll
-            for (int m = 0; m < 4; m++) f[m] = clamp_keep_nan(f[m], -65504.0f, 65504.0f);
-        *(MQ_LDS u32x2*)(lds + ((int)threadIdx.x + u * THREADS) * 32 + part * 8) = u32x2{pack2<D>(f[0], f[1]), pack2<D>(f[2], f[3])};
+        for (int u = 0; u < kPieces; u++) {
+            asm volatile("" : "+v"(coming[u].x), "+v"(coming[u].y), "+v"(coming[u].z), "+v"(coming[u].w), "+v"(coming_e[u]));
+            v[u] = coming[u];
+            e[u] = coming_e[u];
+        }
+    }
+    // Half of an 8-bit piece, eight values, that came through registers, into shared memory: which half first depends on the lane, so
+    // that lanes whose slots lie in the same banks write different halves.
+    __device__ __forceinline__ void put_half(int u, int turn, MQ_LDS char* lds) {
+        if (kDirect) return;
+        const bool high = (turn != 0) != ((threadIdx.x & 8) != 0);
+        const u32x2 a = kept_pack4<D>(high ? v[u].z : v[u].x, e[u]), b = kept_pack4<D>(high ? v[u].w : v[u].y, e[u]);
+        *(MQ_LDS u32x4*)(lds + ((int)threadIdx.x + u * THREADS) * 32 + (high ? 16 : 0)) = u32x4{a.x, a.y, b.x, b.y};
     }
 };
 
@@ -337,38 +351,56 @@ __device__ __forceinline__ void finish_block(const GemmArgs& a, float* sums, int
 #pragma unroll
         for (int x = 0; x < 8; x++) bias[x] = 0.0f;
     }
+    // four rows at a time, whose loads are issued together: one wavefront on a SIMD has nobody to wait behind
+    constexpr int kAtOnce = 4;
+    static_assert(ROWS % (8 * kAtOnce) == 0, "whole rounds");
     with_activation(a.act, [&](auto kind) {
         constexpr int ACT = decltype(kind)::value;
-        for (int r = lane >> 3; r < ROWS; r += 8) {
-            const int64_t row = row0 + r;
-            if (row >= a.nq) break;                        // (the four lanes of 32 columns have one row)
-            const f32x4 lo = *(MQ_LDS const f32x4*)(stage + stage_at(r, 2 * mine)), hi = *(MQ_LDS const f32x4*)(stage + stage_at(r, 2 * mine + 1));
-            float z[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        for (int r0 = lane >> 3; r0 < ROWS; r0 += 8 * kAtOnce) {
+            float z[kAtOnce][8];
+            u32x4 res[kAtOnce];
+            if (row0 + r0 >= a.nq) break;                  // (the four lanes of 32 columns have one row)
 #pragma unroll
-            for (int x = 0; x < 8; x++) z[x] += bias[x];
-            if (a.zq) {
-                float top = 0.0f;
+            for (int i = 0; i < kAtOnce; i++) {
+                const int r = r0 + 8 * i;
+                if (a.res && row0 + r < a.nq) res[i] = ld_row<D>(a.res + (row0 + r) * a.ldr * 2, col, a.np);
+                const f32x4 lo = *(MQ_LDS const f32x4*)(stage + stage_at(r, 2 * mine)), hi = *(MQ_LDS const f32x4*)(stage + stage_at(r, 2 * mine + 1));
 #pragma unroll
-                for (int x = 0; x < 8; x++) top = keep_larger(top, z[x]);
-                const uint32_t m = group_max4(f2u(top)), e = keep_exponent(m);
-                const float inv = e8m0_inverse(e);
-                if (col < a.np) {
-                    uint32_t* to = (uint32_t*)(a.zq + row * a.np + col);
-                    to[0] = keep_codes4(z[0], z[1], z[2], z[3], inv, m == kInfinity);
-                    to[1] = keep_codes4(z[4], z[5], z[6], z[7], inv, m == kInfinity);
-                    if ((lane & 3) == 0) a.zs[row * (a.np / 32) + col / 32] = (uint8_t)e;
+                for (int x = 0; x < 4; x++) {
+                    z[i][x] = lo[x];
+                    z[i][4 + x] = hi[x];
                 }
             }
-            if (a.z) st_row<D>(a.z + row * a.np * 2, col, a.np, pack<D>(z));
 #pragma unroll
-            for (int x = 0; x < 8; x++) z[x] = activate<ACT>(z[x]);
-            if (a.res) {
-                float f[8];
-                unpack<D>(ld_row<D>(a.res + row * a.ldr * 2, col, a.np), f);
+            for (int i = 0; i < kAtOnce; i++) {
+                const int64_t row = row0 + r0 + 8 * i;
+                if (row >= a.nq) break;
 #pragma unroll
-                for (int x = 0; x < 8; x++) z[x] += f[x];
+                for (int x = 0; x < 8; x++) z[i][x] += bias[x];
+                if (a.zq) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int x = 0; x < 8; x++) top = keep_larger(top, z[i][x]);
+                    const uint32_t m = group_max4(f2u(top)), e = keep_exponent(m);
+                    const float inv = e8m0_inverse(e);
+                    if (col < a.np) {
+                        uint32_t* to = (uint32_t*)(a.zq + row * a.np + col);
+                        to[0] = keep_codes4(z[i][0], z[i][1], z[i][2], z[i][3], inv, m == kInfinity);
+                        to[1] = keep_codes4(z[i][4], z[i][5], z[i][6], z[i][7], inv, m == kInfinity);
+                        if ((lane & 3) == 0) a.zs[row * (a.np / 32) + col / 32] = (uint8_t)e;
+                    }
+                }
+                if (a.z) st_row<D>(a.z + row * a.np * 2, col, a.np, pack<D>(z[i]));
+#pragma unroll
+                for (int x = 0; x < 8; x++) z[i][x] = activate<ACT>(z[i][x]);
+                if (a.res) {
+                    float f[8];
+                    unpack<D>(res[i], f);
+#pragma unroll
+                    for (int x = 0; x < 8; x++) z[i][x] += f[x];
+                }
+                st_row<D>(a.out + row * a.np * 2, col, a.np, pack<D>(z[i]));
             }
-            st_row<D>(a.out + row * a.np * 2, col, a.np, pack<D>(z));
         }
     });
 }
@@ -410,11 +442,11 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
         for (int u = 0; u < sq.kPieces; u++) sq.fetch_piece(u, to, left);
         sq.advance();
     };
-    auto put_p = [&](MQ_LDS char* to) {
+    auto put_p = [&](MQ_LDS char* to) {                    // what has arrived in registers
 #pragma unroll
         for (int u = 0; u < sp.kPieces; u++)
 #pragma unroll
-            for (int part = 0; part < 4; part++) sp.put_part(u, part, to);
+            for (int turn = 0; turn < 2; turn++) sp.put_half(u, turn, to);
     };
     constexpr bool kPDirect = PM != kDownKept;
     static_assert(QM != kDownKept, "the first operand may be an 8-bit copy");
@@ -439,17 +471,14 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
         auto after = [&](uint32_t buffer, uint32_t by) { return buffer + by * kFifth >= kAll ? buffer + by * kFifth - kAll : buffer + by * kFifth; };
         static_assert(BP == BQ && sq.kPieces == 8 && sp.kPieces == (kPDirect ? 8 : 4), "buffers of one size, a piece for every other product");
         fetch_p(0, lds0);
+        sp.settle();
         put_p(lds);
         fetch_q(0, lds0 + kFifth);
         fetch_p(1, lds0 + 2 * kFifth);
-        put_p(lds + 2 * kFifth);
         fetch_q(1, lds0 + 3 * kFifth);
-        if (kPDirect) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(sp.kUnits + sq.kUnits) : "memory");
-        else {
-            fetch_p(2, 0);                                  // (into registers)
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
+        asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kPDirect ? sp.kUnits + sq.kUnits : 0) : "memory");
         meet();
+        sp.settle();
         u32x4 p[2][F], q[2][F];
 #pragma unroll
         for (int i = 0; i < F; i++) {
@@ -459,17 +488,18 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
         uint32_t at = 0;                                    // the buffer of P of step t
         for (int t = 0; t < steps; t++) {
             const uint32_t next = after(at, 2), third = after(at, 4);
-            const int left = left_of(t + 2), left_kept = left_of(t + 3);
+            const int left = left_of(t + 2);
             // A wavefront issues an instruction in about four cycles and its product takes 32: what goes between two products is kept
             // short, and the reads come first, so that they are back when the products that need them are due.
 #pragma unroll
             for (int h = 0; h < 4; h++) {
                 if (h == 3) {
                     // this step's fragments are all in registers and so its buffers are free; the next step's operands have arrived,
-                    // whose last pieces were asked for a step ago (P of step t + 2 may still be on its way)
-                    if (kPDirect) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(sp.kUnits) : "memory");
-                    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    // whose last pieces were asked for a step ago (P of step t + 2 may still be on its way; an 8-bit one has come into
+                    // registers)
+                    asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kPDirect ? sp.kUnits : 0) : "memory");
                     meet();
+                    sp.settle();
                 }
                 MQ_LDS char* fromp = lds + (h == 3 ? next : at);
                 MQ_LDS char* fromq = lds + (h == 3 ? after(next, 1) : after(at, 1));
@@ -480,12 +510,14 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
                     else if (m < 2 * F) q[h & 1 ^ 1][m - F] = fq.get(fromq, h + 1 & 3, m - F);
                     else if (kPDirect && h < 2) {            // P of step t + 2, eight pieces in two parts of this step
                         if (m % 2 == 0) sp.fetch_piece((m - 8) / 2 + h * 4, lds0 + third, left);
-                    } else if (!kPDirect && h < 2) {         // or its registers are written out, in sixteen parts
-                        sp.put_part((m - 8) / 4 + h * 2, m % 4, lds + third);
                     } else if (h == 3) {
                         sq.fetch_piece(m - 8, lds0 + at, left);
                     }
-                    if (!kPDirect && h == 3 && m < 8 && m % 2 == 0) sp.fetch_piece(m / 2, 0, left_kept);      // and filled again
+                    // An 8-bit P: that of step t + 2 is asked for, and that of step t + 1 written out of its registers.
+                    if (!kPDirect) {
+                        if (h == 0 && m < 8 && m % 2 == 1) sp.fetch_piece(m / 2, 0, left);
+                        if (h < 2 && m >= 8 && m % 2 == 0) sp.put_half((m - 8) / 4 + h * 2, m / 2 % 2, lds + next);
+                    }
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -498,8 +530,8 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
         meet();
         MQ_LDS char* stage = lds + wave * (TQ * 256);
         const int row = lane & 31, four = lane >> 5;        // a lane has sixteen columns of a row, fours that are eight apart
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
+        auto finish_half = [&](auto which) {               // (written out twice: the sums are registers, whose numbers are constants)
+            constexpr int half = decltype(which)::value;
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -510,7 +542,9 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
                         *(MQ_LDS f32x4*)(stage + stage_at(j * 32 + row, i * 8 + x * 2 + four)) = f32x4{c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3]};
                     }
             finish_block<D, EPILOGUE, TQ>(a, sums ? sums + half * 64 : nullptr, BP, q0 + wq * TQ, p0 + wp * TP + half * 64, stage);
-        }
+        };
+        finish_half(std::integral_constant<int, 0>{});
+        finish_half(std::integral_constant<int, 1>{});
     } else {
         Fragments<PM, BP, FP> fp;
         Fragments<QM, BQ, FQ> fq;
@@ -525,6 +559,7 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
         // registers was loaded a step earlier.
         fetch_p(0, lds0);
         fetch_q(0, lds0 + kPBytes);
+        sp.settle();
         put_p(lds);
         if (!kPDirect) fetch_p(1, 0);
         for (int t = 0; t < steps; t++) {
@@ -532,13 +567,10 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
             const uint32_t next = (uint32_t)(t + 1 & 1) * kBuffer;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             meet();
+            sp.settle();
             fetch_q(t + 1, lds0 + next + kPBytes);
-            if (kPDirect) {
-                fetch_p(t + 1, lds0 + next);
-            } else {
-                put_p(lds + next);
-                fetch_p(t + 2, 0);
-            }
+            if (kPDirect) fetch_p(t + 1, lds0 + next);
+            else fetch_p(t + 2, 0);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 u32x4 p[FP], q[FQ];
@@ -551,6 +583,7 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
 #pragma unroll
                     for (int j = 0; j < FQ; j++) acc[i][j] = mfma<D>(p[i], q[j], acc[i][j]);
             }
+            if (!kPDirect) put_p(lds + next);               // (behind the reads, which would wait for the writes)
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // (as above)
         meet();

@@ -18,10 +18,19 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs a, int bp
     float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (inside) {
         const float* from = a.ws + (int64_t)nth * a.splits * bp * bq + r * bp + c;
-        for (int s = 0; s < a.splits; s++) {
-            const f32x4 v = *(const f32x4*)(from + (int64_t)s * bp * bq);
+        // eight parts' loads at once: their sum is short, and each would wait for memory by itself
+        constexpr int kAtOnce = 8;
+        for (int s0 = 0; s0 < a.splits; s0 += kAtOnce) {
+            f32x4 v[kAtOnce];
 #pragma unroll
-            for (int i = 0; i < 4; i++) z[i] += v[i];
+            for (int s = 0; s < kAtOnce; s++) {
+                v[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (s0 + s < a.splits) v[s] = *(const f32x4*)(from + (int64_t)(s0 + s) * bp * bq);
+            }
+#pragma unroll
+            for (int s = 0; s < kAtOnce; s++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) z[i] += v[s][i];
         }
         add_bias4<D>(a, col, z);
     }
@@ -45,10 +54,20 @@ struct PadArgs {
 __global__ __launch_bounds__(256) void pad_rows_kernel(const PadArgs a) {
     const int which = blockIdx.y;
     if (!a.to[which]) return;
-    const int64_t per_row = (a.cols[which] + 7) / 8, units = a.rows[which] * per_row;
-    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += (int64_t)gridDim.x * 256) {
-        const int64_t row = u / per_row, c = (u - row * per_row) * 8;
-        *(u32x4*)(a.to[which] + u * 16) = ld_row<MQ_BF16>(a.from[which] + row * a.ld[which] * 2, c, a.cols[which]);
+    const int lane = threadIdx.x & (kWave - 1);
+    const int64_t cols = a.cols[which], pieces = (cols + 7) / 8, step = (int64_t)gridDim.x * 4;
+    for (int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave; row < a.rows[which]; row += step) {
+        const char* from = a.from[which] + row * a.ld[which] * 2;
+        char* to = a.to[which] + row * pieces * 16;
+        constexpr int kAtOnce = 4;
+        for (int64_t i = lane; i < pieces; i += kWave * kAtOnce) {
+            u32x4 v[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; u++) v[u] = ld_row<MQ_BF16>(from, (i + u * kWave) * 8, cols);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; u++)
+                if (i + u * kWave < pieces) *(u32x4*)(to + (i + u * kWave) * 16) = v[u];
+        }
     }
 }
 
@@ -133,30 +152,50 @@ __global__ __launch_bounds__(256) void activation_bwd_kernel(const ActGradArgs a
     for (int j = 0; j < 8; j++) db[j] = 0.0f;
     with_activation(a.act, [&](auto kind) {
         constexpr int ACT = decltype(kind)::value;
-        for (int64_t row = (int64_t)blockIdx.y * 4 + wave; row < a.rows; row += (int64_t)gridDim.y * 4) {
-            float g[8];
-            unpack<D>(ld_row<D>(a.dy + row * a.lddy * 2, col, a.n), g);
-            if (ACT != MQ_ACT_NONE) {
-                float z[8];
-                if (KEPT) {
-                    u32x2 c = {0u, 0u};
-                    uint32_t e = 0;
+        const int64_t step = (int64_t)gridDim.y * 4;
+        constexpr int kAtOnce = 2;
+        for (int64_t row0 = (int64_t)blockIdx.y * 4 + wave; row0 < a.rows; row0 += step * kAtOnce) {
+            u32x4 dy[kAtOnce], zv[kAtOnce];
+            uint32_t e[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; i++) {
+                const int64_t row = row0 + i * step;
+                dy[i] = zv[i] = u32x4{0u, 0u, 0u, 0u};
+                e[i] = 0;
+                if (row >= a.rows) continue;
+                dy[i] = ld_row<D>(a.dy + row * a.lddy * 2, col, a.n);
+                if (ACT != MQ_ACT_NONE && KEPT) {
                     if (col < a.n) {
-                        c = *(const u32x2*)(a.z + row * a.n + col);
-                        e = a.zs[row * (a.n / 32) + col / 32];
+                        const u32x2 c = *(const u32x2*)(a.z + row * a.n + col);
+                        zv[i].x = c.x, zv[i].y = c.y;
+                        e[i] = a.zs[row * (a.n / 32) + col / 32];
                     }
-                    const float s = e8m0_value(e);
-                    kept_values4(c.x, s, z);
-                    kept_values4(c.y, s, z + 4);
-                } else {
-                    unpack<D>(ld_row<D>(a.z + row * a.n * 2, col, a.n), z);
+                } else if (ACT != MQ_ACT_NONE) {
+                    zv[i] = ld_row<D>(a.z + row * a.n * 2, col, a.n);
                 }
-#pragma unroll
-                for (int j = 0; j < 8; j++) g[j] *= slope<ACT>(z[j]);
             }
-            if (a.dz) st_row<D>(a.dz + row * a.n * 2, col, a.n, pack<D>(g));
 #pragma unroll
-            for (int j = 0; j < 8; j++) db[j] += g[j];
+            for (int i = 0; i < kAtOnce; i++) {
+                const int64_t row = row0 + i * step;
+                if (row >= a.rows) break;
+                float g[8];
+                unpack<D>(dy[i], g);
+                if (ACT != MQ_ACT_NONE) {
+                    float z[8];
+                    if (KEPT) {
+                        const float s = e8m0_value(e[i]);
+                        kept_values4(zv[i].x, s, z);
+                        kept_values4(zv[i].y, s, z + 4);
+                    } else {
+                        unpack<D>(zv[i], z);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; j++) g[j] *= slope<ACT>(z[j]);
+                }
+                if (a.dz) st_row<D>(a.dz + row * a.n * 2, col, a.n, pack<D>(g));
+#pragma unroll
+                for (int j = 0; j < 8; j++) db[j] += g[j];
+            }
         }
     });
     if (!a.part) return;
@@ -261,18 +300,17 @@ struct Product {
         if (bytes > 0 && (!ws || (uintptr_t)ws % 16)) return mq_fail(MQ_ERR_ARG, "linear: a 16-byte aligned workspace is needed");
         a.p = (const char*)p, a.q = (const char*)q, a.ldp = ldp, a.ldq = ldq, a.np = np, a.nq = nq, a.k = k;
         PadArgs pad{};
-        int64_t units = 0;
+        int64_t most = 0;
         auto copy = [&](int i, const char*& operand, int64_t& ld, int64_t at, int64_t rows, int64_t cols) {
             if (at < 0) return;
             pad.from[i] = operand, pad.ld[i] = ld, pad.rows[i] = rows, pad.cols[i] = cols, pad.to[i] = ws + at;
             operand = ws + at, ld = (cols + 7) / 8 * 8;
-            const int64_t n = rows * (ld / 8);
-            if (n > units) units = n;
+            if (rows > most) most = rows;
         };
         copy(0, a.p, a.ldp, p_at, p_rows, p_cols);
         copy(1, a.q, a.ldq, q_at, q_rows, q_cols);
-        if (units > 0) {
-            const int64_t blocks = (units + 255) / 256;
+        if (most > 0) {
+            const int64_t blocks = (most + 3) / 4;
             hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), 2), dim3(256), 0, st, pad);
         }
         return MQ_OK;

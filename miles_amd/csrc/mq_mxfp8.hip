@@ -186,15 +186,16 @@ __global__ __launch_bounds__(256) void mxfp8_dequant_kernel(const uint8_t* __res
 #pragma unroll
     for (int i = 0; i < kMxBackUnits; i++) {
         const int64_t u = base + i * 256;
-        const float s = e8m0_value(e[i]);
-        float f[8];
-        kept_values4(c[i].x, s, f);
-        if (D != MQ_F32) kept_values4(c[i].y, s, f + 4);
-        if (D == MQ_F16) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) f[j] = clamp_keep_nan(f[j], -65504.0f, 65504.0f);
+        u32x4 out;
+        if (D == MQ_F32) {
+            float f[4];
+            kept_values4(c[i].x, e8m0_value(e[i]), f);
+            out = pack<D>(f);
+        } else {
+            const u32x2 lo = kept_pack4<D>(c[i].x, e[i]), hi = kept_pack4<D>(c[i].y, e[i]);
+            out = u32x4{lo.x, lo.y, hi.x, hi.y};
         }
-        if (u < units) st16(y + u * 16, pack<D>(f));
+        if (u < units) st16(y + u * 16, out);
     }
 }
 

@@ -380,3 +380,26 @@ def test_native_and_python_host_layers_agree(monkeypatch):
     monkeypatch.setattr("miles_amd.utils.mxfp8.native", Declines())
     theirs = everything()
     assert len(ours) == len(theirs) > 100 and all(torch.equal(p, q) for p, q in zip(ours, theirs))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_code_under_every_scale_in_the_weight_gradient(dtype):
+    """dW of one-hot gradients is the kept input itself: every code under every exponent, as the layer's dtype holds it."""
+    m, k = 255, 256 * 32
+    codes = torch.arange(256, dtype=torch.uint8, device=DEV).repeat_interleave(32).repeat(m, 1)
+    scales = torch.arange(m, dtype=torch.uint8, device=DEV).unsqueeze(1).expand(m, k // 32).contiguous()
+    nan = (codes & 0x7F) == 0x7F
+    codes[nan] = 0                                          # (a NaN would reach every row of its column)
+    dz = torch.eye(m, dtype=dtype, device=DEV)
+    dz8 = torch.zeros(m, 256, dtype=dtype, device=DEV)      # (columns a multiple of eight)
+    dz8[:, :m] = dz
+    for g, n in ((dz, m), (dz8, 256)):
+        dw = torch.empty(n, k, dtype=dtype, device=DEV)
+        ws = linear_module._workspace(2, g, codes, True, m, n, k)
+        _lib.check(_lib.load().mq_linear_weight_grad(g.data_ptr(), _lib.DTYPE_CODE[dtype], n, codes.data_ptr(), k, scales.data_ptr(), dw.data_ptr(), m, n, k,
+                                                     None if ws is None else ws.data_ptr(), None))
+        kept = restored64(codes.view(torch.float8_e4m3fn).cpu(), scales.cpu())
+        kept = (kept.clamp(-65504, 65504) if dtype == torch.float16 else kept).to(dtype)
+        want = dz.double().cpu().t() @ kept.double()        # (a value that bf16 holds as an infinity makes its column NaN, 0 times it)
+        got = dw[:m].double().cpu()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0, 1, 2), want.nan_to_num(0, 1, 2))
