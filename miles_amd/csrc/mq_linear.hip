@@ -72,62 +72,119 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const PadArgs a) {
 }
 
 // A few tokens (nq <= 16): what counts is reading the weight once, as fast as memory gives it.  A wavefront has 16 rows of the weight and
-// a share of k; its loads go straight into the operands of the matrix instruction (a lane's 16 elements of each 64 are neighbours, in
-// both operands, so that one load touches whole lines), and the eight wavefronts' sums meet in shared memory.
+// a share of k, in steps of 64, and the wavefronts' sums meet in shared memory.  A step's 128 bytes of each row come into shared memory,
+// in a ring of the wavefront's own (no barrier), eight lanes to a row: loads straight into the operands of the matrix instruction have
+// neighbouring lanes in different rows and pay for each.  Those took, with a weight of 9728 x 2560 that comes from memory, 13.6 us for one
+// token and 20.7 us for sixteen; this takes 12.2 and 14.5 (4.1 and 3.4 TB/s); with 151936 x 2560 141 us and 125 (6.2 TB/s).
+// DIRECT (aligned rows): straight into shared memory, three steps ahead of the one that is worked on.  Rings of three steps took 16.1 us
+// instead of 12.6 with 2560 x 9728, rings of eight 15.2 instead of 12.2 with 9728 x 2560 and 169 instead of 125 with 151936 x 2560, where
+// fewer workgroups are on a compute unit; eight wavefronts 15.2 instead of 12.2.  Rows at other addresses come through registers, four
+// steps at a time: 9727 x 2559 in 27 us for one token and 35 for sixteen, 2560 x 9729 in 25 and 28, where a copy with aligned rows and the
+// tiles of the other kernels take 36 to 37 (the operand's own layout straight from memory: 28, 49, 33 and 60).
 struct FewArgs {
     GemmArgs g;
     int64_t k_wave;            // k of a wavefront, a multiple of 64
 };
-constexpr int kFewWaves = 8;
-template <int D>
+constexpr int kFewWaves = 4, kFewRing = 4;
+template <int D, bool DIRECT>
 __global__ __launch_bounds__(kFewWaves * kWave) void few_rows_kernel(const FewArgs f) {
     const GemmArgs& a = f.g;
-    __shared__ float sums[kFewWaves][16][17];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, j = lane & 15, g = lane >> 4;
+    constexpr int kOperand = 16 * 128, kBuffer = 2 * kOperand;
+    __shared__ __attribute__((aligned(1024))) char shared[kFewWaves * kFewRing * kBuffer];
+    static_assert(sizeof(shared) >= kFewWaves * 16 * 17 * 4, "the sums fit");
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), j = lane & 15, g = lane >> 4;
     const int64_t p0 = (int64_t)blockIdx.x * 16;
     const int64_t k0 = wave * f.k_wave < a.k ? wave * f.k_wave : a.k, k1 = k0 + f.k_wave < a.k ? k0 + f.k_wave : a.k;
-    const char* p = a.p + (p0 + j < a.np ? p0 + j : a.np - 1) * a.ldp * 2;
-    const char* q = a.q + (j < a.nq ? j : a.nq - 1) * a.ldq * 2;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    int64_t k = k0;
-    constexpr int kAhead = 4;                              // loads of 64 k at once
-    for (; k + 64 * kAhead <= k1; k += 64 * kAhead) {
-        u32x4 vp[kAhead][2], vq[kAhead][2];
+    const int span = (int)(k1 - k0), steps = (span + 63) / 64;
+    const char *p = a.p + (p0 * a.ldp + k0) * 2, *q = a.q + k0 * 2;
+    MQ_LDS char* lds = (MQ_LDS char*)shared + wave * (kFewRing * kBuffer);
+    // 16 bytes for each lane, eight rows at a time; the pieces of a row are in an order that spreads the reads over the banks
+    int64_t at_p[2], at_q[2];
+    int piece[2];
 #pragma unroll
-        for (int i = 0; i < kAhead; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                vp[i][h] = ld16_at2(p + (k + i * 64 + g * 16 + h * 8) * 2);
-                vq[i][h] = ld16_at2(q + (k + i * 64 + g * 16 + h * 8) * 2);
-            }
-#pragma unroll
-        for (int i = 0; i < kAhead; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) acc = mfma<D>(vp[i][h], vq[i][h], acc);
+    for (int u = 0; u < 2; u++) {
+        const int at = lane + u * kWave, row = at >> 3;
+        piece[u] = (at & 7) ^ (at >> 4 & 7);
+        at_p[u] = (p0 + row < a.np ? row : a.np - 1 - p0) * a.ldp * 2;
+        at_q[u] = (row < a.nq ? row : a.nq - 1) * a.ldq * 2;
     }
-    for (; k < k1; k += 64) {
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto products = [&](MQ_LDS char* from) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int64_t c = k + g * 16 + h * 8;
-            acc = mfma<D>(ld_row<D>(p, c, k1), ld_row<D>(q, c, k1), acc);
+            const uint32_t at = (uint32_t)(j * 128 + ((g + 4 * h) ^ (j >> 1 & 7)) * 16);
+            acc = mfma<D>(*(MQ_LDS const u32x4*)(from + at), *(MQ_LDS const u32x4*)(from + kOperand + at), acc);
+        }
+    };
+    if (DIRECT) {
+        const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
+        auto ask = [&](int t) {                            // the same number of accesses for every step, also behind the last
+            const int left = span - t * 64;
+            const uint32_t to = lds0 + (uint32_t)(t % kFewRing) * kBuffer;
+            const u32x4 from_p = buffer_of(p + (int64_t)t * 128), from_q = buffer_of(q + (int64_t)t * 128);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const bool inside = piece[u] * 8 < left, is_row = ((lane + u * kWave) >> 3) < a.nq;
+                direct16(to + u * 1024, from_p, inside ? (uint32_t)at_p[u] + piece[u] * 16 : kNowhere);
+                direct16(to + kOperand + u * 1024, from_q, inside && is_row ? (uint32_t)at_q[u] + piece[u] * 16 : kNowhere);
+            }
+        };
+#pragma unroll
+        for (int t = 0; t < kFewRing - 1; t++) ask(t);
+        for (int t = 0; t < steps; t++) {
+            // this step has arrived, and the reads of the one before are done, whose buffer is the next to be filled
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((kFewRing - 2) * 4) : "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            ask(t + kFewRing - 1);
+            products(lds + (t % kFewRing) * kBuffer);
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    } else {
+        u32x4 vp[kFewRing][2], vq[kFewRing][2];
+        auto ask = [&](int t) {
+            if (t >= steps) return;
+            const bool whole = (t + kFewRing) * 64 <= span;
+#pragma unroll
+            for (int i = 0; i < kFewRing; i++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int64_t c = (t + i) * 64 + piece[u] * 8;
+                    vp[i][u] = whole ? ld16_at2(p + at_p[u] + c * 2) : ld_row<D>(p + at_p[u], c, span);
+                    vq[i][u] = whole ? ld16_at2(q + at_q[u] + c * 2) : ld_row<D>(q + at_q[u], c, span);
+                }
+        };
+        ask(0);
+        for (int t = 0; t < steps; t += kFewRing) {
+#pragma unroll
+            for (int i = 0; i < kFewRing; i++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    *(MQ_LDS u32x4*)(lds + i * kBuffer + (lane + u * kWave) * 16) = vp[i][u];
+                    *(MQ_LDS u32x4*)(lds + i * kBuffer + kOperand + (lane + u * kWave) * 16) = vq[i][u];
+                }
+            ask(t + kFewRing);
+#pragma unroll
+            for (int i = 0; i < kFewRing; i++) products(lds + i * kBuffer);
         }
     }
+    __syncthreads();
+    float* sums = (float*)shared;                          // [wave][row of x][17]
 #pragma unroll
-    for (int x = 0; x < 4; x++) sums[wave][j][g * 4 + x] = acc[x];
+    for (int x = 0; x < 4; x++) sums[(wave * 16 + j) * 17 + g * 4 + x] = acc[x];
     __syncthreads();
     const int row = threadIdx.x / 16, c = threadIdx.x % 16;
-    if (row < a.nq && p0 + c < a.np) {                     // (rows 16 and on are no rows)
-        float z = 0.0f;
+    static_assert(kFewWaves * kWave == 256, "a thread for each output");
+    if (row >= a.nq || p0 + c >= a.np) return;
+    float z = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kFewWaves; w++) z += sums[w][row][c];
-        const int64_t at = row * a.np + p0 + c;
-        if (a.bias) z += one_elem<D>(a.bias, p0 + c);
-        if (a.z) store_dtype(a.z, at, z, D);
-        float y = z;
-        with_activation(a.act, [&](auto kind) { y = activate<decltype(kind)::value>(z); });
-        if (a.res) y += one_elem<D>(a.res, row * a.ldr + p0 + c);
-        store_dtype(a.out, at, y, D);
-    }
+    for (int w = 0; w < kFewWaves; w++) z += sums[(w * 16 + row) * 17 + c];
+    const int64_t at = row * a.np + p0 + c;
+    if (a.bias) z += one_elem<D>(a.bias, p0 + c);
+    if (a.z) store_dtype(a.z, at, z, D);
+    float y = z;
+    with_activation(a.act, [&](auto kind) { y = activate<decltype(kind)::value>(z); });
+    if (a.res) y += one_elem<D>(a.res, row * a.ldr + p0 + c);
+    store_dtype(a.out, at, y, D);
 }
 
 struct ActGradArgs {
@@ -361,9 +418,12 @@ extern "C" int mq_linear_forward(const void* x, int dtype, int64_t ldx, const vo
     a.z = (char*)z, a.zq = (uint8_t*)z8, a.zs = z8_scale, a.act = act;
     if (product.few) {
         few.k_wave = (K + kFewWaves * 64 - 1) / (kFewWaves * 64) * 64;
-        const dim3 grid((unsigned)((N + 15) / 16));
-        if (dtype == MQ_F16) hipLaunchKernelGGL(few_rows_kernel<MQ_F16>, grid, dim3(kFewWaves * kWave), 0, st, few);
-        else hipLaunchKernelGGL(few_rows_kernel<MQ_BF16>, grid, dim3(kFewWaves * kWave), 0, st, few);
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)((N + 15) / 16)), dim3(kFewWaves * kWave), 0, st, few); };
+        if (direct_ok(x, M > 1 ? ldx : 8, K) && direct_ok(weight, N > 1 ? ldw : 8, K)) {
+            go(dtype == MQ_F16 ? few_rows_kernel<MQ_F16, true> : few_rows_kernel<MQ_BF16, true>);
+        } else {
+            go(dtype == MQ_F16 ? few_rows_kernel<MQ_F16, false> : few_rows_kernel<MQ_BF16, false>);
+        }
         return mq_check_launch("linear");
     }
     if (const int rc = mq_gemm_forward(dtype, a, product.plan, (float*)ws, st)) return rc;
