@@ -138,14 +138,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     act = ACTIVATIONS[activation]
     codes = scales = None
     if isinstance(checkpoint, ActCheckpoint):
-        if checkpoint.shape != x.shape or checkpoint.codes.device != x.device:
-            raise ValueError(f"linear: a checkpoint of shape {tuple(checkpoint.shape)} on {checkpoint.codes.device} for an input of shape "
-                             f"{tuple(x.shape)} on {x.device}")
-        check_width(k, what)
-        m = math.prod(x.shape[:-1])
-        codes, scales = checkpoint.codes.reshape(m, k).contiguous(), checkpoint.scales.reshape(m, k // MXFP8_GROUP_SIZE).contiguous()
-        if codes.data_ptr() % 16:
-            codes = codes.clone()
+        codes, scales = checkpoint.matrices(x.shape, x.device, what)
     elif checkpoint is not True and checkpoint is not False:
         raise ValueError(f"linear: checkpoint is True, False or an ActCheckpoint, got {type(checkpoint).__name__}")
     keep = checkpoint is not False

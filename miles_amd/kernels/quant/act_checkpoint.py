@@ -11,6 +11,8 @@ by at most half an e4m3 step, 2^-4 of the value (or 2^-10 of the group's scale, 
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from miles_amd import _lib, launch
@@ -37,6 +39,20 @@ class ActCheckpoint:
     def restore(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The values the codes stand for, in `dtype` (as they came, by default)."""
         return mxfp8_dequantize(self.codes, self.scales, self.dtype if dtype is None else dtype)
+
+    def matrices(self, shape: torch.Size, device: torch.device, what: str) -> tuple[torch.Tensor, torch.Tensor]:
+        """(codes [M, K], scales [M, K/32]) for a kernel that takes them as the copy of a tensor of this shape on this device."""
+        codes, scales = self.codes, self.scales
+        if codes.shape != shape or codes.device != device or scales.device != device:
+            raise ValueError(f"{what}: a checkpoint of shape {tuple(codes.shape)} on {codes.device} (scales on {scales.device}) for an input "
+                             f"of shape {tuple(shape)} on {device}")
+        check_width(shape[-1], what)
+        if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8 or scales.shape != (*shape[:-1], shape[-1] // MXFP8_GROUP_SIZE):
+            raise ValueError(f"{what}: a checkpoint of {codes.dtype} codes and {scales.dtype} scales of shape {tuple(scales.shape)}, not of "
+                             f"float8_e4m3fn codes and a uint8 scale for each {MXFP8_GROUP_SIZE} of a row")
+        m = math.prod(shape[:-1])
+        codes = codes.reshape(m, shape[-1]).contiguous()
+        return codes if codes.data_ptr() % 16 == 0 else codes.clone(), scales.reshape(m, shape[-1] // MXFP8_GROUP_SIZE).contiguous()
 
     def __repr__(self) -> str:
         return f"ActCheckpoint(shape={tuple(self.shape)}, dtype={self.dtype}, device={self.codes.device})"

@@ -29,6 +29,20 @@ def test_width_of_an_8_bit_copy():
         check_width(48, "linear")
 
 
+def test_a_checkpoint_that_is_not_the_inputs():
+    codes, scales = torch.zeros(2, 3, 64, dtype=torch.float8_e4m3fn), torch.zeros(2, 3, 2, dtype=torch.uint8)
+    q, s = ActCheckpoint(codes, scales, BF16).matrices(codes.shape, codes.device, "linear")
+    assert q.shape == (6, 64) and s.shape == (6, 2)
+    off = torch.zeros(6 * 64 + 1, dtype=torch.uint8)[1:].view(torch.float8_e4m3fn).view(2, 3, 64)
+    assert ActCheckpoint(off, scales, BF16).matrices(codes.shape, codes.device, "linear")[0].data_ptr() % 16 == 0
+    for q, s, shape, text in ((codes, scales, (6, 64), "a checkpoint of shape"), (codes.to("meta"), scales, codes.shape, "on meta"),
+                              (codes, scales.to("meta"), codes.shape, "scales on meta"), (codes, scales.int(), codes.shape, "uint8"),
+                              (codes.half(), scales, codes.shape, "float8_e4m3fn"), (codes, scales[:, :2], codes.shape, "scales of shape"),
+                              (codes, scales[..., :1], codes.shape, "scales of shape"), (codes[..., :48], scales, (2, 3, 48), "groups of 32")):
+        with pytest.raises(ValueError, match=text):
+            ActCheckpoint(q, s, BF16).matrices(torch.Size(shape), torch.device("cpu"), "linear")
+
+
 P = 0x1000      # a pointer that no refused call follows
 
 
