@@ -320,6 +320,12 @@ __device__ __forceinline__ void meet() {
     asm volatile("" ::: "memory");
 }
 
+// what a wavefront's lanes have written to shared memory is there for its other lanes, and what they have read may be overwritten
+__device__ __forceinline__ void lanes_meet() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // What follows the sums, from shared memory: 64 columns of ROWS rows of one wavefront, in fp32, four columns at position
 // (column / 4) ^ (row & 15) of a row's sixteen.  A lane has eight columns, so that eight lanes store whole lines.
 __device__ __forceinline__ int stage_at(int row, int four) { return row * 256 + ((four ^ (row & 15)) * 16); }
@@ -541,9 +547,11 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
                         const f32x16& c = acc[2 * half + i][j];
                         *(MQ_LDS f32x4*)(stage + stage_at(j * 32 + row, i * 8 + x * 2 + four)) = f32x4{c[4 * x], c[4 * x + 1], c[4 * x + 2], c[4 * x + 3]};
                     }
+            lanes_meet();
             finish_block<D, EPILOGUE, TQ>(a, sums ? sums + half * 64 : nullptr, BP, q0 + wq * TQ, p0 + wp * TP + half * 64, stage);
         };
         finish_half(std::integral_constant<int, 0>{});
+        lanes_meet();
         finish_half(std::integral_constant<int, 1>{});
     } else {
         Fragments<PM, BP, FP> fp;
@@ -593,6 +601,7 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
         for (int i = 0; i < FP; i++)
 #pragma unroll
             for (int j = 0; j < FQ; j++) *(MQ_LDS f32x4*)(stage + stage_at(j * 16 + (lane & 15), i * 4 + (lane >> 4))) = acc[i][j];
+        lanes_meet();
         finish_block<D, EPILOGUE, TQ>(a, sums, BP, q0 + wq * TQ, p0 + wp * TP, stage);
     }
 }

@@ -163,8 +163,10 @@ __global__ __launch_bounds__(kFewWaves * kWave) void few_rows_kernel(const FewAr
                     *(MQ_LDS u32x4*)(lds + i * kBuffer + kOperand + (lane + u * kWave) * 16) = vq[i][u];
                 }
             ask(t + kFewRing);
+            lanes_meet();
 #pragma unroll
             for (int i = 0; i < kFewRing; i++) products(lds + i * kBuffer);
+            lanes_meet();
         }
     }
     __syncthreads();

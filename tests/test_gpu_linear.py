@@ -144,6 +144,18 @@ def test_rows_apart_with_nan_between(m, n, k, left, right):
     assert torch.equal(gr, dy0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [1, 2, 7, 16])
+@pytest.mark.parametrize("n,k", [(17, 1543), (33, 2048), (40, 1096), (16, 255), (1, 256), (15, 257), (160, 4104)])
+def test_a_few_tokens_with_nan_around_their_rows(m, n, k, dtype):
+    g = torch.Generator().manual_seed(m + k)
+    x0, w0 = _whole(g, m, k, dtype=dtype), _whole(g, n, k, dtype=dtype)
+    want = f64((f64(x0) @ f64(w0).t()).to(dtype))
+    for left, right in ((0, 0), (8, 8 - k % 8), (3, 2), (1, 0)):
+        assert torch.equal(f64(linear(_in_nan(x0, left, right), _in_nan(w0, left, right))), want), (left, right)
+    assert torch.equal(f64(linear(x0, _in_nan(w0, 5, 0))), want)
+
+
 def test_strides_and_shapes():
     g = torch.Generator().manual_seed(4)
     big, w = _whole(g, 4, 6, 96, dtype=torch.bfloat16), _whole(g, 40, 64, dtype=torch.bfloat16)
