@@ -18,7 +18,7 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs a, int bp
     float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (inside) {
         const float* from = a.ws + (int64_t)nth * a.splits * bp * bq + r * bp + c;
-        // eight parts' loads at once: their sum is short, and each would wait for memory by itself
+        // eight parts' loads at once (48 x 2560 x 9728 in twelve parts: 4.8 us, and 8.8 by one load after the other)
         constexpr int kAtOnce = 8;
         for (int s0 = 0; s0 < a.splits; s0 += kAtOnce) {
             f32x4 v[kAtOnce];
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs a, int bp
 }
 
 // Operands whose rows do not begin at multiples of 16 bytes, or do not end with a whole piece of eight elements, copied so that they do,
-// zeros behind a row's end; blockIdx.y: which of the two.
+// zeros behind a row's end; blockIdx.y: which of the two.  A wavefront to a row: 777 x 1545 and 1003 x 1545 in 5.8 us.
 struct PadArgs {
     const char* from[2];
     char* to[2];
@@ -200,7 +200,9 @@ struct ActGradArgs {
 };
 
 // dz = dy act'(z) and the sums of its columns.  A wavefront goes down rows of 512 columns, eight to a lane, so that a column's sum
-// stays in a register; the four wavefronts of a workgroup take turns and their sums meet in shared memory.
+// stays in a register; the four wavefronts of a workgroup take turns and their sums meet in shared memory.  Near what
+// memory allows, the slope's arithmetic close behind it: 8192 x 9728 bf16, GELU from 8 bits 82 us (4.9 TB/s), from 16 bits 99 (4.8), the
+// bias alone 31 (5.2); two or four rows' loads at once are no faster.
 template <int D, int KEPT>
 __global__ __launch_bounds__(256) void activation_bwd_kernel(const ActGradArgs a) {
     __shared__ float sums[4][8][kWave + 1];
@@ -211,50 +213,28 @@ __global__ __launch_bounds__(256) void activation_bwd_kernel(const ActGradArgs a
     for (int j = 0; j < 8; j++) db[j] = 0.0f;
     with_activation(a.act, [&](auto kind) {
         constexpr int ACT = decltype(kind)::value;
-        const int64_t step = (int64_t)gridDim.y * 4;
-        constexpr int kAtOnce = 2;
-        for (int64_t row0 = (int64_t)blockIdx.y * 4 + wave; row0 < a.rows; row0 += step * kAtOnce) {
-            u32x4 dy[kAtOnce], zv[kAtOnce];
-            uint32_t e[kAtOnce];
-#pragma unroll
-            for (int i = 0; i < kAtOnce; i++) {
-                const int64_t row = row0 + i * step;
-                dy[i] = zv[i] = u32x4{0u, 0u, 0u, 0u};
-                e[i] = 0;
-                if (row >= a.rows) continue;
-                dy[i] = ld_row<D>(a.dy + row * a.lddy * 2, col, a.n);
-                if (ACT != MQ_ACT_NONE && KEPT) {
+        for (int64_t row = (int64_t)blockIdx.y * 4 + wave; row < a.rows; row += (int64_t)gridDim.y * 4) {
+            float g[8], z[8];
+            unpack<D>(ld_row<D>(a.dy + row * a.lddy * 2, col, a.n), g);
+            if (ACT != MQ_ACT_NONE) {
+                if (!KEPT) {
+                    unpack<D>(ld_row<D>(a.z + row * a.n * 2, col, a.n), z);
+                } else {
+                    u32x2 c = {0u, 0u};
+                    float s = 0.0f;
                     if (col < a.n) {
-                        const u32x2 c = *(const u32x2*)(a.z + row * a.n + col);
-                        zv[i].x = c.x, zv[i].y = c.y;
-                        e[i] = a.zs[row * (a.n / 32) + col / 32];
+                        c = *(const u32x2*)(a.z + row * a.n + col);
+                        s = e8m0_value(a.zs[row * (a.n / 32) + col / 32]);
                     }
-                } else if (ACT != MQ_ACT_NONE) {
-                    zv[i] = ld_row<D>(a.z + row * a.n * 2, col, a.n);
+                    kept_values4(c.x, s, z);
+                    kept_values4(c.y, s, z + 4);
                 }
+#pragma unroll
+                for (int j = 0; j < 8; j++) g[j] *= slope<ACT>(z[j]);
             }
+            if (a.dz) st_row<D>(a.dz + row * a.n * 2, col, a.n, pack<D>(g));
 #pragma unroll
-            for (int i = 0; i < kAtOnce; i++) {
-                const int64_t row = row0 + i * step;
-                if (row >= a.rows) break;
-                float g[8];
-                unpack<D>(dy[i], g);
-                if (ACT != MQ_ACT_NONE) {
-                    float z[8];
-                    if (KEPT) {
-                        const float s = e8m0_value(e[i]);
-                        kept_values4(zv[i].x, s, z);
-                        kept_values4(zv[i].y, s, z + 4);
-                    } else {
-                        unpack<D>(zv[i], z);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; j++) g[j] *= slope<ACT>(z[j]);
-                }
-                if (a.dz) st_row<D>(a.dz + row * a.n * 2, col, a.n, pack<D>(g));
-#pragma unroll
-                for (int j = 0; j < 8; j++) db[j] += g[j];
-            }
+            for (int j = 0; j < 8; j++) db[j] += g[j];
         }
     });
     if (!a.part) return;
@@ -277,7 +257,9 @@ using namespace mq;
 // How a product of np columns, nq rows and k runs: the tile, and which tiles are cut along k.  Tiles that fill every place on the card
 // run whole, round by round; those of a last round that would leave places empty (all of them, of a small product) are cut into as
 // many parts as fill it.  Each candidate's time is estimated from its rounds and the bytes of its partial sums; the constants were
-// fitted to 40 products measured with every tile and up to ten numbers of parts, where the choice loses 2 % against the best.
+// fitted to 40 products measured with every tile and up to ten numbers of parts, where the choice loses 2 % against the best.  Some of
+// them (M x N x K, us by 256 x 256, 128 x 128, 128 x 64): 4099 x 2560 x 4096 92, 105, 116; 12544 x 1152 x 2192 70, 85, 104;
+// 2048 x 2048 x 2048 41, 32, 26; 512 x 4096 x 4096 40, 34, 33, and uncut 76, 53, 43; 48 x 2560 x 9728 28, 24, 19, and uncut 156, 115, 93.
 static GemmPlan gemm_plan(int64_t np, int64_t nq, int64_t k) {
     struct Cost {
         int per_cu;
@@ -375,7 +357,8 @@ struct Product {
         return MQ_OK;
     }
 };
-// few tokens, and nothing that needs 32 columns at once
+// few tokens, and nothing that needs 32 columns at once (sixteen, with 9728 x 2560: 14.5 us, by tiles 17.1; the same kernel with two
+// such operands took 20.9 us for 32 with 2560 x 9728, tiles 18.3)
 static bool few_rows(int product, int64_t M, bool z8) { return product == MQ_LINEAR_FORWARD && M <= 16 && !z8; }
 
 static int check_product(int product, const void* a, int64_t lda, const void* b, int64_t ldb, bool kept, int64_t M, int64_t N, int64_t K) {

@@ -163,7 +163,8 @@ __global__ __launch_bounds__(256) void mxfp8_generic_kernel(const void* __restri
 
 // The way back: code x 2^(e - 127), rounded once to the output's type (for bf16 and fp32 there is nothing to round outside
 // the subnormals).  A finite value that fp16 cannot hold becomes its largest: the code above 65504 stands for a value below it.
-// A lane stores 16 bytes per unit, from one load of eight (16-bit outputs) or four codes, all loads before the first use.
+// A lane stores 16 bytes per unit, from one load of eight (16-bit outputs) or four codes, all loads before the first use.  Bound by HBM:
+// with the quantizer before it, 16384 x 7168 fp32 there and back in 178 us (6.6 TB/s), 4099 x 2560 bf16 in 15.5.
 constexpr int kMxBackUnits = 2;
 template <int D>
 __global__ __launch_bounds__(256) void mxfp8_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale, char* __restrict__ y,

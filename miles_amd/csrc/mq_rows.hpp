@@ -15,7 +15,7 @@ constexpr int kElem = D == MQ_F32 ? 4 : 2;
 template <int D>
 __device__ __forceinline__ float one_elem(const void* p, int64_t i) { return load_f32(p, i, D); }
 
-// kVec elements from any element boundary
+// kVec elements as floats
 template <int D>
 __device__ __forceinline__ void unpack(u32x4 v, float* f) {
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -75,17 +75,6 @@ __device__ __forceinline__ void st_row(void* row, int64_t c, int64_t n, u32x4 v)
             if (D == MQ_F32) ((uint32_t*)row)[c + j] = u[j & 3];
             else ((uint16_t*)row)[c + j] = (uint16_t)(u[j / 2] >> (16 * (j & 1)));
         }
-    }
-}
-// V elements of a vector that is fp32 (WF32) or of type D, zero from n on
-template <int D, int WF32>
-__device__ __forceinline__ void ld_vector(const void* p, int64_t c, int64_t n, float* f) {
-    constexpr int V = kVec<D>;
-    if (WF32) {
-#pragma unroll
-        for (int j = 0; j < V; j += 4) unpack<MQ_F32>(ld_row<MQ_F32>(p, c + j, n), f + j);
-    } else {
-        unpack<D>(ld_row<D>(p, c, n), f);
     }
 }
 
