@@ -199,7 +199,9 @@ struct ActGradArgs {
     int act;
 };
 
-// dz = dy act'(z) and the sums of its columns.  A wavefront goes down rows of 512 columns, eight to a lane, so that a column's sum
+// dz = dy act'(z) and the sums of its columns.  dz is rounded to the tensors' type, because the matrix instructions that take it further
+// have 16-bit operands (a gradient's error is then that of two such roundings, 2.3e-3 of its size in bf16 where one makes 1.7e-3); the
+// sums are of what was not rounded.  A wavefront goes down rows of 512 columns, eight to a lane, so that a column's sum
 // stays in a register; the four wavefronts of a workgroup take turns and their sums meet in shared memory.  Near what
 // memory allows, the slope's arithmetic close behind it: 8192 x 9728 bf16, GELU from 8 bits 82 us (4.9 TB/s), from 16 bits 99 (4.8), the
 // bias alone 31 (5.2); two or four rows' loads at once are no faster.

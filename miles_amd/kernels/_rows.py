@@ -5,6 +5,15 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
+
+
+def wants_graph(*tensors: torch.Tensor | None) -> bool:
+    """Whether a result of these tensors belongs to a graph; also where one carries a forward-mode derivative, which a graph node refuses."""
+    given = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        return True
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in given)
 
 
 def rows(t: torch.Tensor) -> torch.Tensor:

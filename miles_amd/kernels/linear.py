@@ -16,7 +16,7 @@ from torch.autograd.function import once_differentiable
 
 from miles_amd import _lib, launch
 from miles_amd._host import native
-from miles_amd.kernels._rows import address, pitch, rows
+from miles_amd.kernels._rows import address, pitch, rows, wants_graph
 from miles_amd.kernels.quant.act_checkpoint import MXFP8_GROUP_SIZE, ActCheckpoint, check_width, keep8
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}      # MQ_ACT_*
@@ -147,7 +147,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         if act:
             check_width(n, what)
     bias = bias.contiguous() if bias is not None else None
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if wants_graph(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, act, keep, codes, scales)
     y = _forward(rows(x), rows(weight), bias, act, rows(residual) if residual is not None else None, False, False)[0]
     return y.view(*x.shape[:-1], n)

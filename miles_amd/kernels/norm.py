@@ -16,7 +16,7 @@ from torch.autograd.function import once_differentiable
 
 from miles_amd import _lib, launch
 from miles_amd._host import native
-from miles_amd.kernels._rows import address, pitch, rows_like_contiguous
+from miles_amd.kernels._rows import address, pitch, rows_like_contiguous, wants_graph
 from miles_amd.kernels.quant.act_checkpoint import MXFP8_GROUP_SIZE, ActCheckpoint, check_width
 
 
@@ -104,7 +104,7 @@ def _norm(what, x, weight, bias, eps, rms, checkpoint, output_checkpoint):
     weight = weight.contiguous() if weight is not None else None
     bias = bias.contiguous() if bias is not None else None
     eps, rms, copy = float(eps), bool(rms), bool(output_checkpoint)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if wants_graph(x, weight, bias):
         y, yq, ys = _Norm.apply(x, weight, bias, eps, rms, bool(checkpoint), copy)
     else:
         y, _mean, _rstd, _xq, _xs, yq, ys = _forward(x, weight, bias, eps, rms, False, False, copy)

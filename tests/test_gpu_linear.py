@@ -347,6 +347,16 @@ def test_refusals():
         torch.autograd.grad(g.sum(), x)
 
 
+def test_forward_mode_derivatives_are_refused():
+    x, w, _b, _r, _dy = (t.detach() for t in _random(4, 64, 32, torch.bfloat16, seed=15))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: linear(dual, w), lambda: rms_norm(dual)):
+            with pytest.raises((NotImplementedError, RuntimeError)):
+                call()
+        assert torch.equal(linear(x, w), linear(x.clone(), w))
+
+
 def test_native_and_python_host_layers_agree(monkeypatch):
     """An ordinary call makes its graph node in native code, any other in Python: the same bits, and only what asks has a gradient."""
     from miles_amd.kernels import norm as norm_mod
