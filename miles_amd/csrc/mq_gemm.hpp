@@ -419,11 +419,19 @@ __device__ __forceinline__ void finish_block(const GemmArgs& a, float* sums, int
     });
 }
 
+// Buffers of a smaller tile: three of the 128 x 64 one and two workgroups on a compute unit, except in the weight gradient, whose sum is
+// short where this tile is chosen, two and three.  (48 x 2560 x 9728 in us with two and three buffers: forward 18.6 and 16.6, input
+// gradient 17.7 and 16.0, weight gradient 18 and 23; 512 x 2048 x 2048 forward 20.7 and 18.4.  Four and six buffers leave one workgroup:
+// 48 x 2560 x 9728 forward 17 and 18, 2048^3 35 and 37 where three take 25.  The 128 x 128 tile with three: weight gradient of
+// 200 x 2560 x 2560 14.8 for 10.7.)
+constexpr int small_ring(int bq, bool weight_grad) { return bq == 64 && !weight_grad ? 3 : 2; }
+
 template <int D, int PM, int QM, int BP, int BQ, int WP, int WQ, bool EPILOGUE>
 __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1))) void gemm_kernel(const GemmArgs a) {
     constexpr int kThreads = WP * WQ * kWave, TP = BP / WP, TQ = BQ / WQ, FP = TP / 16, FQ = TQ / 16;
     constexpr int kPBytes = BP * kStep * 2, kQBytes = BQ * kStep * 2, kBuffer = kPBytes + kQBytes;
-    __shared__ __attribute__((aligned(1024))) char shared[BP == 256 ? 5 * kPBytes : 2 * kBuffer];
+    constexpr int kRing = small_ring(BQ, QM == kDown);     // buffers of a smaller tile
+    __shared__ __attribute__((aligned(1024))) char shared[BP == 256 ? 5 * kPBytes : kRing * kBuffer];
     MQ_LDS char* lds = (MQ_LDS char*)shared;
     const uint32_t lds0 = (uint32_t)(uintptr_t)lds;
     int tile, part, tp, tq;
@@ -571,21 +579,29 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
         for (int i = 0; i < FP; i++)
 #pragma unroll
             for (int j = 0; j < FQ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        // Several workgroups on a compute unit, two buffers each.  While step t is worked on, step t + 1 is on its way; what goes through
-        // registers was loaded a step earlier.
-        fetch_p(0, lds0);
-        fetch_q(0, lds0 + kPBytes);
-        sp.settle();
-        put_p(lds);
-        if (!kPDirect) fetch_p(1, 0);
+        // Several workgroups on a compute unit, two or three buffers each.  While step t is worked on, the next one or two are on their
+        // way; what goes through registers was loaded a step earlier.
+        static_assert(kPDirect || kRing == 2, "the registers hold the step after the next");
+#pragma unroll
+        for (int t = 0; t < kRing - 1; t++) {
+            fetch_p(t, lds0 + t * kBuffer);
+            fetch_q(t, lds0 + t * kBuffer + kPBytes);
+        }
+        if (!kPDirect) {
+            sp.settle();
+            put_p(lds);
+            fetch_p(1, 0);
+        }
+        uint32_t at = 0;                                    // the buffer of step t
         for (int t = 0; t < steps; t++) {
-            MQ_LDS char* from = lds + (t & 1) * kBuffer;
-            const uint32_t next = (uint32_t)(t + 1 & 1) * kBuffer;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            MQ_LDS char* from = lds + at;
+            const uint32_t before = at == 0 ? (kRing - 1) * kBuffer : at - kBuffer;
+            // this step has arrived, and everybody has read the one before, whose buffer is the next to be filled
+            asm volatile("s_waitcnt vmcnt(%0)" ::"i"((kRing - 2) * (sp.kUnits + sq.kUnits)) : "memory");
             meet();
             sp.settle();
-            fetch_q(t + 1, lds0 + next + kPBytes);
-            if (kPDirect) fetch_p(t + 1, lds0 + next);
+            fetch_q(t + kRing - 1, lds0 + before + kPBytes);
+            if (kPDirect) fetch_p(t + kRing - 1, lds0 + before);
             else fetch_p(t + 2, 0);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -599,7 +615,8 @@ __global__ __launch_bounds__(WP* WQ* kWave) __attribute__((amdgpu_waves_per_eu(1
 #pragma unroll
                     for (int j = 0; j < FQ; j++) acc[i][j] = mfma<D>(p[i], q[j], acc[i][j]);
             }
-            if (!kPDirect) put_p(lds + next);               // (behind the reads, which would wait for the writes)
+            if (!kPDirect) put_p(lds + before);             // (behind the reads, which would wait for the writes)
+            at = at == (kRing - 1) * kBuffer ? 0 : at + kBuffer;
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // (as above)
         meet();

@@ -259,20 +259,20 @@ using namespace mq;
 // How a product of np columns, nq rows and k runs: the tile, and which tiles are cut along k.  Tiles that fill every place on the card
 // run whole, round by round; those of a last round that would leave places empty (all of them, of a small product) are cut into as
 // many parts as fill it.  Each candidate's time is estimated from its rounds and the bytes of its partial sums; the constants were
-// fitted to 40 products measured with every tile and up to ten numbers of parts, where the choice loses 2 % against the best.  Some of
+// fitted to 44 products measured with every tile and up to ten numbers of parts, where the choice loses 1 % against the best.  Some of
 // them (M x N x K, us by 256 x 256, 128 x 128, 128 x 64): 4099 x 2560 x 4096 92, 105, 116; 12544 x 1152 x 2192 70, 85, 104;
-// 2048 x 2048 x 2048 41, 32, 26; 512 x 4096 x 4096 40, 34, 33, and uncut 76, 53, 43; 48 x 2560 x 9728 28, 24, 19, and uncut 156, 115, 93.
-static GemmPlan gemm_plan(int64_t np, int64_t nq, int64_t k) {
+// 2048 x 2048 x 2048 41, 32, 25; 512 x 4096 x 4096 40, 36, 34, and uncut 76, 54, 35; 48 x 2560 x 9728 26, 21, 17, and uncut 156, 114, 70.
+static GemmPlan gemm_plan(bool weight_grad, int64_t np, int64_t nq, int64_t k) {
     struct Cost {
         int per_cu;
         double least_us, step_us, tile_us;                // of a step, of a step for each workgroup on the compute unit, and besides the steps
     };
-    static const Cost costs[3] = {{1, 0.79, 0.93, 8.5}, {2, 0.68, 0.48, 3.2}, {3, 0.49, 0.34, 1.6}};
+    static const Cost costs[4] = {{1, 0.79, 0.93, 8.5}, {2, 0.68, 0.48, 3.2}, {2, 0.32, 0.32, 2.0}, {3, 0.49, 0.34, 1.6}};
     const int64_t steps = k > 0 ? (k + kStep - 1) / kStep : 1;
     GemmPlan best{};
     double best_us = 1e30;
     for (int t = kTileLarge; t <= kTileLow; t++) {
-        const Cost& cost = costs[t];
+        const Cost& cost = costs[t == kTileLow && weight_grad ? 3 : t];
         const int64_t tiles_p = (np + kTileP[t] - 1) / kTileP[t], tiles_q = (nq + kTileQ[t] - 1) / kTileQ[t];
         const int64_t tiles = tiles_p * tiles_q, places = 256 * cost.per_cu, rest = tiles % places;
         auto round_us = [&](int64_t count, int64_t n_steps) {      // so many workgroups at once, of so many steps
@@ -286,7 +286,7 @@ static GemmPlan gemm_plan(int64_t np, int64_t nq, int64_t k) {
             const int64_t parts = rest * splits;
             double us = whole_us + (double)(parts / places) * round_us(places, per);
             if (parts % places) us += round_us(parts % places, per);
-            if (splits > 1) us += 2.5 + (double)parts * kTileP[t] * (double)(nq < kTileQ[t] ? nq : kTileQ[t]) * 8 / 6.4e6;
+            if (splits > 1) us += 2.5 + (double)parts * kTileP[t] * (double)(nq < kTileQ[t] ? nq : kTileQ[t]) * 8 / 5.3e6;
             if (us < best_us) {
                 best_us = us;
                 best = GemmPlan{t, (int)tiles_p, (int)tiles_q, (int)(splits > 1 ? tiles - rest : tiles), (int)splits, per * kStep};
@@ -327,7 +327,7 @@ struct Product {
         p_rows = weight_grad ? M : N, p_cols = K;
         q_rows = M, q_cols = forward ? K : N;
         np = forward ? N : K, nq = weight_grad ? N : M, k = forward ? K : weight_grad ? M : N;
-        plan = few ? GemmPlan{} : gemm_plan(np, nq, k);
+        plan = few ? GemmPlan{} : gemm_plan(weight_grad, np, nq, k);
         bytes = few ? 0 : partial_floats(plan) * 4;
         p_at = few || kept ? -1 : copy_at(p, ldp, p_rows, p_cols);
         q_at = few ? -1 : copy_at(q, ldq, q_rows, q_cols);
@@ -360,7 +360,7 @@ struct Product {
     }
 };
 // few tokens, and nothing that needs 32 columns at once (sixteen, with 9728 x 2560: 14.5 us, by tiles 17.1; the same kernel with two
-// such operands took 20.9 us for 32 with 2560 x 9728, tiles 18.3)
+// such operands took 20.9 us for 32 with 2560 x 9728, where tiles take 15.8 for 17 and 17.0 for 48)
 static bool few_rows(int product, int64_t M, bool z8) { return product == MQ_LINEAR_FORWARD && M <= 16 && !z8; }
 
 static int check_product(int product, const void* a, int64_t lda, const void* b, int64_t ldb, bool kept, int64_t M, int64_t N, int64_t K) {
