@@ -684,6 +684,7 @@ PyMethodDef methods[] = {{"set_error", set_error, METH_O, nullptr},
                          {"keep8", keep8, METH_O, nullptr},
                          {"mxfp8_dequant", (PyCFunction)(void*)mxfp8_dequant, METH_FASTCALL, nullptr},
                          {"linear", (PyCFunction)(void*)linear, METH_FASTCALL, nullptr},
+                         {"once", (PyCFunction)(void*)once_of, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mq_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -41,11 +41,40 @@ at::Tensor one_run(const at::Tensor& t) {
     return (uintptr_t)c.data_ptr() % 16 == 0 ? c : c.clone();
 }
 at::Tensor scratch(int64_t bytes, const at::Tensor& like) { return bytes > 0 ? make({bytes}, at::kByte, like) : at::Tensor(); }
-// A gradient is taken once: where a graph of the backward pass itself is asked for, its results can not be differentiated again.
-torch::autograd::variable_list once(torch::autograd::variable_list grads, bool again, const char* what) {
-    if (!again) return grads;
-    auto refuse = std::make_shared<torch::autograd::DelayedError>(std::string(what) + ": gradients of gradients are not supported", (int64_t)grads.size());
-    return (*refuse)(std::move(grads));
+// Gradients are taken once: where a graph of the backward pass itself is asked for, those that the node now running has made are part of
+// one that refuses to be gone through, and as constants would leave what depends on them out of a second derivative.  Its edges are the
+// node's own and those of the incoming gradients, so that every way to an input that a gradient depends on meets the refusal, also where a
+// caller names the inputs whose gradients it wants.
+void once(torch::autograd::variable_list& made, const torch::autograd::variable_list& incoming, const char* what) {
+    const auto node = torch::autograd::get_current_node();
+    TORCH_CHECK(node, what, ": no backward pass is running");
+    torch::autograd::edge_list edges = node->next_edges();
+    for (const at::Tensor& g : incoming)
+        if (g.defined() && g.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(g));
+    const auto refuse = std::make_shared<torch::autograd::Error>(std::string(what) + ": gradients of gradients are not supported", std::move(edges));
+    for (at::Tensor& g : made) {
+        if (!g.defined()) continue;
+        g = g.detach();
+        torch::autograd::create_gradient_edge(g, refuse);
+    }
+}
+// once(list of gradients, list of incoming gradients, name of the operator) -> list of gradients
+PyObject* once_of(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 3 || !PyList_Check(a[0]) || !PyList_Check(a[1]) || !PyUnicode_Check(a[2])) return PyErr_Format(PyExc_TypeError, "once: (list, list, str)");
+    torch::autograd::variable_list lists[2];
+    for (int which = 0; which < 2; which++)
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[which]); i++) {
+            PyObject* t = PyList_GET_ITEM(a[which], i);
+            if (!THPVariable_Check(t)) return PyErr_Format(PyExc_TypeError, "once: lists of tensors");
+            lists[which].push_back(THPVariable_Unpack(t));
+        }
+    once(lists[0], lists[1], PyUnicode_AsUTF8(a[2]));
+    Owned out = owned(PyList_New((Py_ssize_t)lists[0].size()));
+    if (!out) return nullptr;
+    for (size_t i = 0; i < lists[0].size(); i++) PyList_SET_ITEM(out.ptr(), (Py_ssize_t)i, THPVariable_Wrap(lists[0][i]));
+    return out.release().ptr();
+    END_HANDLE_TH_ERRORS
 }
 
 // ---- norms -----------------------------------------------------------------------------------------------------------------
@@ -109,7 +138,10 @@ struct Norm : torch::autograd::Function<Norm> {
         checked(mq_norm_backward(dy.data_ptr(), dtype_code(dy.scalar_type()), n, x.data_ptr(), n, (const uint8_t*)pointer(xs), (const float*)pointer(mean),
                                  (const float*)pointer(rstd), pointer(w), dtype_code(vector), pointer(dx), pointer(dw), pointer(db),
                                  (float*)pointer(ws), m, n, rms, stream_of(dy)));
-        return once({dx, dw, db, at::Tensor()}, again, "norm");
+        torch::autograd::variable_list out{dx, dw, db};
+        if (again) once(out, grads, "norm");
+        out.resize(4);
+        return out;
     }
 };
 // norm(x, weight | None, bias | None, eps, rms, keep in 8 bits, copy of the result) -> y, (y, codes, scales) or None
@@ -269,7 +301,11 @@ struct Linear : torch::autograd::Function<Linear> {
                                               pointer(ws), stream));
             }
         }
-        return once({dx, dw, db, need_r ? grads[0] : at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()}, again, "linear");
+        torch::autograd::variable_list out{dx, dw, db};
+        if (again) once(out, grads, "linear");
+        out.push_back(need_r ? grads[0] : at::Tensor());    // (handed on as it is)
+        out.resize(8);
+        return out;
     }
 };
 // linear(x, weight, bias | None, activation code, residual | None, keep in 8 bits, codes | None, scales | None) -> y or None

@@ -2,10 +2,13 @@
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
 from torch.autograd import forward_ad
+
+from miles_amd._host import native
 
 
 def wants_graph(*tensors: torch.Tensor | None) -> bool:
@@ -14,6 +17,26 @@ def wants_graph(*tensors: torch.Tensor | None) -> bool:
     if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         return True
     return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in given)
+
+
+def gradients_once(what: str):
+    """For a `backward` whose gradients come out of kernels: where a graph of the backward pass itself is asked for
+    (`create_graph=True`), they are part of one that refuses to be gone through.  They would pass for constants otherwise, also where
+    the incoming gradient is one.  An incoming gradient that is handed on stays as it is."""
+    def wrap(backward):
+        @functools.wraps(backward)
+        def once(ctx, *grads):
+            again = torch.is_grad_enabled()
+            with torch.no_grad():
+                out = backward(ctx, *grads)
+            if not again:
+                return out
+            given = [g for g in grads if g is not None]
+            made = [o for o in out if o is not None and not any(o is g for g in given)]
+            refused = dict(zip(map(id, made), native.once(made, given, what)))
+            return tuple(refused.get(id(o), o) for o in out)
+        return once
+    return wrap
 
 
 def rows(t: torch.Tensor) -> torch.Tensor:

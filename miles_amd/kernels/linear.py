@@ -12,11 +12,10 @@ import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from miles_amd import _lib, launch
 from miles_amd._host import native
-from miles_amd.kernels._rows import address, pitch, rows, wants_graph
+from miles_amd.kernels._rows import address, gradients_once, pitch, rows, wants_graph
 from miles_amd.kernels.quant.act_checkpoint import MXFP8_GROUP_SIZE, ActCheckpoint, check_width, keep8
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}      # MQ_ACT_*
@@ -67,7 +66,7 @@ class _Linear(torch.autograd.Function):
         return y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
-    @once_differentiable
+    @gradients_once("linear")
     def backward(ctx, dy):
         kept, x_scales, z, z_scales, weight = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]

@@ -12,11 +12,10 @@ Gradients are deterministic: the rows' sums are added in an order that depends o
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from miles_amd import _lib, launch
 from miles_amd._host import native
-from miles_amd.kernels._rows import address, pitch, rows_like_contiguous, wants_graph
+from miles_amd.kernels._rows import address, gradients_once, pitch, rows_like_contiguous, wants_graph
 from miles_amd.kernels.quant.act_checkpoint import MXFP8_GROUP_SIZE, ActCheckpoint, check_width
 
 
@@ -55,7 +54,7 @@ class _Norm(torch.autograd.Function):
         return y, yq, ys
 
     @staticmethod
-    @once_differentiable
+    @gradients_once("norm")
     def backward(ctx, dy, *_):
         x, xs, mean, rstd, weight = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad[:3]

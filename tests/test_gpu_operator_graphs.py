@@ -1,0 +1,63 @@
+"""The graph nodes of the norms and linear layers, in native code and in Python, under everything that torch does with a graph."""
+
+import pytest
+import torch
+
+from miles_amd.kernels.linear import linear
+from miles_amd.kernels.norm import layer_norm, rms_norm
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+class _Declines:
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+@pytest.fixture(params=["native", "python"])
+def host(request, monkeypatch):
+    """Both host layers: what is ordinary makes its node in native code, anything else in Python."""
+    if request.param == "python":
+        for module in ("miles_amd.kernels.linear", "miles_amd.kernels.norm", "miles_amd.kernels.quant.act_checkpoint", "miles_amd.utils.mxfp8"):
+            monkeypatch.setattr(f"{module}.native", _Declines())
+    return request.param
+
+
+def _leaves(*shapes, dtype=torch.bfloat16, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(s, generator=g).to(dtype).to(DEV).requires_grad_(True) for s in shapes]
+
+
+# name -> (shapes of the leaves, the call)
+CALLS = {
+    "linear": (((24, 64), (96, 64)), lambda x, w: linear(x, w)),
+    "linear_few": (((3, 64), (96, 64), (96,)), lambda x, w, b: linear(x, w, b, activation="gelu")),
+    "linear_residual": (((24, 64), (96, 64), (96,), (24, 96)), lambda x, w, b, r: linear(x, w, b, activation="silu", residual=r)),
+    "linear_kept": (((24, 64), (96, 64), (96,), (24, 96)), lambda x, w, b, r: linear(x, w, b, activation="gelu_tanh", residual=r, checkpoint=True)),
+    "layer_norm": (((24, 64), (64,), (64,)), lambda x, w, b: layer_norm(x, w, b)),
+    "layer_norm_bias": (((24, 64), (64,)), lambda x, b: layer_norm(x, None, b)),
+    "layer_norm_kept": (((24, 64), (64,), (64,)), lambda x, w, b: layer_norm(x, w, b, checkpoint=True)),
+    "rms_norm": (((24, 64), (64,)), lambda x, w: rms_norm(x, w)),
+    "rms_norm_kept": (((24, 64), (64,)), lambda x, w: rms_norm(x, w, checkpoint=True, output_checkpoint=True)[0]),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("loss", [lambda y: y.float().sum(), lambda y: y.float().square().sum()], ids=["constant", "dependent"])
+def test_gradients_of_gradients_are_refused_and_not_left_out(name, loss, host):
+    """A gradient that came out as a constant would leave a penalty on it out of the result without a word."""
+    shapes, call = CALLS[name]
+    leaves = _leaves(*shapes)
+    plain = torch.autograd.grad(loss(call(*leaves)), leaves)
+    y = call(*leaves)
+    grads = torch.autograd.grad(loss(y), leaves, create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(plain, grads))
+    for i, g in enumerate(grads):
+        if i == 3:                                         # a residual's gradient is the incoming one
+            continue
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="gradients of gradients are not supported"):
+            torch.autograd.grad(loss(y) + g.float().square().sum(), leaves, retain_graph=True)
+        with pytest.raises(RuntimeError, match="gradients of gradients are not supported"):
+            torch.autograd.grad(g.float().sum(), leaves, retain_graph=True, allow_unused=True)
