@@ -49,6 +49,7 @@ class _Norm(torch.autograd.Function):
         y, mean, rstd, xq, xs, yq, ys = _forward(x, weight, bias, eps, rms, True, keep, copy)
         ctx.save_for_backward(xq if keep else x, xs, mean, rstd, weight)
         ctx.rms, ctx.shape = rms, x.shape
+        ctx.vector = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
         if copy:
             ctx.mark_non_differentiable(yq, ys)
         return y, yq, ys
@@ -61,7 +62,7 @@ class _Norm(torch.autograd.Function):
         dy2 = rows_like_contiguous(dy)
         m, n = dy2.shape
         x2 = x if xs is not None else rows_like_contiguous(x)
-        vector = weight.dtype if weight is not None else dy.dtype
+        vector = ctx.vector
         lib = _lib.load()
         launch.note_direct_call()
         dx = torch.empty(ctx.shape, dtype=dy.dtype, device=dy.device) if want_x else None
