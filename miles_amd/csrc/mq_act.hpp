@@ -38,22 +38,24 @@ __device__ __forceinline__ float activate(float z) {
     if (ACT == MQ_ACT_GELU_TANH) return z * sigmoid(1.5957691216057308f * z * __builtin_fmaf(0.044715f, z * z, 1.0f));
     return z;
 }
-// the slope of the activation at z
+// The slope of the activation at z.  From 128 on it is 0 or 1 in fp32, and there it is taken: a larger z, or its cube, would be an
+// infinity times 0 (z is finite, or an infinity that an 8-bit copy made of a value next to the largest).  A NaN stays.
 template <int ACT>
 __device__ __forceinline__ float slope(float z) {
     if (ACT == MQ_ACT_RELU) return z > 0.0f ? 1.0f : z == z ? 0.0f : z;
+    const float c = __builtin_fabsf(z) > 128.0f ? __builtin_copysignf(128.0f, z) : z;
     if (ACT == MQ_ACT_SILU) {
-        const float s = sigmoid(z);
-        return s * __builtin_fmaf(z, 1.0f - s, 1.0f);
+        const float s = sigmoid(c);
+        return s * __builtin_fmaf(c, 1.0f - s, 1.0f);
     }
     if (ACT == MQ_ACT_GELU) {
         float bell, share;
-        normal_share(z, bell, share);
-        return __builtin_fmaf(z * 0.3989422804014327f, bell, share);
+        normal_share(c, bell, share);
+        return __builtin_fmaf(c * 0.3989422804014327f, bell, share);
     }
     if (ACT == MQ_ACT_GELU_TANH) {
-        const float s = sigmoid(1.5957691216057308f * z * __builtin_fmaf(0.044715f, z * z, 1.0f));
-        return s * __builtin_fmaf(1.5957691216057308f * z * __builtin_fmaf(0.134145f, z * z, 1.0f), 1.0f - s, 1.0f);
+        const float s = sigmoid(1.5957691216057308f * c * __builtin_fmaf(0.044715f, c * c, 1.0f));
+        return s * __builtin_fmaf(1.5957691216057308f * c * __builtin_fmaf(0.134145f, c * c, 1.0f), 1.0f - s, 1.0f);
     }
     return 1.0f;
 }

@@ -3,6 +3,8 @@
 import pytest
 import torch
 
+from miles_amd import _lib
+from miles_amd.kernels.linear import ACTIVATIONS, linear
 from miles_amd.kernels.norm import layer_norm
 from tests.operator_checks import f64, within
 
@@ -30,3 +32,31 @@ def test_the_gradient_of_an_fp32_bias_without_a_weight_is_fp32(place, dtype):
     db = torch.autograd.grad(layer_norm(x, None, b), b, dy)[0]
     assert db.dtype == torch.float32 and db[5] == 100_000
     within(db, f64(dy).sum(0), 100 * 2.0**-24 * f64(dy).abs().sum(0), "db")
+
+
+# magnitudes from where every activation is saturated in fp32 up to the types' largest finite values
+FAR = {torch.bfloat16: [20.0, 1e3, 65504.0, 1e10, 2e13, 1e19, 2e19, 1e30, torch.finfo(torch.bfloat16).max], torch.float16: [20.0, 1e3, 4096.0, 65504.0]}
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("act", [a for a in ACTIVATIONS if a])
+def test_arguments_far_out(act, dtype):
+    """There an activation is its argument or 0, and its slope 1 or 0 (the nearest place, -20, is 2e-9 of them off in SiLU, whose values
+    are -20 e^-20 and less); one NaN would take a row of dx and one of dW with it."""
+    far = torch.tensor(FAR[dtype], dtype=dtype, device=DEV)
+    z = torch.cat([far, -far])
+    n, k = z.numel(), 32
+    x, dy = torch.zeros(3, k, dtype=dtype, device=DEV).requires_grad_(True), torch.ones(3, n, dtype=dtype, device=DEV)
+    w, b = torch.eye(n, k, dtype=dtype, device=DEV).requires_grad_(True), z.clone().requires_grad_(True)
+    y = linear(x, w, b, activation=act)
+    on = (z > 0).double()
+    assert (f64(y) - f64(z) * on).abs().max() <= 2.0**-24
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert (f64(db) - 3 * on).abs().max() <= 2.0**-22 and (f64(dx) - (f64(dy) * on) @ f64(w)).abs().max() <= 2.0**-23 and (dw == 0).all()
+    # from 16-bit and from 8-bit copies alike
+    pad = torch.cat([z, torch.zeros(-n % 32, dtype=dtype, device=DEV)])
+    x, b = torch.zeros(3, k, dtype=dtype, device=DEV), pad.clone().requires_grad_(True)
+    y = linear(x, torch.zeros(pad.numel(), k, dtype=dtype, device=DEV), b, activation=act, checkpoint=True)
+    db = torch.autograd.grad(y, b, torch.ones_like(y))[0]
+    assert db.isfinite().all() and ((db[:n] == 3) | (db[:n] == 0) | (z.abs() < far.max() * 2.0**-8)).all()
+    assert (db[:n][z == far.max()] == 3).all() and (db[:n][z == -far.max()] == 0).all()      # (bf16: kept as infinities)
