@@ -60,3 +60,25 @@ def test_arguments_far_out(act, dtype):
     db = torch.autograd.grad(y, b, torch.ones_like(y))[0]
     assert db.isfinite().all() and ((db[:n] == 3) | (db[:n] == 0) | (z.abs() < far.max() * 2.0**-8)).all()
     assert (db[:n][z == far.max()] == 3).all() and (db[:n][z == -far.max()] == 0).all()      # (bf16: kept as infinities)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("rows", [3, 40])
+def test_small_values_of_gelu_keep_their_bits(rows, dtype):
+    """Down to where bf16 results are subnormal: Phi is claimed to 5e-5 of itself below -3 and to 2.5e-7 everywhere; 16 steps of fp32 (up to
+    84 of them in the exponent's product) and half a step of the result come on top."""
+    z = torch.linspace(-12.75, 1, 4096, dtype=torch.float64).to(dtype).to(DEV)
+    phi, bell = torch.special.erfc(f64(z) * -(0.5**0.5)) / 2, torch.exp(-f64(z).square() / 2) / (2 * torch.pi) ** 0.5
+    off = torch.where(f64(z) < -3, 5e-5 * phi, torch.full_like(phi, 2.5e-7)) + (16 + f64(z).square()) * 2.0**-24 * phi
+    half, smallest = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    x, w = torch.zeros(rows, 32, dtype=dtype, device=DEV), torch.zeros(4096, 32, dtype=dtype, device=DEV)
+    y = f64(linear(x, w, z, activation="gelu"))
+    want = f64(z) * phi
+    assert ((y - want).abs() <= half * want.abs() + 1.01 * f64(z).abs() * off + smallest / 2).all()
+    assert (y == y[0]).all()
+    slopes = torch.empty_like(z)
+    _lib.check(_lib.load().mq_activation_backward(torch.ones_like(z).data_ptr(), _lib.DTYPE_CODE[dtype], 4096, z.data_ptr(), None, ACTIVATIONS["gelu"],
+                                                  slopes.data_ptr(), None, None, 1, 4096, None))
+    want = phi + f64(z) * bell
+    off += (16 + f64(z).square()) * 2.0**-24 * f64(z).abs() * bell
+    assert ((f64(slopes) - want).abs() <= half * want.abs() + 1.01 * off + smallest / 2).all()
