@@ -333,9 +333,11 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (call.keep && (k % 32 != 0 || (act != MQ_ACT_NONE && n % 32 != 0))) Py_RETURN_NONE;
     if (codes) {
         if (!call.keep || codes->sizes() != x->sizes() || codes->scalar_type() != at::kFloat8_e4m3fn || codes->device() != x->device()) Py_RETURN_NONE;
-        if (scales->scalar_type() != at::kByte || scales->numel() * 32 != codes->numel() || scales->dim() == 0 || scales->size(-1) * 32 != k ||
-            scales->device() != x->device() || (uintptr_t)codes->data_ptr() % 16)
+        if (scales->scalar_type() != at::kByte || scales->dim() != codes->dim() || scales->size(-1) * 32 != k || scales->device() != x->device() ||
+            (uintptr_t)codes->data_ptr() % 16)
             Py_RETURN_NONE;
+        for (int64_t i = 0; i + 1 < codes->dim(); i++)
+            if (scales->size(i) != codes->size(i)) Py_RETURN_NONE;
         call.codes = *codes, call.scales = *scales;
     }
     at::Tensor y;

@@ -6,6 +6,7 @@ import torch
 from miles_amd import _lib
 from miles_amd.kernels.linear import ACTIVATIONS, linear
 from miles_amd.kernels.norm import layer_norm
+from miles_amd.kernels.quant.act_checkpoint import ActCheckpoint, checkpoint_activation
 from tests.operator_checks import f64, within
 
 pytestmark = pytest.mark.gpu
@@ -82,3 +83,14 @@ def test_small_values_of_gelu_keep_their_bits(rows, dtype):
     want = phi + f64(z) * bell
     off += (16 + f64(z).square()) * 2.0**-24 * f64(z).abs() * bell
     assert ((f64(slopes) - want).abs() <= half * want.abs() + 1.01 * off + smallest / 2).all()
+
+
+def test_scales_of_another_shape_are_refused_whatever_their_number():
+    x = torch.randn(6, 4, 64, device=DEV).bfloat16().requires_grad_(True)
+    w = torch.randn(32, 64, device=DEV).bfloat16().requires_grad_(True)
+    kept = checkpoint_activation(x)
+    for scales in (kept.scales.reshape(4, 6, 2), kept.scales.reshape(24, 2), kept.scales.reshape(6, 8), kept.scales.unsqueeze(0)):
+        for arg in (x, x.detach()):
+            with pytest.raises(ValueError, match="scales of shape"):
+                linear(arg, w, checkpoint=ActCheckpoint(kept.codes, scales, x.dtype))
+    assert linear(x, w, checkpoint=kept).shape == (6, 4, 32)
