@@ -40,6 +40,13 @@ at::Tensor one_run(const at::Tensor& t) {
     const at::Tensor c = t.contiguous();
     return (uintptr_t)c.data_ptr() % 16 == 0 ? c : c.clone();
 }
+// A tensor that was saved, as the kernels read it: hooks on saved tensors may give back anything, and a kernel has no way to see it.
+at::Tensor unpacked(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like, const char* what) {
+    if (!t.defined()) return t;
+    TORCH_CHECK(t.sizes() == sizes && t.scalar_type() == dtype && t.device() == like.device() && t.layout() == at::kStrided, what,
+                ": a saved tensor came back as ", t.toString(), t.sizes(), " on ", t.device(), ", not of the type, shape and device that it was saved with");
+    return one_run(t);
+}
 at::Tensor scratch(int64_t bytes, const at::Tensor& like) { return bytes > 0 ? make({bytes}, at::kByte, like) : at::Tensor(); }
 // Gradients are taken once: where a graph of the backward pass itself is asked for, those that the node now running has made are part of
 // one that refuses to be gone through, and as constants would leave what depends on them out of a second derivative.  Its edges are the
@@ -124,12 +131,15 @@ struct Norm : torch::autograd::Function<Norm> {
         const bool again = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &x = saved[0], &xs = saved[1], &mean = saved[2], &rstd = saved[3], &w = saved[4];
         const at::Tensor dy = one_run(grads[0]);
-        const bool rms = ctx->saved_data["rms"].toBool(), want_x = ctx->needs_input_grad(0), want_w = w.defined() && ctx->needs_input_grad(1);
         const int64_t bias = ctx->saved_data["bias"].toInt(), n = dy.size(-1), m = dy.numel() / n;
-        const bool want_b = bias >= 0 && ctx->needs_input_grad(w.defined() ? 2 : 1);
-        const at::ScalarType vector = w.defined() ? w.scalar_type() : bias >= 0 ? (at::ScalarType)bias : dy.scalar_type();
+        const bool kept8 = saved[1].defined(), weight = saved[4].defined();
+        const at::ScalarType vector = weight ? saved[4].scalar_type() : bias >= 0 ? (at::ScalarType)bias : dy.scalar_type();
+        const at::Tensor x = kept8 ? unpacked(saved[0], {m, n}, at::kFloat8_e4m3fn, dy, "norm") : unpacked(saved[0], dy.sizes(), dy.scalar_type(), dy, "norm");
+        const at::Tensor xs = unpacked(saved[1], {m, n / 32}, at::kByte, dy, "norm"), mean = unpacked(saved[2], {m}, at::kFloat, dy, "norm"),
+                         rstd = unpacked(saved[3], {m}, at::kFloat, dy, "norm"), w = unpacked(saved[4], {n}, vector, dy, "norm");
+        const bool rms = ctx->saved_data["rms"].toBool(), want_x = ctx->needs_input_grad(0), want_w = weight && ctx->needs_input_grad(1);
+        const bool want_b = bias >= 0 && ctx->needs_input_grad(weight ? 2 : 1);
         at::Tensor dx, dw, db;
         if (want_x) dx = make(dy.sizes(), dy.scalar_type(), dy);
         if (want_w) dw = make({n}, vector, dy);
@@ -269,7 +279,6 @@ struct Linear : torch::autograd::Function<Linear> {
         const bool again = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &kept = saved[0], &scales = saved[1], &z = saved[2], &zs = saved[3], &w = saved[4];
         const int act = (int)ctx->saved_data["act"].toInt();
         const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
@@ -281,6 +290,12 @@ struct Linear : torch::autograd::Function<Linear> {
             const int64_t n = dy.size(-1), k = sizes.back(), m = dy.numel() / n;
             const int dtype = dtype_code(dy.scalar_type());
             const hipStream_t stream = stream_of(dy);
+            std::vector<int64_t> groups = sizes;
+            groups.back() /= 32;
+            const at::Tensor kept = unpacked(saved[0], sizes, saved[1].defined() ? at::kFloat8_e4m3fn : dy.scalar_type(), dy, "linear"),
+                             scales = unpacked(saved[1], groups, at::kByte, dy, "linear"),
+                             z = unpacked(saved[2], {m, n}, saved[3].defined() ? at::kFloat8_e4m3fn : dy.scalar_type(), dy, "linear"),
+                             zs = unpacked(saved[3], {m, n / 32}, at::kByte, dy, "linear"), w = unpacked(saved[4], {n, k}, dy.scalar_type(), dy, "linear");
             at::Tensor dz = dy;
             if (need_b || act != MQ_ACT_NONE) {
                 if (act != MQ_ACT_NONE) dz = make({m, n}, dy.scalar_type(), dy);

@@ -39,6 +39,22 @@ def gradients_once(what: str):
     return wrap
 
 
+def unpacked(t: torch.Tensor | None, shape, dtype: torch.dtype, device: torch.device, what: str) -> torch.Tensor | None:
+    """A tensor that was saved, as the kernels may read it: hooks on saved tensors may give back anything, and a kernel has no way to see it."""
+    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != device):
+        raise RuntimeError(f"{what}: a saved tensor came back as {t.dtype} {tuple(t.shape)} on {t.device}, not of the type, shape and device that "
+                           f"it was saved with ({dtype} {tuple(shape)} on {device})")
+    return t
+
+
+def one_run(t: torch.Tensor | None) -> torch.Tensor | None:
+    """t as one run of memory that begins at a multiple of 16 bytes."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def rows(t: torch.Tensor) -> torch.Tensor:
     """t [..., n] as a matrix whose rows may lie apart (a view where there is one; rows that overlap are copied)."""
     n = t.shape[-1]

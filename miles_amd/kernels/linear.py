@@ -15,7 +15,7 @@ import torch
 
 from miles_amd import _lib, launch
 from miles_amd._host import native
-from miles_amd.kernels._rows import address, gradients_once, pitch, rows, wants_graph
+from miles_amd.kernels._rows import address, gradients_once, one_run, pitch, rows, unpacked, wants_graph
 from miles_amd.kernels.quant.act_checkpoint import MXFP8_GROUP_SIZE, ActCheckpoint, check_width, keep8
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}      # MQ_ACT_*
@@ -76,6 +76,14 @@ class _Linear(torch.autograd.Function):
         launch.note_direct_call()
         dz = dy2 = rows(dy)
         m = dy2.shape[0]
+        saved = lambda t, shape, dtype: unpacked(t, shape, dtype, device, "linear")  # noqa: E731
+        if x_scales is not None:
+            kept, x_scales = one_run(saved(kept, (m, k), torch.float8_e4m3fn)), one_run(saved(x_scales, (m, k // MXFP8_GROUP_SIZE), torch.uint8))
+        else:
+            kept = saved(kept, ctx.x_shape, ctx.dtype)
+        z = one_run(saved(z, (m, n), ctx.dtype if z_scales is None else torch.float8_e4m3fn))
+        z_scales = one_run(saved(z_scales, (m, n // MXFP8_GROUP_SIZE), torch.uint8))
+        weight = saved(weight, (n, k), ctx.dtype)
         with _lib.on_device(device):
             stream = _lib.stream_ptr(device)
             if need_b or (ctx.act and (need_x or need_w)):

@@ -15,7 +15,7 @@ import torch
 
 from miles_amd import _lib, launch
 from miles_amd._host import native
-from miles_amd.kernels._rows import address, gradients_once, pitch, rows_like_contiguous, wants_graph
+from miles_amd.kernels._rows import address, gradients_once, one_run, pitch, rows_like_contiguous, unpacked, wants_graph
 from miles_amd.kernels.quant.act_checkpoint import MXFP8_GROUP_SIZE, ActCheckpoint, check_width
 
 
@@ -61,8 +61,15 @@ class _Norm(torch.autograd.Function):
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
         dy2 = rows_like_contiguous(dy)
         m, n = dy2.shape
-        x2 = x if xs is not None else rows_like_contiguous(x)
         vector = ctx.vector
+        saved = lambda t, shape, dtype: unpacked(t, shape, dtype, dy.device, "norm")  # noqa: E731
+        if xs is not None:
+            x2 = one_run(saved(x, (m, n), torch.float8_e4m3fn))
+            xs = one_run(saved(xs, (m, n // MXFP8_GROUP_SIZE), torch.uint8))
+        else:
+            x2 = rows_like_contiguous(saved(x, ctx.shape, dy.dtype))
+        mean, rstd, weight = (one_run(saved(t, shape, dtype)) for t, shape, dtype in
+                              ((mean, (m,), torch.float32), (rstd, (m,), torch.float32), (weight, (n,), vector)))
         lib = _lib.load()
         launch.note_direct_call()
         dx = torch.empty(ctx.shape, dtype=dy.dtype, device=dy.device) if want_x else None

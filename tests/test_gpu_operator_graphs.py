@@ -61,3 +61,45 @@ def test_gradients_of_gradients_are_refused_and_not_left_out(name, loss, host):
             torch.autograd.grad(loss(y) + g.float().square().sum(), leaves, retain_graph=True)
         with pytest.raises(RuntimeError, match="gradients of gradients are not supported"):
             torch.autograd.grad(g.float().sum(), leaves, retain_graph=True, allow_unused=True)
+
+
+def _loss(y):
+    return (y.float() * torch.linspace(-1, 1, y.numel(), device=DEV).view(y.shape)).sum()
+
+
+def _elsewhere(t):
+    """The same values in other places: the last two dimensions the other way round in memory, or off 16 bytes."""
+    if t.dim() > 1:
+        return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+    run = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:]
+    return run.copy_(t)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_hooks_on_saved_tensors(name, host):
+    """What a hook gives back is read as it lies, and refused where it is not what was saved: the kernels have its address alone."""
+    shapes, call = CALLS[name]
+    leaves = _leaves(*shapes)
+    want = torch.autograd.grad(_loss(call(*leaves)), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        y = call(*leaves)
+    assert all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(_loss(y), leaves)))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), _elsewhere):
+        y = call(*leaves)
+    assert all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(_loss(y), leaves)))
+    count = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: count.append(1) or t.detach(), lambda t: t):
+        call(*leaves)
+    for which in range(len(count)):
+        for change in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t.reshape(-1)[: t.numel() // 2], lambda t: t.unsqueeze(0)):
+            packed = []
+
+            def pack(t):
+                packed.append(t.detach())
+                return len(packed) - 1
+
+            with torch.autograd.graph.saved_tensors_hooks(pack, lambda i: change(packed[i]) if i == which else packed[i]):
+                y = call(*leaves)
+            assert len(packed) == len(count)
+            with pytest.raises(RuntimeError, match="a saved tensor came back as|weight has the input's type"):
+                torch.autograd.grad(_loss(y), leaves)

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from miles_amd.kernels._rows import gradients_once
+from miles_amd.kernels._rows import gradients_once, one_run, unpacked
 
 
 class _Times(torch.autograd.Function):
@@ -38,3 +38,15 @@ def test_gradients_of_gradients_are_refused_and_not_left_out(loss):
         assert torch.allclose(torch.autograd.grad(gr.sum(), r)[0], torch.full_like(r, 2))
     gx = torch.autograd.grad(loss(_Times.apply(x, w.detach(), r)), x, create_graph=True)[0]
     assert gx.requires_grad
+
+
+def test_a_saved_tensor_that_came_back_as_another_is_refused():
+    t = torch.zeros(4, 6, dtype=torch.bfloat16)
+    device = torch.device("cpu")
+    assert unpacked(None, (4, 6), t.dtype, device, "linear") is None and unpacked(t, (4, 6), t.dtype, device, "linear") is t
+    for other in (t.float(), t[:3], t[0], t.view(2, 12), t.to("meta")):
+        with pytest.raises(RuntimeError, match="linear: a saved tensor came back as"):
+            unpacked(other, (4, 6), t.dtype, device, "linear")
+    for other in (t.t().contiguous().t(), torch.zeros(25, dtype=t.dtype)[1:].view(4, 6)):
+        run = one_run(other)
+        assert run.is_contiguous() and run.data_ptr() % 16 == 0 and torch.equal(run, t)
