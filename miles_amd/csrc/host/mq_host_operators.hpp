@@ -34,7 +34,22 @@ using Input = std::optional<at::Tensor>;
 Input input(const at::Tensor* t) { return t ? Input(*t) : Input(); }
 at::Tensor maybe(const Input& t) { return t.has_value() ? *t : at::Tensor(); }
 void* pointer(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-void checked(int rc) { TORCH_CHECK(rc == MQ_OK, mq_last_error()); }
+// what the library refuses, on its way through torch's functions to the caller, who is given a MilesQuantError
+struct Refusal : std::runtime_error {
+    using std::runtime_error::runtime_error;
+};
+void checked(int rc) {
+    if (rc != MQ_OK) throw Refusal(mq_last_error());
+}
+template <class F>
+PyObject* or_refused(F&& call) {
+    try {
+        return call();
+    } catch (const Refusal& why) {
+        PyErr_SetString(g_error ? g_error : PyExc_RuntimeError, why.what());
+        return nullptr;
+    }
+}
 // t as one run of memory that begins at a multiple of 16 bytes
 at::Tensor one_run(const at::Tensor& t) {
     const at::Tensor c = t.contiguous();
@@ -157,33 +172,35 @@ struct Norm : torch::autograd::Function<Norm> {
 // norm(x, weight | None, bias | None, eps, rms, keep in 8 bits, copy of the result) -> y, (y, codes, scales) or None
 PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 7) return PyErr_Format(PyExc_TypeError, "norm: 7 arguments");
-    const at::Tensor *x = ordinary(a[0]), *w, *b;
-    NormCall call;
-    if (listing() || !ordinary_moment() || !simple(x) || x->dim() == 0 || dtype_code(x->scalar_type()) < 0 || (uintptr_t)x->data_ptr() % 16) Py_RETURN_NONE;
-    if (!optional_simple(a[1], w) || !optional_simple(a[2], b) || !truth(a[4], call.rms) || !truth(a[5], call.keep) || !truth(a[6], call.copy)) Py_RETURN_NONE;
-    if (!PyFloat_Check(a[3])) Py_RETURN_NONE;
-    call.eps = PyFloat_AS_DOUBLE(a[3]);
-    const int64_t columns = x->size(-1);
-    if ((call.keep || call.copy) && columns % 32 != 0) Py_RETURN_NONE;
-    for (const at::Tensor* v : {w, b})
-        if (v && (v->dim() != 1 || v->size(0) != columns || v->device() != x->device() ||
-                  (v->scalar_type() != x->scalar_type() && v->scalar_type() != at::kFloat)))
-            Py_RETURN_NONE;
-    if (w && b && w->scalar_type() != b->scalar_type()) Py_RETURN_NONE;
-    at::Tensor y;
-    {
-        pybind11::gil_scoped_release no_gil;
-        if (wants_graph({x, w, b})) {
-            y = Norm::apply(*x, input(w), input(b), &call);
-        } else {
-            at::NoGradGuard no_grad;
-            NormKept none;
-            y = norm_forward(*x, maybe(w), maybe(b), call, false, none);
+    return or_refused([&]() -> PyObject* {
+        if (n != 7) return PyErr_Format(PyExc_TypeError, "norm: 7 arguments");
+        const at::Tensor *x = ordinary(a[0]), *w, *b;
+        NormCall call;
+        if (listing() || !ordinary_moment() || !simple(x) || x->dim() == 0 || dtype_code(x->scalar_type()) < 0 || (uintptr_t)x->data_ptr() % 16) Py_RETURN_NONE;
+        if (!optional_simple(a[1], w) || !optional_simple(a[2], b) || !truth(a[4], call.rms) || !truth(a[5], call.keep) || !truth(a[6], call.copy)) Py_RETURN_NONE;
+        if (!PyFloat_Check(a[3])) Py_RETURN_NONE;
+        call.eps = PyFloat_AS_DOUBLE(a[3]);
+        const int64_t columns = x->size(-1);
+        if ((call.keep || call.copy) && columns % 32 != 0) Py_RETURN_NONE;
+        for (const at::Tensor* v : {w, b})
+            if (v && (v->dim() != 1 || v->size(0) != columns || v->device() != x->device() ||
+                      (v->scalar_type() != x->scalar_type() && v->scalar_type() != at::kFloat)))
+                Py_RETURN_NONE;
+        if (w && b && w->scalar_type() != b->scalar_type()) Py_RETURN_NONE;
+        at::Tensor y;
+        {
+            pybind11::gil_scoped_release no_gil;
+            if (wants_graph({x, w, b})) {
+                y = Norm::apply(*x, input(w), input(b), &call);
+            } else {
+                at::NoGradGuard no_grad;
+                NormKept none;
+                y = norm_forward(*x, maybe(w), maybe(b), call, false, none);
+            }
         }
-    }
-    if (!call.copy) return THPVariable_Wrap(std::move(y));
-    return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(y)), THPVariable_Wrap(std::move(call.yq)), THPVariable_Wrap(std::move(call.ys)));
+        if (!call.copy) return THPVariable_Wrap(std::move(y));
+        return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(y)), THPVariable_Wrap(std::move(call.yq)), THPVariable_Wrap(std::move(call.ys)));
+    });
     END_HANDLE_TH_ERRORS
 }
 
@@ -199,37 +216,41 @@ void keep_into(const at::Tensor& x, at::Tensor& codes, at::Tensor& scales) {
 // keep8(x) -> (codes, scales) or None
 PyObject* keep8(PyObject*, PyObject* o) {
     HANDLE_TH_ERRORS
-    const at::Tensor* x = ordinary(o);
-    if (listing() || !ordinary_moment() || !simple(x) || x->dim() == 0 || dtype_code(x->scalar_type()) < 0 || x->size(-1) % 32 != 0) Py_RETURN_NONE;
-    at::Tensor codes, scales;
-    {
-        pybind11::gil_scoped_release no_gil;
-        at::NoGradGuard no_grad;
-        keep_into(*x, codes, scales);
-    }
-    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(codes)), THPVariable_Wrap(std::move(scales)));
+    return or_refused([&]() -> PyObject* {
+        const at::Tensor* x = ordinary(o);
+        if (listing() || !ordinary_moment() || !simple(x) || x->dim() == 0 || dtype_code(x->scalar_type()) < 0 || x->size(-1) % 32 != 0) Py_RETURN_NONE;
+        at::Tensor codes, scales;
+        {
+            pybind11::gil_scoped_release no_gil;
+            at::NoGradGuard no_grad;
+            keep_into(*x, codes, scales);
+        }
+        return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(codes)), THPVariable_Wrap(std::move(scales)));
+    });
     END_HANDLE_TH_ERRORS
 }
 // mxfp8_dequant(codes, scales, dtype) -> values or None
 PyObject* mxfp8_dequant(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 3) return PyErr_Format(PyExc_TypeError, "mxfp8_dequant: 3 arguments");
-    const at::Tensor *q = ordinary(a[0]), *s = ordinary(a[1]);
-    if (listing() || !ordinary_moment() || !simple(q) || !simple(s) || q->scalar_type() != at::kFloat8_e4m3fn || s->scalar_type() != at::kByte) Py_RETURN_NONE;
-    if (!THPDtype_Check(a[2]) || dtype_code(((THPDtype*)a[2])->scalar_type) < 0) Py_RETURN_NONE;
-    const at::ScalarType out = ((THPDtype*)a[2])->scalar_type;
-    if (q->dim() == 0 || s->dim() != q->dim() || q->device() != s->device() || q->size(-1) != s->size(-1) * 32) Py_RETURN_NONE;
-    for (int64_t i = 0; i + 1 < q->dim(); i++)
-        if (q->size(i) != s->size(i)) Py_RETURN_NONE;
-    at::Tensor y;
-    {
-        pybind11::gil_scoped_release no_gil;
-        at::NoGradGuard no_grad;
-        y = make(q->sizes(), out, *q);
-        checked(mq_mxfp8_dequant(q->data_ptr(), (const uint8_t*)s->data_ptr(), y.data_ptr(), dtype_code(out), q->numel() / q->size(-1), q->size(-1),
-                                 stream_of(*q)));
-    }
-    return THPVariable_Wrap(std::move(y));
+    return or_refused([&]() -> PyObject* {
+        if (n != 3) return PyErr_Format(PyExc_TypeError, "mxfp8_dequant: 3 arguments");
+        const at::Tensor *q = ordinary(a[0]), *s = ordinary(a[1]);
+        if (listing() || !ordinary_moment() || !simple(q) || !simple(s) || q->scalar_type() != at::kFloat8_e4m3fn || s->scalar_type() != at::kByte) Py_RETURN_NONE;
+        if (!THPDtype_Check(a[2]) || dtype_code(((THPDtype*)a[2])->scalar_type) < 0) Py_RETURN_NONE;
+        const at::ScalarType out = ((THPDtype*)a[2])->scalar_type;
+        if (q->dim() == 0 || s->dim() != q->dim() || q->device() != s->device() || q->size(-1) != s->size(-1) * 32) Py_RETURN_NONE;
+        for (int64_t i = 0; i + 1 < q->dim(); i++)
+            if (q->size(i) != s->size(i)) Py_RETURN_NONE;
+        at::Tensor y;
+        {
+            pybind11::gil_scoped_release no_gil;
+            at::NoGradGuard no_grad;
+            y = make(q->sizes(), out, *q);
+            checked(mq_mxfp8_dequant(q->data_ptr(), (const uint8_t*)s->data_ptr(), y.data_ptr(), dtype_code(out), q->numel() / q->size(-1), q->size(-1),
+                                     stream_of(*q)));
+        }
+        return THPVariable_Wrap(std::move(y));
+    });
     END_HANDLE_TH_ERRORS
 }
 
@@ -326,47 +347,49 @@ struct Linear : torch::autograd::Function<Linear> {
 // linear(x, weight, bias | None, activation code, residual | None, keep in 8 bits, codes | None, scales | None) -> y or None
 PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
     HANDLE_TH_ERRORS
-    if (count != 8) return PyErr_Format(PyExc_TypeError, "linear: 8 arguments");
-    const at::Tensor *x = ordinary(a[0]), *w = ordinary(a[1]), *b, *r, *codes, *scales;
-    if (listing() || !ordinary_moment() || !simple(x) || !simple(w) || !optional_simple(a[2], b) || !optional_simple(a[4], r)) Py_RETURN_NONE;
-    if (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kHalf) Py_RETURN_NONE;
-    int64_t act;
-    LinearCall call;
-    if (!integer(a[3], act) || act < 0 || act > MQ_ACT_GELU_TANH || !truth(a[5], call.keep)) Py_RETURN_NONE;
-    if (!optional_simple(a[6], codes) || !optional_simple(a[7], scales) || !codes != !scales) Py_RETURN_NONE;
-    call.act = (int)act;
-    if (x->dim() == 0 || w->dim() != 2 || w->size(1) != x->size(-1)) Py_RETURN_NONE;
-    const int64_t n = w->size(0), k = w->size(1);
-    if (b && (b->dim() != 1 || b->size(0) != n)) Py_RETURN_NONE;
-    if (r) {
-        if (r->dim() != x->dim() || r->size(-1) != n) Py_RETURN_NONE;
-        for (int64_t i = 0; i + 1 < x->dim(); i++)
-            if (r->size(i) != x->size(i)) Py_RETURN_NONE;
-    }
-    for (const at::Tensor* t : {w, b, r})
-        if (t && (t->scalar_type() != x->scalar_type() || t->device() != x->device())) Py_RETURN_NONE;
-    if (call.keep && (k % 32 != 0 || (act != MQ_ACT_NONE && n % 32 != 0))) Py_RETURN_NONE;
-    if (codes) {
-        if (!call.keep || codes->sizes() != x->sizes() || codes->scalar_type() != at::kFloat8_e4m3fn || codes->device() != x->device()) Py_RETURN_NONE;
-        if (scales->scalar_type() != at::kByte || scales->dim() != codes->dim() || scales->size(-1) * 32 != k || scales->device() != x->device() ||
-            (uintptr_t)codes->data_ptr() % 16)
-            Py_RETURN_NONE;
-        for (int64_t i = 0; i + 1 < codes->dim(); i++)
-            if (scales->size(i) != codes->size(i)) Py_RETURN_NONE;
-        call.codes = *codes, call.scales = *scales;
-    }
-    at::Tensor y;
-    {
-        pybind11::gil_scoped_release no_gil;
-        if (wants_graph({x, w, b, r})) {
-            y = Linear::apply(*x, *w, input(b), input(r), &call, x->requires_grad(), w->requires_grad(), b && b->requires_grad());
-        } else {
-            at::NoGradGuard no_grad;
-            at::Tensor z, zs;
-            y = linear_forward(*x, *w, maybe(b), maybe(r), call, false, z, zs);
+    return or_refused([&]() -> PyObject* {
+        if (count != 8) return PyErr_Format(PyExc_TypeError, "linear: 8 arguments");
+        const at::Tensor *x = ordinary(a[0]), *w = ordinary(a[1]), *b, *r, *codes, *scales;
+        if (listing() || !ordinary_moment() || !simple(x) || !simple(w) || !optional_simple(a[2], b) || !optional_simple(a[4], r)) Py_RETURN_NONE;
+        if (x->scalar_type() != at::kBFloat16 && x->scalar_type() != at::kHalf) Py_RETURN_NONE;
+        int64_t act;
+        LinearCall call;
+        if (!integer(a[3], act) || act < 0 || act > MQ_ACT_GELU_TANH || !truth(a[5], call.keep)) Py_RETURN_NONE;
+        if (!optional_simple(a[6], codes) || !optional_simple(a[7], scales) || !codes != !scales) Py_RETURN_NONE;
+        call.act = (int)act;
+        if (x->dim() == 0 || w->dim() != 2 || w->size(1) != x->size(-1)) Py_RETURN_NONE;
+        const int64_t n = w->size(0), k = w->size(1);
+        if (b && (b->dim() != 1 || b->size(0) != n)) Py_RETURN_NONE;
+        if (r) {
+            if (r->dim() != x->dim() || r->size(-1) != n) Py_RETURN_NONE;
+            for (int64_t i = 0; i + 1 < x->dim(); i++)
+                if (r->size(i) != x->size(i)) Py_RETURN_NONE;
         }
-    }
-    return THPVariable_Wrap(std::move(y));
+        for (const at::Tensor* t : {w, b, r})
+            if (t && (t->scalar_type() != x->scalar_type() || t->device() != x->device())) Py_RETURN_NONE;
+        if (call.keep && (k % 32 != 0 || (act != MQ_ACT_NONE && n % 32 != 0))) Py_RETURN_NONE;
+        if (codes) {
+            if (!call.keep || codes->sizes() != x->sizes() || codes->scalar_type() != at::kFloat8_e4m3fn || codes->device() != x->device()) Py_RETURN_NONE;
+            if (scales->scalar_type() != at::kByte || scales->dim() != codes->dim() || scales->size(-1) * 32 != k || scales->device() != x->device() ||
+                (uintptr_t)codes->data_ptr() % 16)
+                Py_RETURN_NONE;
+            for (int64_t i = 0; i + 1 < codes->dim(); i++)
+                if (scales->size(i) != codes->size(i)) Py_RETURN_NONE;
+            call.codes = *codes, call.scales = *scales;
+        }
+        at::Tensor y;
+        {
+            pybind11::gil_scoped_release no_gil;
+            if (wants_graph({x, w, b, r})) {
+                y = Linear::apply(*x, *w, input(b), input(r), &call, x->requires_grad(), w->requires_grad(), b && b->requires_grad());
+            } else {
+                at::NoGradGuard no_grad;
+                at::Tensor z, zs;
+                y = linear_forward(*x, *w, maybe(b), maybe(r), call, false, z, zs);
+            }
+        }
+        return THPVariable_Wrap(std::move(y));
+    });
     END_HANDLE_TH_ERRORS
 }
 

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from miles_amd import _lib
 from miles_amd.kernels.linear import linear
 from miles_amd.kernels.norm import layer_norm, rms_norm
 
@@ -103,3 +104,11 @@ def test_hooks_on_saved_tensors(name, host):
             assert len(packed) == len(count)
             with pytest.raises(RuntimeError, match="a saved tensor came back as|weight has the input's type"):
                 torch.autograd.grad(_loss(y), leaves)
+
+
+def test_what_the_library_refuses_is_its_own_error_in_both_host_layers(host):
+    x, w = (torch.zeros(1, 1 << 22, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    for wanted in (False, True):
+        with pytest.raises(_lib.MilesQuantError, match="linear: tensor too large"):
+            linear(x.requires_grad_(wanted), w)
+    assert linear(x[:, :64], w[:, :64]).shape == (1, 1)
