@@ -73,10 +73,15 @@ __device__ __forceinline__ f32x16 mfma(u32x4 p, u32x4 q, f32x16 c) {
 }
 
 // 16 bytes from memory straight into shared memory: lane i's go to `lds` + 16 i (lds uniform), from rsrc's base + offset, zeros where
-// the offset is not below 2^31 - 1.  The instruction has no register result; the caller waits for it.
+// the offset is not below 2^31 - 1.  The instruction has no register result; the caller waits for it.  It writes m0 and says so: that is
+// one of the compiler's reserved registers, which sets it before each instruction of its own that reads it and merges settings that
+// nothing between them is declared to change.  (The warning is about reserved registers in general.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void direct16(uint32_t lds, u32x4 rsrc, uint32_t offset) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc) : "m0", "memory");
 }
+#pragma clang diagnostic pop
 constexpr uint32_t kNowhere = 0x80000000u;
 
 __device__ __forceinline__ u32x4 buffer_of(const char* base) {
