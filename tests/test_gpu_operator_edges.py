@@ -94,3 +94,23 @@ def test_scales_of_another_shape_are_refused_whatever_their_number():
             with pytest.raises(ValueError, match="scales of shape"):
                 linear(arg, w, checkpoint=ActCheckpoint(kept.codes, scales, x.dtype))
     assert linear(x, w, checkpoint=kept).shape == (6, 4, 32)
+
+
+@pytest.mark.parametrize("dtype", [*HALVES, torch.float32])
+@pytest.mark.parametrize("n", [1, 40, 96, 1000, 2560, 2563, 7168, 33000])
+def test_a_row_of_one_value_has_no_spread(n, dtype):
+    """Sums of n times 1000 or -3.5 are exact below 2^24 quanta, their quotients by n too: xhat is 0 and with it everything that it is a factor of.
+    What is left of dx, rstd (g - mean g), is off by 2^-18 of the magnitudes as all of the norms' sums are."""
+    g = torch.Generator().manual_seed(n)
+    x = torch.empty(9, n, dtype=dtype, device=DEV)
+    x[::2], x[1::2] = 1000.0, -3.5
+    w, b = ((torch.randn(n, generator=g)).to(dtype).to(DEV).requires_grad_(True) for _ in range(2))
+    dy = torch.randn((9, n), generator=g).to(dtype).to(DEV)
+    for place in (torch.Tensor.contiguous, _off):
+        leaf = place(x).requires_grad_(True)
+        y = layer_norm(leaf, w, b, 1e-5)
+        dx, dw, db = torch.autograd.grad(y, (leaf, w, b), dy)
+        assert torch.equal(y, b.detach().expand(9, n)) and (dw == 0).all()
+        grads = f64(dy) * f64(w)
+        rstd = 1e5**0.5
+        within(dx, rstd * (grads - grads.mean(1, keepdim=True)), 4 * rstd * 2.0**-18 * (grads.abs() + grads.abs().mean(1, keepdim=True)), "dx")
