@@ -1,11 +1,15 @@
 """The graph nodes of the norms and linear layers, in native code and in Python, under everything that torch does with a graph."""
 
+import threading
+
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint as recomputed
 
 from miles_amd import _lib
 from miles_amd.kernels.linear import linear
 from miles_amd.kernels.norm import layer_norm, rms_norm
+from miles_amd.kernels.quant.act_checkpoint import checkpoint_activation
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -112,3 +116,103 @@ def test_what_the_library_refuses_is_its_own_error_in_both_host_layers(host):
         with pytest.raises(_lib.MilesQuantError, match="linear: tensor too large"):
             linear(x.requires_grad_(wanted), w)
     assert linear(x[:, :64], w[:, :64]).shape == (1, 1)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_an_input_written_between_forward_and_backward_is_noticed(name, host):
+    shapes, call = CALLS[name]
+    for which in range(len(shapes)):
+        leaves = _leaves(*shapes)
+        want = torch.autograd.grad(_loss(call(*leaves)), leaves)
+        y = call(*leaves)
+        with torch.no_grad():
+            leaves[which].mul_(2)
+        # x in 8 bits, or its normalized values, are the layer's own; a bias and a residual are not needed
+        if (which == 0 and name.endswith("_kept")) or (which == 1 and name == "layer_norm_bias") or which >= 2:
+            assert all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(_loss(y), leaves)))
+        else:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(_loss(y), leaves)
+
+
+def test_a_copy_written_between_forward_and_backward_is_noticed(host):
+    x, w = _leaves((24, 64), (96, 64))
+    for part in ("codes", "scales"):
+        kept = checkpoint_activation(x)
+        y = linear(x, w, checkpoint=kept)
+        getattr(kept, part).view(torch.uint8).zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(_loss(y), w)
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_in_the_backward_pass(name, reentrant, host):
+    shapes, call = CALLS[name]
+    leaves = _leaves(*shapes)
+    want = torch.autograd.grad(_loss(call(*leaves)), leaves)
+    _loss(recomputed(call, *leaves, use_reentrant=reentrant)).backward()
+    assert all(torch.equal(p, t.grad) for p, t in zip(want, leaves))
+
+
+def test_calls_and_backward_passes_of_several_threads(host):
+    per_thread = [{name: _leaves(*shapes, seed=i) for name, (shapes, _call) in CALLS.items()} for i in range(4)]
+
+    def everything(mine):
+        out = []
+        for name, (_shapes, call) in CALLS.items():
+            y = call(*mine[name])
+            out += [y.detach(), *torch.autograd.grad(_loss(y), mine[name])]
+        return out
+
+    want = [everything(mine) for mine in per_thread]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got = everything(per_thread[i])
+                torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(p, q) for p, q in zip(got, want[i])):
+                wrong.append(i)
+        except Exception as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
+
+
+class _Tagged(torch.Tensor):
+    """A subclass: never taken by the native layer."""
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_transforms_are_refused_and_subclasses_are_not(name):
+    shapes, call = CALLS[name]
+    leaves = [t.detach() for t in _leaves(*shapes)]
+    x, rest = leaves[0], leaves[1:]
+    for transformed in (lambda: torch.func.grad(lambda a: call(a, *rest).float().sum())(x),
+                        lambda: torch.func.grad(lambda a: call(x, a, *rest[1:]).float().sum())(rest[0]),
+                        lambda: torch.func.vmap(lambda a: call(a, *rest))(torch.stack([x, x])),
+                        lambda: torch.func.vmap(lambda a: call(x, a, *rest[1:]))(torch.stack([rest[0], rest[0]])),
+                        lambda: torch.func.jvp(lambda a: call(a, *rest), (x,), (x,))):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            transformed()
+    tagged = call(x.as_subclass(_Tagged).requires_grad_(True), *rest)
+    assert torch.equal(tagged.detach().as_subclass(torch.Tensor), call(*leaves))
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_compiled_functions_call_them_as_they_are(name):
+    shapes, call = CALLS[name]
+    leaves = _leaves(*shapes)
+    torch._dynamo.reset()
+    compiled = torch.compile(lambda *a: call(*a) * 2, backend="eager")
+    y = compiled(*leaves)
+    want = call(*leaves) * 2
+    assert torch.equal(y, want)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(_loss(y), leaves), torch.autograd.grad(_loss(want), leaves)))
