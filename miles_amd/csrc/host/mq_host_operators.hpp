@@ -60,7 +60,7 @@ at::Tensor unpacked(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType d
     if (!t.defined()) return t;
     TORCH_CHECK(t.sizes() == sizes && t.scalar_type() == dtype && t.device() == like.device() && t.layout() == at::kStrided, what,
                 ": a saved tensor came back as ", t.toString(), t.sizes(), " on ", t.device(), ", not of the type, shape and device that it was saved with");
-    return one_run(t);
+    return t.contiguous();
 }
 at::Tensor scratch(int64_t bytes, const at::Tensor& like) { return bytes > 0 ? make({bytes}, at::kByte, like) : at::Tensor(); }
 // Gradients are taken once: where a graph of the backward pass itself is asked for, those that the node now running has made are part of
@@ -150,7 +150,7 @@ struct Norm : torch::autograd::Function<Norm> {
         const int64_t bias = ctx->saved_data["bias"].toInt(), n = dy.size(-1), m = dy.numel() / n;
         const bool kept8 = saved[1].defined(), weight = saved[4].defined();
         const at::ScalarType vector = weight ? saved[4].scalar_type() : bias >= 0 ? (at::ScalarType)bias : dy.scalar_type();
-        const at::Tensor x = kept8 ? unpacked(saved[0], {m, n}, at::kFloat8_e4m3fn, dy, "norm") : unpacked(saved[0], dy.sizes(), dy.scalar_type(), dy, "norm");
+        const at::Tensor x = one_run(kept8 ? unpacked(saved[0], {m, n}, at::kFloat8_e4m3fn, dy, "norm") : unpacked(saved[0], dy.sizes(), dy.scalar_type(), dy, "norm"));
         const at::Tensor xs = unpacked(saved[1], {m, n / 32}, at::kByte, dy, "norm"), mean = unpacked(saved[2], {m}, at::kFloat, dy, "norm"),
                          rstd = unpacked(saved[3], {m}, at::kFloat, dy, "norm"), w = unpacked(saved[4], {n}, vector, dy, "norm");
         const bool rms = ctx->saved_data["rms"].toBool(), want_x = ctx->needs_input_grad(0), want_w = weight && ctx->needs_input_grad(1);
@@ -313,10 +313,12 @@ struct Linear : torch::autograd::Function<Linear> {
             const hipStream_t stream = stream_of(dy);
             std::vector<int64_t> groups = sizes;
             groups.back() /= 32;
-            const at::Tensor kept = unpacked(saved[0], sizes, saved[1].defined() ? at::kFloat8_e4m3fn : dy.scalar_type(), dy, "linear"),
-                             scales = unpacked(saved[1], groups, at::kByte, dy, "linear"),
-                             z = unpacked(saved[2], {m, n}, saved[3].defined() ? at::kFloat8_e4m3fn : dy.scalar_type(), dy, "linear"),
-                             zs = unpacked(saved[3], {m, n / 32}, at::kByte, dy, "linear"), w = unpacked(saved[4], {n, k}, dy.scalar_type(), dy, "linear");
+            auto values = [&](const at::Tensor& t, bool codes, at::IntArrayRef shape) {        // 16-bit ones begin anywhere
+                return codes ? one_run(unpacked(t, shape, at::kFloat8_e4m3fn, dy, "linear")) : unpacked(t, shape, dy.scalar_type(), dy, "linear");
+            };
+            const at::Tensor kept = values(saved[0], saved[1].defined(), sizes), scales = unpacked(saved[1], groups, at::kByte, dy, "linear"),
+                             z = values(saved[2], saved[3].defined(), {m, n}), zs = unpacked(saved[3], {m, n / 32}, at::kByte, dy, "linear"),
+                             w = values(saved[4], false, {n, k});
             at::Tensor dz = dy;
             if (need_b || act != MQ_ACT_NONE) {
                 if (act != MQ_ACT_NONE) dz = make({m, n}, dy.scalar_type(), dy);
