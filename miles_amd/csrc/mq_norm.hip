@@ -654,14 +654,23 @@ extern "C" int mq_norm_forward(const void* x, int dtype, int64_t ldx, const void
     if (((uintptr_t)xhat8 | (uintptr_t)y8) % 8) return mq_fail(MQ_ERR_ARG, "norm: 8-bit copies start at a multiple of 8 bytes");
     const int64_t ldy = rows > 1 ? n : ldx;
     if (!same_offsets(x, ldx, y, ldy, rows, dtype) || ((xhat8 || y8) && ((uintptr_t)x % 16 || !same_offsets(x, ldx, y, 0, rows, dtype)))) return norm_offsets();
-    const NormArgs a{x, weight, bias, y, (uint8_t*)xhat8, xhat8_scale, (uint8_t*)y8, y8_scale, mean, rstd, rows, ldx, (int)n, eps, rms};
     const hipStream_t st = (hipStream_t)stream;
+    const int64_t pieces = norm_pieces(x, rows > 1 ? ldx : 0, n, dtype);
     norm_types(dtype, wdtype, [&](auto d, auto wf) {
         constexpr int D = decltype(d)::value, WF = decltype(wf)::value;
-        norm_shape<0>(norm_pieces(x, rows > 1 ? ldx : 0, n, dtype), [&](auto wave, auto units, unsigned lanes) {
+        norm_shape<0>(pieces, [&](auto wave, auto units, unsigned lanes) {
             constexpr int W = decltype(wave)::value, U = decltype(units)::value;
-            if constexpr (U == 0) hipLaunchKernelGGL((norm_fwd_long_kernel<D, WF>), dim3((unsigned)rows), dim3(lanes), 0, st, a);
-            else hipLaunchKernelGGL((norm_fwd_kernel<D, WF, W, U>), dim3((unsigned)(W ? (rows + 3) / 4 : rows)), dim3(lanes), 0, st, a);
+            // A launch has fewer than 2^32 lanes, 64 to a row or up to 1024.  (The rows of a launch are a multiple of eight, so that those of the
+            // next begin at the offsets in 16 bytes that the first launch's have.)
+            constexpr int64_t kMost = W ? 1 << 25 : 1 << 21;
+            for (int64_t at = 0; at < rows; at += kMost) {
+                const int64_t count = rows - at < kMost ? rows - at : kMost;
+                auto from = [&](auto* p, int64_t row) { return p ? p + at * row : p; };
+                const NormArgs a{(const char*)x + at * ldx * kElem<D>, weight, bias, (char*)y + at * n * kElem<D>, from((uint8_t*)xhat8, n), from(xhat8_scale, n / 32),
+                                 from((uint8_t*)y8, n), from(y8_scale, n / 32), from(mean, 1), from(rstd, 1), count, ldx, (int)n, eps, rms};
+                if constexpr (U == 0) hipLaunchKernelGGL((norm_fwd_long_kernel<D, WF>), dim3((unsigned)count), dim3(lanes), 0, st, a);
+                else hipLaunchKernelGGL((norm_fwd_kernel<D, WF, W, U>), dim3((unsigned)(W ? (count + 3) / 4 : count)), dim3(lanes), 0, st, a);
+            }
         });
     });
     return mq_check_launch("norm forward");

@@ -5,7 +5,7 @@ import torch
 
 from miles_amd import _lib
 from miles_amd.kernels.linear import ACTIVATIONS, linear
-from miles_amd.kernels.norm import layer_norm
+from miles_amd.kernels.norm import layer_norm, rms_norm
 from miles_amd.kernels.quant.act_checkpoint import ActCheckpoint, checkpoint_activation
 from tests.operator_checks import f64, within
 
@@ -114,3 +114,36 @@ def test_a_row_of_one_value_has_no_spread(n, dtype):
         grads = f64(dy) * f64(w)
         rstd = 1e5**0.5
         within(dx, rstd * (grads - grads.mean(1, keepdim=True)), 4 * rstd * 2.0**-18 * (grads.abs() + grads.abs().mean(1, keepdim=True)), "dx")
+
+
+@pytest.mark.parametrize("n,rows", [(4, (1 << 26) + 9), (5, (1 << 26) + 9), (1032, (1 << 21) + 77)])
+def test_rows_beyond_one_launch(n, rows):
+    """More rows than a launch has lanes for; each has the bits that it has in a short tensor."""
+    x = torch.empty((rows, n), dtype=torch.bfloat16, device=DEV)
+    x.view(torch.int16).random_(0x3C00, 0x4000)
+    w, b = (torch.randn(n, device=DEV).bfloat16().requires_grad_(True) for _ in range(2))
+    x.requires_grad_(True)
+    for call in (lambda t: layer_norm(t, w, b), lambda t: rms_norm(t, w)):
+        y = call(x)
+        dx = torch.autograd.grad(y, x, y.detach())[0]
+        for at in (0, 1 << 20, (1 << 21) - 16, 1 << 21, (1 << 25) - 16, 1 << 26, rows - 32):
+            at = min(at, rows - 32) // 8 * 8
+            part = x[at:at + 32].detach().requires_grad_(True)
+            want = call(part)
+            assert torch.equal(y[at:at + 32], want), at
+            assert torch.equal(dx[at:at + 32], torch.autograd.grad(want, part, want.detach())[0]), at
+        del y, dx
+
+
+def test_8_bit_copies_of_rows_beyond_one_launch():
+    rows, n = (1 << 25) + 41, 32
+    x = torch.empty((rows, n), dtype=torch.bfloat16, device=DEV)
+    x.view(torch.int16).random_(0x3C00, 0x4000)
+    x.requires_grad_(True)
+    y, copy = rms_norm(x, checkpoint=True, output_checkpoint=True)
+    dx = torch.autograd.grad(y, x, y.detach())[0]
+    for at in (0, (1 << 25) - 16, rows // 8 * 8 - 32):
+        part = x[at:at + 32].detach().requires_grad_(True)
+        want, kept = rms_norm(part, checkpoint=True, output_checkpoint=True)
+        assert torch.equal(copy.codes[at:at + 32].view(torch.uint8), kept.codes.view(torch.uint8)) and torch.equal(copy.scales[at:at + 32], kept.scales)
+        assert torch.equal(dx[at:at + 32], torch.autograd.grad(want, part, want.detach())[0])
