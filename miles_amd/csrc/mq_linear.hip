@@ -461,7 +461,7 @@ extern "C" int mq_activation_backward(const void* dy, int dtype, int64_t lddy, c
                                       void* dbias, float* ws, int64_t M, int64_t N, void* stream) {
     if (const int rc = check_dtype(dtype)) return rc;
     if (M < 0 || N < 0) return mq_fail(MQ_ERR_ARG, "linear: bad argument");
-    if (M > 0x7FFFFF00 || N > 0x7FFFFF00) return mq_fail(MQ_ERR_ARG, "linear: tensor too large");
+    if (M > 0x7FFFFF00 || N > 0x1FFFFF00) return mq_fail(MQ_ERR_ARG, "linear: tensor too large");      // (eight lanes to a column of the sums, 2^32 to a launch)
     if (act < MQ_ACT_NONE || act > MQ_ACT_GELU_TANH) return mq_fail(MQ_ERR_ARG, "linear: unknown activation");
     if (M > 1 && lddy < N) return mq_fail(MQ_ERR_ARG, "linear: rows overlap");
     if (N == 0 || (M == 0 && !dbias)) return MQ_OK;

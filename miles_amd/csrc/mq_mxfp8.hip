@@ -263,7 +263,7 @@ extern "C" int mq_mxfp8_dequant(const void* q, const uint8_t* scale, void* y, in
     if ((uintptr_t)y % 16) return mq_fail(MQ_ERR_ARG, "the output starts at a multiple of 16 bytes");
     if (rows == 0 || K == 0) return MQ_OK;
     const int64_t units = rows * (K / (dtype == MQ_F32 ? 4 : 8)), blocks = (units + 256 * kMxBackUnits - 1) / (256 * kMxBackUnits);
-    if (blocks > 0x7FFFFFF0) return mq_fail(MQ_ERR_ARG, "tensor too large");
+    if (blocks >= 1 << 24) return mq_fail(MQ_ERR_ARG, "tensor too large");          // (256 lanes each: a launch has fewer than 2^32)
     const dim3 grid((unsigned)blocks), blk(256);
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == MQ_F32) hipLaunchKernelGGL(mxfp8_dequant_kernel<MQ_F32>, grid, blk, 0, st, (const uint8_t*)q, scale, (char*)y, units);
