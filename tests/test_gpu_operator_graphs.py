@@ -216,3 +216,51 @@ def test_compiled_functions_call_them_as_they_are(name):
     want = call(*leaves) * 2
     assert torch.equal(y, want)
     assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(_loss(y), leaves), torch.autograd.grad(_loss(want), leaves)))
+
+
+class _Drops(torch.autograd.Function):
+    """Hands no gradient back."""
+
+    @staticmethod
+    def forward(ctx, y):
+        return y.clone()
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_no_gradient_from_downstream_counts_as_zeros(name, host):
+    shapes, call = CALLS[name]
+    leaves = _leaves(*shapes)
+    grads = torch.autograd.grad(_loss(_Drops.apply(call(*leaves))), leaves, allow_unused=True)
+    assert all(g is None or (g == 0).all() for g in grads)
+
+
+# sizes whose products are cut along k, whose rows end off 16 bytes or inside a tile, and that have more rows than sets of lanes
+WIDE = {
+    "linear_cut": (((48, 4096), (520, 4096), (520,), (48, 520)), lambda x, w, b, r: linear(x, w, b, activation="gelu", residual=r)),
+    "linear_cut_kept": (((333, 2048), (96, 2048), (96,), (333, 96)), lambda x, w, b, r: linear(x, w, b, activation="silu", residual=r, checkpoint=True)),
+    "linear_large": (((1100, 2112), (2080, 2112), (2080,), (1100, 2080)), lambda x, w, b, r: linear(x, w, b, activation="gelu", residual=r, checkpoint=True)),
+    "linear_odd": (((301, 777), (131, 777), (131,), (301, 131)), lambda x, w, b, r: linear(x, w, b, activation="gelu", residual=r)),
+    "norm_odd": (((2100, 1031), (1031,), (1031,)), lambda x, w, b: layer_norm(x, w, b)),
+    "norm_kept": (((700, 2080), (2080,), (2080,)), lambda x, w, b: layer_norm(x, w, b, checkpoint=True)),
+    "norm_long": (((5, 33001), (33001,), (33001,)), lambda x, w, b: layer_norm(x, w, b)),
+}
+
+
+@pytest.mark.parametrize("name", {**CALLS, **WIDE})
+def test_scratch_memory_is_written_before_it_is_read(name, host):
+    """Fresh memory filled with NaNs, as torch does on demand: nothing of it comes out."""
+    shapes, call = {**CALLS, **WIDE}[name]
+    leaves = _leaves(*shapes)
+    y = call(*leaves)
+    want = [y, *torch.autograd.grad(_loss(y), leaves)]
+    torch.use_deterministic_algorithms(True)
+    try:
+        y = call(*leaves)
+        got = [y, *torch.autograd.grad(_loss(y), leaves)]
+    finally:
+        torch.use_deterministic_algorithms(False)
+    assert not any(t.isnan().any() for t in want) and all(torch.equal(p, q) for p, q in zip(got, want))
