@@ -106,7 +106,7 @@ int mq_mxfp8_quant(const void* w, int dtype, void* q, uint8_t* scale, int64_t ro
  *   y [rows,K] contiguous and 16-byte aligned. */
 int mq_mxfp8_dequant(const void* q, const uint8_t* scale, void* y, int dtype, int64_t rows, int64_t K, void* stream);
 
-/* Layer norm and RMS norm (no counterpart in the reference, which takes them from its trainer's libraries).
+/* Layer norm and RMS norm (beside the reference's quantizers, not for one of them).
  *   mean = sum(x)/n (rms != 0: 0), rstd = 1/sqrt(sum((x-mean)^2)/n + eps), xhat = (x-mean) rstd, y = xhat weight + bias
  * x [rows,n] dtype, rows ldx elements apart; row i of x and of y have the same address modulo 16 bytes, for every i (contiguous
  * tensors that begin at multiples of 16 do, whatever n), and with 8-bit copies it is 0; weight, bias [n] of type wdtype (dtype or MQ_F32), either may
@@ -127,14 +127,14 @@ int mq_norm_backward(const void* dy, int dtype, int64_t lddy, const void* x, int
                      int64_t rows, int64_t n, int rms, void* stream);
 int mq_norm_backward_parts(int64_t rows, int64_t n);
 
-/* Linear layers with bias, activation and residual in the product's epilogue (no counterpart in the reference).  All tensors of one
+/* Linear layers with bias, activation and residual in the product's epilogue (likewise).  All tensors of one
  * dtype, MQ_BF16 or MQ_F16; sums in fp32.
  *   z = x weight^T + bias, y = act(z) + residual;  x [M,K], weight [N,K], residual [M,N] with rows ldx, ldw, ldr elements apart,
  *   bias [N] and residual may be NULL; y [M,N] contiguous.
  *   Kept for the backward pass where the pointer is not NULL: z [M,N] contiguous, or z8 / z8_scale: z as MXFP8 ([M,N], [M,N/32];
  *   N a multiple of 32; 4-byte aligned).
  * Backward: mq_activation_backward makes dz = dy act'(z) (z, or z8 with z8_scale not NULL) [M,N] contiguous and dbias = sum over rows
- *   of dz; with MQ_ACT_NONE z is not read and dz may be NULL.  Its ws: mq_activation_backward_parts(M, N) * N floats where dbias
+ *   of dz before its rounding; with MQ_ACT_NONE z is not read and dz may be NULL.  Its ws: mq_activation_backward_parts(M, N) * N floats where dbias
  *   is wanted.  mq_linear_input_grad: dx [M,K] = dz weight.  mq_linear_weight_grad: dweight [N,K] = dz^T x, x as above or
  *   its MXFP8 copy (x_scale not NULL, K a multiple of 32, codes contiguous and 16-byte aligned), which is not restored in memory.
  * ws of the products: mq_linear_workspace's bytes (0: ws may be NULL), 16-byte aligned, for partial sums and for copies of operands

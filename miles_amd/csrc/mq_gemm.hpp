@@ -17,7 +17,7 @@
 // Large products are bound by the matrix cores: 8192^3 in bf16 783 us (1405 TFLOP/s at the clock that the card holds then; matrix
 // instructions take 76 % of the cycles), 8192 x 9728 x 2560 forward 346, input gradient 330, weight gradient 336, from 8 bits 375, and
 // forward with GELU and 8 bits of its argument 428, whose epilogue has one wavefront a SIMD to run on.  With zeros, at full clock, 8192^3
-// takes 580 us, and 546 where every step reads the same operands again, from the nearest cache: the way from memory costs 8 % (13 % at
+// takes 580 us, and 546 in a copy where every step reads the same operands again, from the nearest cache: the way from memory costs 8 % (13 % at
 // 16384 x 2048 x 7168), since a buffer of the next step but one is free only when this step's last fragments have been read.  Small
 // products are bound by that way throughout: 2048^3 25 us.
 #pragma once

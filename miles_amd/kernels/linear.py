@@ -1,6 +1,8 @@
 """Linear layers with bias, activation and residual in the product's epilogue, and their backward passes.
 
-The products run on the matrix cores with fp32 sums; one rounding makes the result.  For the backward pass a layer keeps its
+The products run on the matrix cores with fp32 sums; one rounding makes the result.  In the backward pass of an activation, the
+gradient of its argument is rounded to the tensors' type on its way into the two products behind it (in fp16 it is an infinity
+beyond 65504), not in the bias's gradient.  For the backward pass a layer keeps its
 input and, where it has an activation, what that is applied to: both as they are, or (`checkpoint=True`) both in 8 bits.  The
 weight's gradient is then taken from the codes directly, whose values are exact in bf16.  Gradients are deterministic and can
 be taken once (there is no gradient of a gradient).
