@@ -147,3 +147,27 @@ def test_8_bit_copies_of_rows_beyond_one_launch():
         want, kept = rms_norm(part, checkpoint=True, output_checkpoint=True)
         assert torch.equal(copy.codes[at:at + 32].view(torch.uint8), kept.codes.view(torch.uint8)) and torch.equal(copy.scales[at:at + 32], kept.scales)
         assert torch.equal(dx[at:at + 32], torch.autograd.grad(want, part, want.detach())[0])
+
+
+@pytest.mark.parametrize("dtype,small,large", [(torch.float16, 2.0**-24, 8.0), (torch.bfloat16, 2.0**-133, 2.0**20)])
+@pytest.mark.parametrize("m,n,k", [(3, 64, 64), (40, 64, 64), (300, 512, 256), (1024, 2048, 512)])
+def test_subnormal_operands_count(m, n, k, dtype, small, large):
+    """Whole multiples of the smallest subnormal: exact sums, as with any whole numbers."""
+    g = torch.Generator().manual_seed(k)
+    x = (torch.randint(-3, 4, (m, k), generator=g).double() * small).to(dtype).to(DEV).requires_grad_(True)
+    w = (torch.randint(-2, 3, (n, k), generator=g).double() * large).to(dtype).to(DEV).requires_grad_(True)
+    y = linear(x, w)
+    assert torch.equal(f64(y), f64((f64(x) @ f64(w).t()).to(dtype)))
+    dw = torch.autograd.grad(y, w, torch.ones_like(y))[0]
+    assert torch.equal(f64(dw), f64(f64(x).sum(0).expand(n, k).to(dtype)))
+
+
+def test_a_residual_that_is_the_input():
+    x, w = (torch.randn(s, 96, device=DEV).bfloat16().requires_grad_(True) for s in (40, 96))
+    y = linear(x, w, residual=x)
+    dy = torch.randn_like(y)
+    before = dy.clone()
+    dx = torch.autograd.grad(y, x, dy)[0]
+    apart = x.detach().clone().requires_grad_(True)
+    through = torch.autograd.grad(linear(apart, w, residual=x.detach()), apart, dy)[0]
+    assert torch.equal(dx, through + dy) and torch.equal(dy, before)

@@ -195,11 +195,17 @@ def test_transforms_are_refused_and_subclasses_are_not(name):
     shapes, call = CALLS[name]
     leaves = [t.detach() for t in _leaves(*shapes)]
     x, rest = leaves[0], leaves[1:]
+    wanted = [t.clone().requires_grad_(True) for t in leaves]
+
+    def batched_gradients(y):
+        return torch.autograd.grad(y, wanted, torch.stack([y.detach(), y.detach()]), is_grads_batched=True)
+
     for transformed in (lambda: torch.func.grad(lambda a: call(a, *rest).float().sum())(x),
                         lambda: torch.func.grad(lambda a: call(x, a, *rest[1:]).float().sum())(rest[0]),
                         lambda: torch.func.vmap(lambda a: call(a, *rest))(torch.stack([x, x])),
                         lambda: torch.func.vmap(lambda a: call(x, a, *rest[1:]))(torch.stack([rest[0], rest[0]])),
-                        lambda: torch.func.jvp(lambda a: call(a, *rest), (x,), (x,))):
+                        lambda: torch.func.jvp(lambda a: call(a, *rest), (x,), (x,)),
+                        lambda: batched_gradients(call(*wanted))):
         with pytest.raises((RuntimeError, NotImplementedError)):
             transformed()
     tagged = call(x.as_subclass(_Tagged).requires_grad_(True), *rest)
