@@ -25,6 +25,7 @@ __device__ __forceinline__ void normal_share(float z, float& bell, float& share)
     const float tail = t * p * bell;
     share = z < 0.0f ? tail : 1.0f - tail;
 }
+// (0 from -87.4 down, where the reciprocal would be subnormal: what SiLU and tanh GELU lose there is below 1.1e-36)
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z)); }
 
 template <int ACT>
