@@ -155,6 +155,55 @@ int mq_linear_input_grad(const void* dz, int dtype, int64_t lddz, const void* we
 int mq_linear_weight_grad(const void* dz, int dtype, int64_t lddz, const void* x, int64_t ldx, const uint8_t* x_scale, void* dweight,
                           int64_t M, int64_t N, int64_t K, void* ws, void* stream);
 
+/* Rotary positions (beside the norms and linear layers, likewise without a counterpart in the reference's quantizers).
+ * Of every vector of `dim` elements (dtype, at most 1024 of them) the first 2 pairs are turned: angle = position inv_freq[i],
+ *   c = fl32(scale cos(angle)), s = fl32(scale sin(angle)), angle, cosine and sine in 64 bits;
+ *   (a, b) -> (a c - b s, b c + a s) for the elements i and i + pairs, or (interleaved != 0) 2i and 2i + 1; back != 0: s -> -s, which is the
+ *   backward pass.  The elements behind the pairs stay as they are.
+ * x: one or two tensors of the same tokens (queries and keys; host pointer).  positions: int32 or (positions64 != 0) int64, of token t of
+ *   batch entry b at b position_batch_stride + t.  inv_freq [pairs]: fp32 or (freq64 != 0) fp64.  Any alignment and strides of the
+ *   inputs; accesses are of 16 bytes where every vector and its halves begin at multiples of 16. */
+typedef struct mq_heads {
+    const void* in;                    /* element (b, t, h, i) at b batch_stride + t token_stride + h head_stride + i */
+    void* out;                         /* [batch, tokens, heads, dim] contiguous */
+    int64_t heads, batch_stride, token_stride, head_stride;
+} mq_heads;
+int mq_rotary(const mq_heads* x, int n, int dtype, int64_t batch, int64_t tokens, int64_t dim, const void* positions, int positions64,
+              int64_t position_batch_stride, const void* inv_freq, int freq64, int64_t pairs, int interleaved, double scale, int back, void* stream);
+
+/* A paged cache of keys and values: pages of `page_size` places (a power of two, 16 to 1024), a vector of key_dim and one of value_dim elements for
+ * each place and key head (at most 256, multiples of 8; of 32 in 8 bits).  dtype: MQ_BF16 or MQ_F16, of the tensors that go in and come out.
+ *   16 bits (key_scales, value_scales NULL): keys [pages, kv_heads, key_dim / 8, page_size, 8], values [pages, kv_heads, page_size, value_dim]
+ *   8 bits (MXFP8 along a vector): keys [pages, kv_heads, key_dim / 16, page_size, 16] and values [pages, kv_heads, page_size, value_dim] e4m3fn codes,
+ *     key_scales [pages, kv_heads, key_dim / 32, page_size] and value_scales [.., value_dim / 32, page_size] exponent bytes
+ * A key's pieces of 16 bytes lie beside those of its neighbours, which is how the matrix instructions take them.  All of it contiguous and
+ * 16-byte aligned.  Slot s is place s % page_size of page s / page_size. */
+typedef struct mq_paged_cache {
+    void *keys, *values;
+    uint8_t *key_scales, *value_scales;
+    int64_t pages, page_size, kv_heads, key_dim, value_dim;
+    int dtype;
+} mq_paged_cache;
+/* Writes the vectors of `tokens` tokens into their slots (int32 or int64; outside of the cache: the token is left out), the keys turned as
+ * mq_rotary does it (pairs 0: as they are; else a multiple of 8) and, in 8 bits, quantized from the turned fp32 values.  q (NULL: none): queries of the same tokens, turned into
+ * q->out, also those of tokens that are left out.  k->out and v->out are not used, nor the batch strides.  Inputs: 16-byte aligned, strides multiples of 8.
+ * Slots differ from each other; of a slot that is given twice the contents are any mix of the two, and nothing else is touched. */
+int mq_cache_append(const mq_paged_cache* cache, const mq_heads* k, const mq_heads* v, const mq_heads* q, int64_t tokens, const void* slots, int slots64,
+                    const void* positions, int positions64, const void* inv_freq, int freq64, int64_t pairs, int interleaved, double scale, void* stream);
+
+/* Attention of one token a sequence over a paged cache:
+ *   out[b, h] = sum over t of p_t v_t / (sum over t of p_t + exp(sinks[h])),  p_t = exp(scale q[b, h] . k_t),
+ * t from max(0, length - window) (window 0: from 0) to length - 1; no such t: zeros.  Head h reads key head h / (heads / kv_heads).
+ * Token t of sequence b is place t % page_size of page table[b, t / page_size] (rows table_stride apart, `width` of them); tokens on a page that
+ * the cache has not, or behind the table's width, are left out.  A negative length is 0.  sinks [heads] fp32 or NULL.
+ * q: element (b, h, i) at b q_batch_stride + h q_head_stride + i, 16-byte aligned, strides multiples of 8; out [batch, heads, value_dim] contiguous, 16-byte aligned.
+ * ws: mq_paged_attention_workspace's bytes (0: may be NULL), 16-byte aligned.  The work is split by lengths that the device reads, the launch by
+ * sizes alone: a captured call holds for other lengths and tables.  Sums are added in an order that depends on the lengths and sizes. */
+int mq_paged_attention_workspace(const mq_paged_cache* cache, int64_t batch, int64_t heads, int64_t width, int64_t window, int64_t* bytes);
+int mq_paged_attention(const mq_paged_cache* cache, const void* q, int64_t q_batch_stride, int64_t q_head_stride, const int32_t* table,
+                       int64_t table_stride, int64_t width, const int32_t* lengths, const float* sinks, double scale, int64_t window, void* out,
+                       int64_t batch, int64_t heads, void* ws, void* stream);
+
 /* FP8 128x128 block-scaled source -> MXFP8           tools/convert_hf_to_mxfp8.py:56-102,180-195
  * A source tensor is e4m3fn codes x [M,K] with one scale per 128x128 tile: a grid of at least ceil(M/128) rows and
  * ceil(K/128) columns whose rows are lds elements apart (the reference crops a larger grid, :79,:91).

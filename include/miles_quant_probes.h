@@ -52,6 +52,12 @@ enum { MQP_FLAT_2_1 = 0, MQP_FLAT_1_2 = 1, MQP_LOOP_2_1 = 2, MQP_TILE_2_1 = 3, M
  * workgroups of 64 KiB) with the given numbers of looks: of a record's first workgroup, and of those that watch its word. */
 struct mq_job;
 int mqp_nvfp4_one_pass(const struct mq_job* jobs, int n, int first_polls, int patience, void* stream);
+/* The paged cache's arithmetic of places as its kernels do it, on the host: of 16 tokens (half 0 or 1 of 32, `tile` of those that a sequence of `length` has in view)
+ * on the page that a table gives as `id`.  out: first token seen, end, tiles, whether anything is read, page, place, bytes of keys that may be read from there
+ * on, bytes of values.  mqp_paged_slot: 1 if a slot is one of the cache's, 0 if not. */
+int mqp_paged_places(int32_t id, int64_t pages, int64_t length, int64_t capacity, int64_t window, int tile, int half, int key_row, int value_row,
+                     int page_shift, int64_t* out);
+int mqp_paged_slot(int64_t slot, int64_t slots);
 int mqp_stream_probe(int shape, const void* src, void* dst, int64_t nbytes, int64_t param, void* stream);
 
 #ifdef __cplusplus

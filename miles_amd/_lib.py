@@ -18,7 +18,7 @@ MQ_BF16, MQ_F16, MQ_F32 = 0, 1, 2
 DTYPE_CODE = {torch.bfloat16: MQ_BF16, torch.float16: MQ_F16, torch.float32: MQ_F32}
 
 _c = ctypes
-_vp, _i64, _i32, _f32, _u32 = _c.c_void_p, _c.c_int64, _c.c_int, _c.c_float, _c.c_uint32
+_vp, _i64, _i32, _f32, _u32, _f64 = _c.c_void_p, _c.c_int64, _c.c_int, _c.c_float, _c.c_uint32, _c.c_double
 
 # symbol -> argtypes; every function returns int except the two noted below
 SIGNATURES = {
@@ -40,6 +40,10 @@ SIGNATURES = {
     "mq_activation_backward_parts": [_i64, _i64],
     "mq_linear_input_grad": [_vp, _i32, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp],
     "mq_linear_weight_grad": [_vp, _i32, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp],
+    "mq_rotary": [_vp, _i32, _i32, _i64, _i64, _i64, _vp, _i32, _i64, _vp, _i32, _i64, _i32, _f64, _i32, _vp],
+    "mq_cache_append": [_vp, _vp, _vp, _vp, _i64, _vp, _i32, _vp, _i32, _vp, _i32, _i64, _i32, _f64, _vp],
+    "mq_paged_attention_workspace": [_vp, _i64, _i64, _i64, _i64, _vp],
+    "mq_paged_attention": [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _f64, _i64, _vp, _i64, _i64, _vp, _vp],
     "mq_e8m0_bytes_to_f32": [_vp, _vp, _i64, _vp],
     "mq_fp8_scales_pow2_flag": [_vp, _i64, _i64, _i64, _vp, _vp],
     "mq_e8m0_expand_tile_scales": [_vp, _i32, _i64, _vp, _i64, _i64, _vp],
@@ -87,6 +91,19 @@ class Job(_c.Structure):
     _fields_ = [("kind", _c.c_int32), ("dtype", _c.c_int32), ("inp", _vp), ("out", _vp), ("scale", _vp),
                 ("aux", _vp), ("aux2", _vp), ("rows", _i64), ("cols", _i64), ("ld", _i64), ("p0", _c.c_int32),
                 ("p1", _c.c_int32), ("rows_per_block", _i64), ("block_stride", _i64)]
+
+
+class Heads(_c.Structure):
+    """struct mq_heads of include/miles_quant.h"""
+
+    _fields_ = [("inp", _vp), ("out", _vp), ("heads", _i64), ("batch_stride", _i64), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class Cache(_c.Structure):
+    """struct mq_paged_cache of include/miles_quant.h"""
+
+    _fields_ = [("keys", _vp), ("values", _vp), ("key_scales", _vp), ("value_scales", _vp), ("pages", _i64), ("page_size", _i64),
+                ("kv_heads", _i64), ("key_dim", _i64), ("value_dim", _i64), ("dtype", _c.c_int)]
 
 
 _lib = None

@@ -17,6 +17,8 @@ SIGNATURES = {
     "mqp_selftest_reciprocal": [_vp, _vp],
     "mqp_copy_bytes": [_vp, _vp, _i64, _vp],
     "mqp_nvfp4_one_pass": [_vp, _i32, _i32, _i32, _vp],
+    "mqp_paged_places": [_i32, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp],
+    "mqp_paged_slot": [_i64, _i64],
     "mqp_stream_probe": [_i32, _vp, _vp, _i64, _i64, _vp],
 }
 FLAT_2_1, FLAT_1_2, LOOP_2_1, TILE_2_1, TILE_READ, TILE_WRITE = range(6)      # MQP_* shapes of mqp_stream_probe

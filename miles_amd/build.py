@@ -24,7 +24,8 @@ LIB_PATH = os.path.join(LIB_DIR, "libmiles_quant.so")
 PROBES_LIB_PATH = os.path.join(LIB_DIR, "libmq_probes.so")
 
 SOURCES = ["mq_core.hip", "mq_fp8_block.hip", "mq_mxfp8.hip", "mq_rescale.hip", "mq_mxfp4.hip", "mq_fake_quant.hip", "mq_int4.hip", "mq_nvfp4.hip", "mq_fp8_tensor.hip", "mq_sync.hip",
-           "mq_norm.hip", "mq_linear.hip", "mq_gemm_forward.hip", "mq_gemm_input_grad.hip", "mq_gemm_weight_grad.hip"]
+           "mq_norm.hip", "mq_linear.hip", "mq_gemm_forward.hip", "mq_gemm_input_grad.hip", "mq_gemm_weight_grad.hip",
+           "mq_rotary.hip", "mq_cache.hip", "mq_attend.hip", "mq_attend_bf16.hip", "mq_attend_bf16_kept.hip", "mq_attend_f16.hip", "mq_attend_f16_kept.hip"]
 HOST_LIB_PATH = os.path.join(LIB_DIR, "mq_host.so")
 HOST_SOURCE = os.path.join(CSRC, "host", "mq_host.cpp")
 PROBE_SOURCES = ["mq_selftest.hip", "mq_probe.hip"]

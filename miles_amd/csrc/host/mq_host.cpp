@@ -650,6 +650,7 @@ PyObject* int4_fake(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }  // namespace
 
 #include "mq_host_operators.hpp"
+#include "mq_host_serving.hpp"
 
 namespace {
 
@@ -684,6 +685,9 @@ PyMethodDef methods[] = {{"set_error", set_error, METH_O, nullptr},
                          {"keep8", keep8, METH_O, nullptr},
                          {"mxfp8_dequant", (PyCFunction)(void*)mxfp8_dequant, METH_FASTCALL, nullptr},
                          {"linear", (PyCFunction)(void*)linear, METH_FASTCALL, nullptr},
+                         {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL, nullptr},
+                         {"append", (PyCFunction)(void*)append, METH_FASTCALL, nullptr},
+                         {"attend", (PyCFunction)(void*)attend, METH_FASTCALL, nullptr},
                          {"once", (PyCFunction)(void*)once_of, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "mq_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

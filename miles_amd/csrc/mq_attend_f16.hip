@@ -1,0 +1,3 @@
+#include "mq_attend.hpp"
+
+int mq_attend_f16(const mq::AttendArgs& a, int nk, int nv, unsigned grid, hipStream_t st) { return mq::attend_launch<MQ_F16, false>(a, nk, nv, grid, st); }

@@ -6,6 +6,7 @@
 
 #include "mq_common.hpp"
 #include "mq_group.hpp"
+#include "mq_paged.hpp"
 #include "mq_probes_internal.hpp"
 
 static thread_local char g_probe_err[256] = "";
@@ -156,3 +157,14 @@ extern "C" int mqp_stream_probe(int shape, const void* src, void* dst, int64_t n
     }
     return mqp_fail(MQP_ERR_ARG, "unknown probe shape");
 }
+
+extern "C" int mqp_paged_places(int32_t id, int64_t pages, int64_t length, int64_t capacity, int64_t window, int tile, int half, int key_row, int value_row,
+                                int page_shift, int64_t* out) {
+    const mq::Seen seen = mq::seen_of(length, capacity, window);
+    const int tiles = mq::tiles_of(seen), first = seen.lo / mq::kTile * mq::kTile + tile * mq::kTile + half * 16, place = first & ((1 << page_shift) - 1);
+    const mq::Half h = mq::half_of((uint32_t)id, (uint32_t)pages, first, seen, tile < tiles);
+    const int64_t said[8] = {seen.lo, seen.hi, tiles, h.some, h.page, place, mq::bytes_to_end(h, key_row, page_shift, place, 16), mq::bytes_to_last(h, value_row, first, seen)};
+    for (int i = 0; i < 8; i++) out[i] = said[i];
+    return MQP_OK;
+}
+extern "C" int mqp_paged_slot(int64_t slot, int64_t slots) { return mq::inside(slot, slots); }

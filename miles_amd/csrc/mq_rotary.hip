@@ -1,0 +1,149 @@
+// Rotary positions, forward and backward (the backward pass turns by the negative angle).
+//
+// A workgroup has some tokens: its lanes compute the tokens' cosines and sines into shared memory, then go through the heads' vectors in
+// 16-byte accesses, of which those of the halves layout come in pairs.
+#include "mq_rotary.hpp"
+
+namespace mq {
+
+struct RotaryArgs {
+    const char* in[2];
+    char* out[2];
+    int64_t batch_stride[2], token_stride[2], head_stride[2];    // of the inputs, elements
+    int heads[2];
+    int64_t position_batch_stride;
+    RotaryTurn turn;
+    int64_t tokens, total;         // of a batch entry, and of all
+    int64_t first;                 // token of this launch
+    int dim, per;                  // elements of a vector; tokens of a workgroup
+    int units_head;                // of a vector: accesses (pairs of them in the halves layout), or single elements
+    SmallDivisor by_token, by_head;
+};
+constexpr int kRotaryThreads = 256, kRotaryTurns = 2048, kRotaryTokens = 16;
+
+// VEC: every vector begins at a multiple of 16 bytes, and so does its second half; else element by element
+template <int D, bool INTER, bool VEC>
+__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a) {
+    constexpr int V = VEC ? kVec<D> : 1;
+    __shared__ __attribute__((aligned(16))) f32x2_t cs[kRotaryTurns];
+    __shared__ int64_t from[2][kRotaryTokens];
+    const int64_t token0 = a.first + (int64_t)blockIdx.x * a.per;
+    const int here = (int)(a.total - token0 < a.per ? a.total - token0 : a.per), pairs = a.turn.pairs;
+    for (int i = threadIdx.x; i < here * pairs; i += kRotaryThreads) {
+        const int t = i / pairs;
+        const int64_t b = (token0 + t) / a.tokens;
+        cs[i] = turn_of(a.turn, index_at(a.turn.positions, b * a.position_batch_stride + token0 + t - b * a.tokens, a.turn.positions64), i - t * pairs);
+    }
+    if ((int)threadIdx.x < 2 * here) {
+        const int t = threadIdx.x >> 1, w = threadIdx.x & 1;
+        const int64_t b = (token0 + t) / a.tokens;
+        from[w][t] = b * a.batch_stride[w] + (token0 + t - b * a.tokens) * a.token_stride[w];
+    }
+    __syncthreads();
+    const uint32_t units = (uint32_t)a.by_token.d, n = (uint32_t)here * units;
+    const int turned = VEC ? (INTER ? 2 * pairs / V : pairs / V) : pairs;
+    for (uint32_t i = threadIdx.x; i < n; i += kRotaryThreads) {
+        const uint32_t t = VEC ? divide(i, a.by_token) : i / units, in_token = i - t * units;
+        uint32_t head = VEC ? divide(in_token, a.by_head) : in_token / a.by_head.d;
+        const int unit = (int)(in_token - head * a.by_head.d);
+        const int w = head >= (uint32_t)a.heads[0];
+        if (w) head -= a.heads[0];
+        const char* x = a.in[w] + (from[w][t] + (int64_t)head * a.head_stride[w]) * kElem<D>;
+        char* y = a.out[w] + ((token0 + t) * a.heads[w] + head) * (int64_t)a.dim * kElem<D>;
+        const f32x2_t* turn = cs + t * pairs;
+        if (VEC) {
+            if (unit >= turned) {                                         // behind the part that is turned
+                const int at = (2 * pairs + (unit - turned) * V) * kElem<D>;
+                st16(y + at, ld16(x + at));
+            } else if (INTER) {
+                u32x4 v = ld16(x + unit * 16);
+                turn_neighbours<D>(v, turn + unit * (V / 2));
+                st16(y + unit * 16, v);
+            } else {
+                const int half = pairs * kElem<D>;
+                u32x4 u = ld16(x + unit * 16), v = ld16(x + half + unit * 16);
+                turn_halves<D>(u, v, turn + unit * V);
+                st16(y + unit * 16, u);
+                st16(y + half + unit * 16, v);
+            }
+        } else if (unit >= turned) {
+            const int at = pairs + unit;
+            store_dtype(y, at, load_f32(x, at, D), D);
+        } else {
+            const int i0 = INTER ? 2 * unit : unit, i1 = INTER ? i0 + 1 : unit + pairs;
+            const float p = load_f32(x, i0, D), q = load_f32(x, i1, D);
+            store_dtype(y, i0, p * turn[unit].x - q * turn[unit].y, D);
+            store_dtype(y, i1, q * turn[unit].x + p * turn[unit].y, D);
+        }
+    }
+}
+
+template <int D>
+int rotary_launch(RotaryArgs a, bool inter, bool vec, hipStream_t st) {
+    constexpr int64_t kMost = 1 << 23;                    // workgroups of a launch, which has fewer than 2^32 lanes
+    for (; a.first < a.total; a.first += kMost * a.per) {
+        const int64_t left = (a.total - a.first + a.per - 1) / a.per;
+        const dim3 grid((unsigned)(left < kMost ? left : kMost));
+        if (vec && inter) rotary_kernel<D, true, true><<<grid, kRotaryThreads, 0, st>>>(a);
+        else if (vec) rotary_kernel<D, false, true><<<grid, kRotaryThreads, 0, st>>>(a);
+        else if (inter) rotary_kernel<D, true, false><<<grid, kRotaryThreads, 0, st>>>(a);
+        else rotary_kernel<D, false, false><<<grid, kRotaryThreads, 0, st>>>(a);
+        const int rc = mq_check_launch("mq_rotary");
+        if (rc != MQ_OK) return rc;
+    }
+    return MQ_OK;
+}
+
+}  // namespace mq
+
+extern "C" int mq_rotary(const struct mq_heads* x, int n, int dtype, int64_t batch, int64_t tokens, int64_t dim, const void* positions, int positions64,
+                         int64_t position_batch_stride, const void* inv_freq, int freq64, int64_t pairs, int interleaved, double scale, int back, void* stream) {
+    using namespace mq;
+    if (!x || n < 1 || n > 2 || dtype < MQ_BF16 || dtype > MQ_F32 || batch < 0 || tokens < 0 || dim < 0 || pairs < 0 || 2 * pairs > dim)
+        return mq_fail(MQ_ERR_ARG, "mq_rotary: bad argument");
+    if (dim > 1024) return mq_fail(MQ_ERR_ARG, "mq_rotary: vectors of at most 1024 elements");
+    if (batch && tokens > INT32_MAX / batch) return mq_fail(MQ_ERR_ARG, "mq_rotary: tensor too large");
+    int64_t heads = 0;
+    for (int w = 0; w < n; w++) {
+        if (x[w].heads < 0) return mq_fail(MQ_ERR_ARG, "mq_rotary: bad argument");
+        if (x[w].heads > 65535) return mq_fail(MQ_ERR_ARG, "mq_rotary: tensor too large");
+        heads += x[w].heads;
+    }
+    if (batch * tokens * dim * heads == 0) return MQ_OK;
+    const int elem = dtype == MQ_F32 ? 4 : 2, v = 16 / elem;
+    RotaryArgs a = {};
+    bool vec = dim % v == 0 && pairs * (interleaved ? 2 : 1) % v == 0;
+    if ((pairs && (!positions || !inv_freq))) return mq_fail(MQ_ERR_ARG, "mq_rotary: null pointer");
+    for (int w = 0; w < n; w++) {
+        if (x[w].heads && (!x[w].in || !x[w].out)) return mq_fail(MQ_ERR_ARG, "mq_rotary: null pointer");
+        a.in[w] = (const char*)x[w].in;
+        a.out[w] = (char*)x[w].out;
+        a.batch_stride[w] = x[w].batch_stride;
+        a.token_stride[w] = x[w].token_stride;
+        a.head_stride[w] = x[w].head_stride;
+        a.heads[w] = (int)x[w].heads;
+        if (x[w].heads)
+            vec = vec && ((uintptr_t)x[w].in | (uintptr_t)x[w].out) % 16 == 0 && (batch == 1 || x[w].batch_stride % v == 0) &&
+                  (tokens == 1 || x[w].token_stride % v == 0) && (x[w].heads == 1 || x[w].head_stride % v == 0);
+    }
+    a.position_batch_stride = position_batch_stride;
+    a.turn = RotaryTurn{positions, inv_freq, scale, (int)pairs, positions64, freq64, back};
+    a.tokens = tokens;
+    a.total = batch * tokens;
+    a.dim = (int)dim;
+    const int64_t units = vec ? (interleaved ? dim / v : (dim - pairs) / v) : dim - pairs;
+    if (heads * units > 65535 * (vec ? 1 : 64)) return mq_fail(MQ_ERR_ARG, "mq_rotary: tensor too large");
+    a.units_head = (int)units;
+    // Tokens of a workgroup: enough for all lanes to have an angle to compute, while there are workgroups for every compute unit.
+    int64_t per = 1;
+    while (per < kRotaryTokens && per * 2 * pairs <= kRotaryTurns && per * pairs < kRotaryThreads && a.total / (per * 2) >= 1024 &&
+           per * 2 * heads * units * heads * units < (1ll << 32))
+        per *= 2;
+    a.per = (int)per;
+    a.by_token = small_divisor((uint32_t)(heads * units));
+    a.by_head = small_divisor((uint32_t)units);
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == MQ_BF16) return rotary_launch<MQ_BF16>(a, interleaved, vec, st);
+    if (dtype == MQ_F16) return rotary_launch<MQ_F16>(a, interleaved, vec, st);
+    return rotary_launch<MQ_F32>(a, interleaved, vec, st);
+}
