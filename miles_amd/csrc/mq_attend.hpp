@@ -21,24 +21,37 @@ struct AttendArgs {
     const int32_t *table, *lengths;
     const float* sinks;
     char* out;
-    float* parts;                  // partial results, null: every workgroup has whole sequences (direct)
+    float* parts;                  // partial results: a first and a last one of every worker
     uint32_t* starts;              // [batch + 1]: units before each sequence, and all of them
     int64_t q_batch, q_head, table_stride, capacity, window;
     uint32_t pages;
     uint32_t key_page, value_page, key_scale_page, value_scale_page;      // bytes of a page, below 2^31
     int batch, heads, kv_heads, group, key_dim, value_dim, page_shift;
-    int blocks;                    // of heads of a key head: groups of 16 x head_waves
-    int head_waves;                // wavefronts of a workgroup that share tokens and have different heads: 1, 2 or 4
-    uint32_t least;                // units that a workgroup takes at least
-    float scale;                   // with log2(e)
+    int blocks;                    // of query heads of a key head, block_heads each
+    int head_waves;                // wavefronts that share tokens and have 16 different heads of a block each: 1 to 4
+    int block_heads;
+    uint32_t least;                // units that a worker takes at least
+    float scale;                   // with log2(e), positive
+    uint32_t flip;                 // signs of two elements of a query, where the scale was negative
 };
-// A unit of work is a tile of 32 tokens of one key head for one block of query heads; units are numbered by sequence, key head, block
-// and tile.
+// A row is a sequence's key head and a block of its query heads; rows are numbered by sequence, key head and block.  A row's units of work are
+// its tiles of 32 tokens, behind kRowUnits that stand for what a row costs beside them.
+constexpr uint32_t kRowUnits = 4;
 constexpr float kLowest = -3.0e38f;                      // the maximum of no scores: finite, so that differences are numbers
-constexpr int kAttendThreads = 256, kAttendWaves = 4, kRowPad = 132;
+constexpr float kSlack = 8.0f;
+constexpr int kAttendWaves = 4, kRowPad = 132;           // of a workgroup whose workers share rows out
 
-// floats of a workgroup's partial result: 16 heads x 128 NV sums for each head wave, then their maxima and totals
-__host__ __device__ inline int64_t part_floats(int head_waves, int nv) { return (int64_t)head_waves * 16 * (128 * nv + 2); }
+// Workers of a workgroup that shares rows out: four, or one of several head waves, which go through their tiles in step
+__host__ __device__ constexpr int attend_workers(int head_waves) { return head_waves > 1 ? 1 : kAttendWaves; }
+// keys, values, queries and sums that fill the registers of one wavefront a SIMD
+__host__ __device__ constexpr bool attend_is_wide(int nk, int nv) { return nv == 2 && nk > 4; }
+// floats of a worker's partial result: 128 NV sums for each head of a block, then their maxima and totals
+__host__ __device__ inline int64_t part_floats(int block_heads, int nv) { return (int64_t)block_heads * (128 * nv + 2); }
+__host__ __device__ inline uint32_t units_of(int tiles) { return tiles ? (uint32_t)tiles + kRowUnits : 0u; }
+__host__ __device__ inline uint32_t units_of_worker(uint32_t total, uint32_t workers, uint32_t least) {
+    const uint32_t share = (total + workers - 1) / workers;
+    return share > least ? share : least;
+}
 
 #define MQ_CONST __attribute__((address_space(4)))
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -62,25 +75,19 @@ __device__ __forceinline__ float sum_of_head(float v) {
     return u2f(y[0]) + u2f(y[1]);
 }
 
-// Sums of units over all sequences before this lane's (inclusive), 256 sequences at a time
-__device__ __forceinline__ uint32_t scan_units(uint32_t v, uint32_t* waves, uint32_t& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {           // inclusive
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
         const uint32_t up = __shfl_up(v, d);
         if (lane >= d) v += up;
     }
-    if (lane == 63) waves[wave] = v;
-    __syncthreads();
-    uint32_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kAttendWaves; w++) {
-        if (w < wave) before += waves[w];
-        total += waves[w];
-    }
-    __syncthreads();
-    return v + before;
+    return v;
 }
 
 template <int D>
@@ -98,101 +105,97 @@ __device__ __forceinline__ float finish_factor(const AttendArgs& a, int head, fl
     return l == 0.0f ? 0.0f : 1.0f / l;
 }
 
-template <int D, bool KEPT, int NK, int NV>
-__global__ __launch_bounds__(kAttendThreads, NV == 2 && NK > 4 ? 1 : 2) void attend_kernel(const AttendArgs a) {
+// Not DIRECT: workgroups of kAttendWaves wavefronts, head_waves of them a worker, whose share of all units it finds by itself and which nothing else
+// waits for.  DIRECT: a workgroup has one row, its wavefronts every so manieth tile of it, and their sums meet in shared memory.
+// SHARED: several head waves, whose accesses to the same lines meet in the compute unit's cache; else every line is read by one wavefront once, and
+// the accesses say so, which is worth a tenth of the bandwidth.
+template <int D, bool KEPT, int NK, int NV, bool DIRECT, bool SHARED>
+__global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 2) void attend_kernel(const AttendArgs a) {
+    constexpr int kPolicy = SHARED ? 0 : 2;               // (2: non-temporal)
     constexpr int kLoads = KEPT ? NK / 2 : NK;            // of a tile's half's keys
-    __shared__ __attribute__((aligned(16))) float sums[kAttendWaves][16 * kRowPad];
-    __shared__ float tops[kAttendWaves][16], totals[kAttendWaves][16];
-    __shared__ uint32_t scratch[2 * kAttendWaves + 1];
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x / kWave), c = lane & 15, g = lane >> 4;
-    const int per_tile = a.kv_heads * a.blocks;           // units of a tile of tokens
+    const int rows = a.kv_heads * a.blocks;               // of a sequence
+    const int head_wave = SHARED ? wave % a.head_waves : 0;
 
     // ---- which units
     int b;
-    uint32_t rest, left;                                  // first unit within its sequence, and how many
-    bool first_of_workgroup = true;
-    if (!a.parts) {
-        const int inner = (int)blockIdx.x % per_tile;
-        b = (int)blockIdx.x / per_tile;
+    uint32_t rest, left, worker = 0;                      // first unit within its sequence, and how many
+    bool first_of_worker = true;
+    if (DIRECT) {
+        const int row = (int)blockIdx.x % rows;
+        b = (int)blockIdx.x / rows;
         const int tiles = tiles_of(seen_uniform(a, b));
-        rest = (uint32_t)inner * tiles;
-        left = tiles;
         if (tiles == 0) {                                 // nothing to see
             const int n = a.group * a.value_dim / 8;
-            if (inner % a.blocks == 0) {
-                char* to = a.out + ((int64_t)b * a.heads + (int64_t)(inner / a.blocks) * a.group) * a.value_dim * 2;
-                for (int i = threadIdx.x; i < n; i += kAttendThreads) *(u32x4*)(to + (int64_t)i * 16) = u32x4{0u, 0u, 0u, 0u};
+            if (row % a.blocks == 0) {
+                char* to = a.out + ((int64_t)b * a.heads + (int64_t)(row / a.blocks) * a.group) * a.value_dim * 2;
+                for (int i = threadIdx.x; i < n; i += (int)blockDim.x) *(u32x4*)(to + (int64_t)i * 16) = u32x4{0u, 0u, 0u, 0u};
             }
             return;
         }
+        rest = (uint32_t)row * units_of(tiles);
+        left = units_of(tiles);
     } else {
-        uint32_t total = 0, inclusive = 0, chunk;
-        for (int b0 = 0; b0 < a.batch; b0 += kAttendThreads) {
-            const int mine = b0 + (int)threadIdx.x;
-            const uint32_t units = mine < a.batch ? (uint32_t)tiles_of(seen_by(a, mine)) * per_tile : 0u;
-            inclusive = total + scan_units(units, scratch, chunk);
-            if (blockIdx.x == 0 && mine < a.batch) a.starts[mine] = inclusive - units;
-            total += chunk;
-        }
-        if (blockIdx.x == 0 && threadIdx.x == 0) a.starts[a.batch] = total;
-        const uint32_t share = (total + gridDim.x - 1) / gridDim.x, per = share > a.least ? share : a.least;
-        const uint64_t u0 = (uint64_t)blockIdx.x * per;
-        // sequences without a token are shared out among all workgroups
-        for (int e = blockIdx.x; e < a.batch; e += gridDim.x) {
-            if (tiles_of(seen_uniform(a, e)) != 0) continue;
+        const uint32_t workers = gridDim.x * (SHARED ? 1 : kAttendWaves);
+        worker = SHARED ? blockIdx.x : blockIdx.x * kAttendWaves + wave;
+        uint32_t total = 0, units = 0;
+        for (int s = lane; s < a.batch; s += 64) total += (units = units_of(tiles_of(seen_by(a, s))) * rows);
+        total = (uint32_t)uniform((int)wave_sum(total));
+        const uint32_t per = units_of_worker(total, workers, a.least);
+        const uint64_t u0 = (uint64_t)worker * per;
+        // sequences without a token are shared out among all workers
+        for (int e = (int)worker; e < a.batch; e += (int)workers) {
+            if (tiles_of(seen_uniform(a, e)) != 0 || head_wave != 0) continue;
             char* to = a.out + (int64_t)e * a.heads * a.value_dim * 2;
-            for (int i = threadIdx.x; i < a.heads * a.value_dim / 8; i += kAttendThreads) *(u32x4*)(to + (int64_t)i * 16) = u32x4{0u, 0u, 0u, 0u};
+            for (int i = lane; i < a.heads * a.value_dim / 8; i += 64) *(u32x4*)(to + (int64_t)i * 16) = u32x4{0u, 0u, 0u, 0u};
         }
-        if (u0 >= total) return;
+        const bool notes = blockIdx.x == 0 && wave == 0;  // the sequences' first units, for the join
+        if (notes && lane == 0) a.starts[a.batch] = total;
+        if (u0 >= total && !notes) return;
         left = (uint32_t)uniform((int)(total - (uint32_t)u0 < per ? total - (uint32_t)u0 : per));
         // the sequence of unit u0: as many as end at or before it come first
-        uint32_t running = 0;
-        for (int b0 = 0;; b0 += kAttendThreads) {
-            if (a.batch > kAttendThreads) {
-                const int mine = b0 + (int)threadIdx.x;
-                const uint32_t units = mine < a.batch ? (uint32_t)tiles_of(seen_by(a, mine)) * per_tile : 0u;
-                inclusive = running + scan_units(units, scratch, chunk);
-                running += chunk;
-                if (running <= (uint32_t)u0) continue;
+        uint32_t before = 0;
+        b = -1;
+        rest = 0;
+        for (int s0 = 0; s0 < a.batch && (b < 0 || notes); s0 += 64) {
+            const int s = s0 + lane;
+            if (a.batch > 64) units = s < a.batch ? units_of(tiles_of(seen_by(a, s))) * rows : 0u;
+            const uint32_t inclusive = before + wave_scan(units);
+            if (notes && s < a.batch) a.starts[s] = inclusive - units;
+            const uint32_t end = (uint32_t)__builtin_amdgcn_readlane((int)inclusive, 63);
+            if (b < 0 && end > (uint32_t)u0) {
+                const int n = __builtin_popcountll(__ballot(inclusive <= (uint32_t)u0));
+                b = s0 + n;
+                rest = (uint32_t)u0 - (uint32_t)__builtin_amdgcn_readlane((int)(inclusive - units), n);
             }
-            const bool before = b0 + (int)threadIdx.x < a.batch && inclusive <= (uint32_t)u0;
-            const uint64_t votes = __ballot(before);
-            if (lane == 0) scratch[kAttendWaves + wave] = (uint32_t)__builtin_popcountll(votes);
-            __syncthreads();
-            int n = 0;
-            for (int w = 0; w < kAttendWaves; w++) n += (int)scratch[kAttendWaves + w];
-            b = b0 + uniform(n);
-            if ((int)threadIdx.x == n) {
-                const int tiles = tiles_of(seen_by(a, b));
-                scratch[2 * kAttendWaves] = (uint32_t)u0 - (inclusive - (uint32_t)tiles * per_tile);
-            }
-            __syncthreads();
-            rest = (uint32_t)uniform((int)scratch[2 * kAttendWaves]);
-            break;
+            before = end;
         }
+        if (u0 >= total) return;
     }
 
-    const int head_wave = wave & (a.head_waves - 1), token_wave = wave / a.head_waves, token_waves = kAttendWaves / a.head_waves;
+    const int token_wave = DIRECT ? wave / a.head_waves : 0, token_waves = DIRECT ? (int)blockDim.x / kWave / a.head_waves : 1;
     const uint32_t k_lane = (uint32_t)(((g << a.page_shift) + c) * 16), k_step = (uint32_t)(4 << a.page_shift) * 16;
     const int key_row = a.key_dim * (KEPT ? 1 : 2), value_row = a.value_dim * (KEPT ? 1 : 2);
     const uint32_t v_lane = (uint32_t)(4 * g * value_row + c * (KEPT ? 8 : 16));
 
-    for (;;) {                                            // a sequence's key head and block of query heads, or the part of it that is this workgroup's
+    for (;;) {                                            // a row, or the part of it that is this worker's
         const Seen seen = seen_uniform(a, b);
-        const int tiles = tiles_of(seen), inner = (int)(rest / (uint32_t)tiles), tile0 = (int)(rest - (uint32_t)inner * tiles);
-        const int tile1 = (uint32_t)(tiles - tile0) < left ? tiles : tile0 + (int)left;
-        const int kv = inner / a.blocks, block = inner - kv * a.blocks, head0 = (block * a.head_waves + head_wave) * 16;      // within the group
+        const int tiles = tiles_of(seen);
+        const uint32_t units = units_of(tiles), row = rest / units, from = rest - row * units, to = units - from < left ? units : from + left;
+        const int tile0 = from > kRowUnits ? (int)(from - kRowUnits) : 0, tile1 = to > kRowUnits ? (int)(to - kRowUnits) : 0;
+        const int kv = (int)row / a.blocks, block = (int)row - kv * a.blocks, head0 = block * a.block_heads + head_wave * 16;      // within the group
         const int heads_here = a.group - head0 < 16 ? a.group - head0 : 16;
         const int t_base = seen.lo / kTile * kTile;
-        const int64_t row = (int64_t)b * a.table_stride;
-
+        left -= to - from;
+        rest += to - from;
+        if (tile0 < tile1) {
         u32x4 q[NK];
         {
             const char* from = a.q + ((int64_t)b * a.q_batch + (int64_t)(kv * a.group + head0 + c) * a.q_head) * 2;
 #pragma unroll
             for (int j = 0; j < NK; j++) {
                 const int at = KEPT ? (j / 2) * 64 + g * 16 + (j & 1) * 8 : j * 32 + g * 8;
-                q[j] = c < heads_here && at < a.key_dim ? *(const u32x4*)(from + at * 2) : u32x4{0u, 0u, 0u, 0u};
+                q[j] = c < heads_here && at < a.key_dim ? *(const u32x4*)(from + at * 2) ^ a.flip : u32x4{0u, 0u, 0u, 0u};
             }
         }
         f32x4 acc[NV * 8];
@@ -236,7 +239,7 @@ __global__ __launch_bounds__(kAttendThreads, NV == 2 && NK > 4 ? 1 : 2) void att
                                                                     bytes_to_end(at[h], key_row, a.page_shift, place, 16), 0x00027000);
 #pragma unroll
                 for (int j = 0; j < kLoads; j++)          // (pieces behind the key's end: zeros)
-                    k[h][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (int)(k_lane + j * k_step), 0, 0));
+                    k[h][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (int)(k_lane + j * k_step), 0, kPolicy));
                 if (KEPT) {
                     const auto scales = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(key_scales) + (uint64_t)at[h].page * a.key_scale_page + place, 0,
                                                                           bytes_to_end(at[h], a.key_dim / 32, a.page_shift, place, 1), 0x00027000);
@@ -249,16 +252,15 @@ __global__ __launch_bounds__(kAttendThreads, NV == 2 && NK > 4 ? 1 : 2) void att
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int first = t_base + t * kTile + h * 16, place = first & ((1 << a.page_shift) - 1);
-                const int before = seen.lo - first - 4 * g;       // tokens of this lane's that lie before a window
                 const auto from = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(values) + (uint64_t)at[h].page * a.value_page + place * value_row, 0,
                                                                     bytes_to_last(at[h], value_row, first, seen), 0x00027000);
 #pragma unroll
                 for (int nv = 0; nv < NV; nv++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const uint32_t at_v = i < before ? kNowhere : v_lane + i * value_row + nv * (KEPT ? 128 : 256);
-                        if (KEPT) v8[nv][h * 4 + i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(from, (int)at_v, 0, 0));
-                        else v[nv][h * 4 + i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (int)at_v, 0, 0));
+                        const uint32_t at_v = v_lane + i * value_row + nv * (KEPT ? 128 : 256);
+                        if (KEPT) v8[nv][h * 4 + i] = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(from, (int)at_v, 0, kPolicy));
+                        else v[nv][h * 4 + i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (int)at_v, 0, kPolicy));
                     }
                 if (KEPT) {
                     const auto scales = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(value_scales) + (uint64_t)at[h].page * a.value_scale_page + place, 0,
@@ -283,22 +285,19 @@ __global__ __launch_bounds__(kAttendThreads, NV == 2 && NK > 4 ? 1 : 2) void att
         __builtin_amdgcn_sched_barrier(0);
         while (t < tile1) {
             const int next = t + token_waves;
+            if (SHARED && !DIRECT) __builtin_amdgcn_s_barrier();
             // ---- scores
-            f32x4 s[2];
+            f32x4 s[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                s[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (KEPT) {
 #pragma unroll
-                    for (int j = 0; j < kLoads; j++) {
+                for (int j = 0; j < kLoads; j++) {
+                    if (KEPT) {
                         const u32x2 p0 = kept_pack4<D>(k[h][j].x, ke[h][j]), p1 = kept_pack4<D>(k[h][j].y, ke[h][j]);
                         const u32x2 p2 = kept_pack4<D>(k[h][j].z, ke[h][j]), p3 = kept_pack4<D>(k[h][j].w, ke[h][j]);
                         s[h] = mfma<D>(u32x4{p0.x, p0.y, p1.x, p1.y}, q[2 * j], s[h]);
                         s[h] = mfma<D>(u32x4{p2.x, p2.y, p3.x, p3.y}, q[2 * j + 1], s[h]);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < kLoads; j++) s[h] = mfma<D>(k[h][j], q[j], s[h]);
+                    } else s[h] = mfma<D>(k[h][j], q[j], s[h]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -307,29 +306,42 @@ __global__ __launch_bounds__(kAttendThreads, NV == 2 && NK > 4 ? 1 : 2) void att
             __builtin_amdgcn_sched_barrier(0);
             // ---- weights
             const int first = t_base + t * kTile;
-            float p[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) p[i] = s[i / 4][i & 3] * a.scale;
-            if (!(first >= seen.lo && first + kTile <= seen.hi && at[0].some && at[1].some)) {
+            const bool full = first >= seen.lo && first + kTile <= seen.hi && at[0].some && at[1].some;
+            if (!full) {
+                // what is not seen: no weight; values before a window as zeros (behind the last token they are), and in 8 bits the scales, which
+                // may be any bytes there, a NaN's among them
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const int token = first + (i / 4) * 16 + 4 * g + (i & 3);
-                    if (token < seen.lo || token >= seen.hi || !at[i / 4].some) p[i] = -__builtin_inff();
+                    const bool hidden = token < seen.lo || token >= seen.hi || !at[i / 4].some;
+                    if (hidden) s[i / 4][i & 3] = -__builtin_inff();
+#pragma unroll
+                    for (int nv = 0; nv < NV; nv++) {
+                        if (KEPT) {
+                            if (token < seen.lo) v8[nv][i] = u32x2{0u, 0u};
+                            if (hidden) ve[i / 4][nv] &= ~(0xFFu << (8 * (i & 3)));
+                        } else if (token < seen.lo) v[nv][i] = u32x4{0u, 0u, 0u, 0u};
+                    }
                 }
             }
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) p[i] = s[i / 4][i & 3];
             float most = p[0];
 #pragma unroll
             for (int i = 1; i < 8; i++) most = __builtin_fmaxf(most, p[i]);
-            const float higher = __builtin_fmaxf(top, max_of_head(most));
-            if (__any(higher > top)) {
-                const float f = __builtin_amdgcn_exp2f(top - higher);
+            // The running maximum need not be the largest: weights up to 2^kSlack of it are numbers as good.  Sums are rescaled when it is passed by
+            // more, which after a row's first tile hardly ever is.
+            const float higher = max_of_head(most) * a.scale;
+            if (__any(higher > top + kSlack)) {
+                const float now = __builtin_fmaxf(top, higher), f = __builtin_amdgcn_exp2f(top - now);
                 total *= f;
 #pragma unroll
                 for (int i = 0; i < NV * 8; i++) acc[i] *= f;
-                top = higher;
+                top = now;
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(p[i] - top);
+            for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], a.scale, -top));
 #pragma unroll
             for (int i = 0; i < 8; i++) total += p[i];
             uint32_t big[4], small[4];
@@ -340,22 +352,13 @@ __global__ __launch_bounds__(kAttendThreads, NV == 2 && NK > 4 ? 1 : 2) void att
             }
             const u32x4 weights = {big[0], big[1], big[2], big[3]}, remainders = {small[0], small[1], small[2], small[3]};
             // ---- values
-            uint32_t scale_mask[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
-            if (KEPT) {                                   // scales of tokens that are not seen: any bytes, a NaN's among them
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int end = seen.hi - (first + h * 16 + 4 * g), begin = seen.lo - (first + h * 16 + 4 * g);
-                    if (end < 4) scale_mask[h] = end <= 0 ? 0u : 0xFFFFFFFFu >> (32 - 8 * end);
-                    if (begin > 0) scale_mask[h] &= begin >= 4 ? 0u : 0xFFFFFFFFu << (8 * begin);
-                }
-            }
 #pragma unroll
             for (int nv = 0; nv < NV; nv++) {
                 u32x4 x[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     if (KEPT) {
-                        const uint32_t e = (ve[i / 4][nv] & scale_mask[i / 4]) >> (8 * (i & 3)) & 0xFFu;
+                        const uint32_t e = ve[i / 4][nv] >> (8 * (i & 3)) & 0xFFu;
                         const u32x2 lo = kept_pack4<D>(v8[nv][i].x, e), hi = kept_pack4<D>(v8[nv][i].y, e);
                         x[i] = u32x4{lo.x, lo.y, hi.x, hi.y};
                     } else x[i] = v[nv][i];
@@ -378,80 +381,103 @@ __global__ __launch_bounds__(kAttendThreads, NV == 2 && NK > 4 ? 1 : 2) void att
             at[1] = at_next[1];
         }
 
-        // ---- the wavefronts' sums together: those that have the same heads, in their order
+        // ---- where the sums go
         total = sum_of_head(total);
-        if (g == 0) {
-            tops[wave][c] = top;
-            totals[wave][c] = total;
-        }
-        __syncthreads();
-        float highest = kLowest;
-        for (int w = 0; w < token_waves; w++) highest = __builtin_fmaxf(highest, tops[w * a.head_waves + head_wave][c]);
-        const float mine = __builtin_amdgcn_exp2f(top - highest);
-        const bool whole = tile0 == 0 && tile1 == tiles;
-        float* part = whole ? nullptr : a.parts + ((int64_t)blockIdx.x * 2 + (first_of_workgroup ? 0 : 1)) * part_floats(a.head_waves, NV);
+        if (!DIRECT) {
+            const bool whole = tile0 == 0 && tile1 == tiles;
+            const int in_block = head_wave * 16 + c, head = kv * a.group + head0 + c;
+            float* part = a.parts + ((int64_t)worker * 2 + (first_of_worker ? 0 : 1)) * part_floats(a.block_heads, NV);
+            if (c < heads_here) {
+                const float times = whole ? finish_factor(a, head, top, total) : 1.0f;
+                if (!whole && g == 0) *(f32x2*)(part + a.block_heads * (128 * NV) + in_block * 2) = f32x2{top, total};
 #pragma unroll
-        for (int nv = 0; nv < NV; nv++) {
-            if (nv) __syncthreads();
+                for (int nv = 0; nv < NV; nv++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float* to = &sums[wave][c * kRowPad + 8 * (4 * g + r)];
-                *(f32x4*)to = f32x4{acc[nv * 8 + 0][r], acc[nv * 8 + 1][r], acc[nv * 8 + 2][r], acc[nv * 8 + 3][r]} * mine;
-                *(f32x4*)(to + 4) = f32x4{acc[nv * 8 + 4][r], acc[nv * 8 + 5][r], acc[nv * 8 + 6][r], acc[nv * 8 + 7][r]} * mine;
+                    for (int r = 0; r < 4; r++) {
+                        const int at_dim = nv * 128 + 8 * (4 * g + r);
+                        if (at_dim >= a.value_dim) continue;
+                        float f[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) f[e] = acc[nv * 8 + e][r] * times;
+                        if (whole) store8<D>(a.out + (((int64_t)b * a.heads + head) * a.value_dim + at_dim) * 2, f);
+                        else {
+                            float* sums = part + in_block * (128 * NV) + at_dim;
+                            *(f32x4*)sums = f32x4{f[0], f[1], f[2], f[3]};
+                            *(f32x4*)(sums + 4) = f32x4{f[4], f[5], f[6], f[7]};
+                        }
+                    }
             }
-            __syncthreads();
-            const int h = (int)threadIdx.x >> 4, at = ((int)threadIdx.x & 15) * 8;
-            for (int hw = 0; hw < a.head_waves; hw++) {
-                const int head = (block * a.head_waves + hw) * 16 + h;               // within the group
-                if (head >= a.group) continue;
-                float m = kLowest, l = 0.0f, f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                for (int w = 0; w < token_waves; w++) m = __builtin_fmaxf(m, tops[w * a.head_waves + hw][h]);
-                for (int w = 0; w < token_waves; w++) {
-                    const int from = w * a.head_waves + hw;
-                    l += totals[from][h] * __builtin_amdgcn_exp2f(tops[from][h] - m);
-                    const f32x4 x = *(const f32x4*)&sums[from][h * kRowPad + at], y = *(const f32x4*)&sums[from][h * kRowPad + at + 4];
+        } else {
+            // the wavefronts' sums together: those that have the same heads, in their order
+            __shared__ __attribute__((aligned(16))) float sums[DIRECT ? kAttendWaves : 1][16 * kRowPad];
+            __shared__ float tops[DIRECT ? kAttendWaves : 1][16], totals[DIRECT ? kAttendWaves : 1][16];
+            if (g == 0) {
+                tops[wave][c] = top;
+                totals[wave][c] = total;
+            }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        f[i] += x[i];
-                        f[4 + i] += y[i];
-                    }
+            for (int nv = 0; nv < NV; nv++) {
+                __syncthreads();
+                float highest = kLowest;
+                for (int w = 0; w < token_waves; w++) highest = __builtin_fmaxf(highest, tops[w * a.head_waves + head_wave][c]);
+                const float mine = __builtin_amdgcn_exp2f(top - highest);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float* sum = &sums[wave][c * kRowPad + 8 * (4 * g + r)];
+                    const f32x4* x = &acc[nv * 8];
+                    *(f32x4*)sum = f32x4{x[0][r], x[1][r], x[2][r], x[3][r]} * mine;
+                    *(f32x4*)(sum + 4) = f32x4{x[4][r], x[5][r], x[6][r], x[7][r]} * mine;
                 }
-                if (part) {
-                    float* to = part + (hw * 16 + h) * (128 * NV) + nv * 128 + at;
-                    *(f32x4*)to = f32x4{f[0], f[1], f[2], f[3]};
-                    *(f32x4*)(to + 4) = f32x4{f[4], f[5], f[6], f[7]};
-                    if (nv == 0 && at == 0) {
-                        float* ml = part + a.head_waves * 16 * (128 * NV) + (hw * 16 + h) * 2;
-                        ml[0] = m;
-                        ml[1] = l;
+                __syncthreads();
+                for (int i = threadIdx.x; i < a.head_waves * 256; i += (int)blockDim.x) {
+                    const int hw = i >> 8, h = i >> 4 & 15, at_dim = (i & 15) * 8, head = block * a.block_heads + hw * 16 + h;               // within the group
+                    if (head >= a.group || nv * 128 + at_dim >= a.value_dim) continue;
+                    float m = kLowest, l = 0.0f, f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int w = 0; w < token_waves; w++) m = __builtin_fmaxf(m, tops[w * a.head_waves + hw][h]);
+                    for (int w = 0; w < token_waves; w++) {
+                        const int of = w * a.head_waves + hw;
+                        l += totals[of][h] * __builtin_amdgcn_exp2f(tops[of][h] - m);
+                        const f32x4 x = *(const f32x4*)&sums[of][h * kRowPad + at_dim], y = *(const f32x4*)&sums[of][h * kRowPad + at_dim + 4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            f[j] += x[j];
+                            f[4 + j] += y[j];
+                        }
                     }
-                } else if (nv * 128 + at < a.value_dim) {
                     const int64_t to_head = (int64_t)kv * a.group + head;
                     const float times = finish_factor(a, (int)to_head, m, l);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) f[i] *= times;
-                    store8<D>(a.out + (((int64_t)b * a.heads + to_head) * a.value_dim + nv * 128 + at) * 2, f);
+                    for (int j = 0; j < 8; j++) f[j] *= times;
+                    store8<D>(a.out + (((int64_t)b * a.heads + to_head) * a.value_dim + nv * 128 + at_dim) * 2, f);
                 }
             }
+            return;
+        }
         }
         // ---- what comes next
-        left -= (uint32_t)(tile1 - tile0);
         if (left == 0) return;
-        first_of_workgroup = false;
-        rest += (uint32_t)(tile1 - tile0);
-        if (rest == (uint32_t)tiles * per_tile) {
+        first_of_worker = false;
+        if (rest == units * rows) {
             rest = 0;
             do b++;
             while (tiles_of(seen_uniform(a, b)) == 0);
         }
-        __syncthreads();                                  // shared memory is free again
     }
 }
 
+template <int D, bool KEPT, int NK, int NV, bool SHARED>
+void attend_launch(const AttendArgs& a, bool direct, unsigned grid, hipStream_t st) {
+    if (direct) attend_kernel<D, KEPT, NK, NV, true, SHARED><<<grid, kAttendWaves / a.head_waves * a.head_waves * kWave, 0, st>>>(a);
+    else attend_kernel<D, KEPT, NK, NV, false, SHARED><<<grid, (SHARED ? a.head_waves : kAttendWaves) * kWave, 0, st>>>(a);
+}
+template <int D, bool KEPT, int NK, int NV>
+void attend_launch(const AttendArgs& a, bool direct, unsigned grid, hipStream_t st) {
+    a.head_waves > 1 ? attend_launch<D, KEPT, NK, NV, true>(a, direct, grid, st) : attend_launch<D, KEPT, NK, NV, false>(a, direct, grid, st);
+}
 template <int D, bool KEPT>
-int attend_launch(const AttendArgs& a, int nk, int nv, unsigned grid, hipStream_t st) {
+int attend_launch(const AttendArgs& a, int nk, int nv, bool direct, unsigned grid, hipStream_t st) {
 #define MQ_ATTEND(NK, NV) \
-    if (nk == NK && nv == NV) attend_kernel<D, KEPT, NK, NV><<<grid, kAttendThreads, 0, st>>>(a)
+    if (nk == NK && nv == NV) attend_launch<D, KEPT, NK, NV>(a, direct, grid, st)
     MQ_ATTEND(2, 1);
     MQ_ATTEND(4, 1);
     MQ_ATTEND(6, 1);
@@ -466,7 +492,7 @@ int attend_launch(const AttendArgs& a, int nk, int nv, unsigned grid, hipStream_
 
 }  // namespace mq
 
-int mq_attend_bf16(const mq::AttendArgs& a, int nk, int nv, unsigned grid, hipStream_t st);
-int mq_attend_bf16_kept(const mq::AttendArgs& a, int nk, int nv, unsigned grid, hipStream_t st);
-int mq_attend_f16(const mq::AttendArgs& a, int nk, int nv, unsigned grid, hipStream_t st);
-int mq_attend_f16_kept(const mq::AttendArgs& a, int nk, int nv, unsigned grid, hipStream_t st);
+int mq_attend_bf16(const mq::AttendArgs& a, int nk, int nv, bool direct, unsigned grid, hipStream_t st);
+int mq_attend_bf16_kept(const mq::AttendArgs& a, int nk, int nv, bool direct, unsigned grid, hipStream_t st);
+int mq_attend_f16(const mq::AttendArgs& a, int nk, int nv, bool direct, unsigned grid, hipStream_t st);
+int mq_attend_f16_kept(const mq::AttendArgs& a, int nk, int nv, bool direct, unsigned grid, hipStream_t st);

@@ -1,3 +1,5 @@
 #include "mq_attend.hpp"
 
-int mq_attend_f16_kept(const mq::AttendArgs& a, int nk, int nv, unsigned grid, hipStream_t st) { return mq::attend_launch<MQ_F16, true>(a, nk, nv, grid, st); }
+int mq_attend_f16_kept(const mq::AttendArgs& a, int nk, int nv, bool direct, unsigned grid, hipStream_t st) {
+    return mq::attend_launch<MQ_F16, true>(a, nk, nv, direct, grid, st);
+}
