@@ -1,7 +1,7 @@
 // Rotary positions, forward and backward (the backward pass turns by the negative angle).
 //
-// A workgroup has some tokens: its lanes compute the tokens' cosines and sines into shared memory, then go through the heads' vectors in
-// 16-byte accesses, of which those of the halves layout come in pairs.
+// A workgroup has some tokens: its lanes compute the tokens' cosines and sines into shared memory and go through the heads' vectors in
+// 16-byte accesses, of which those of the halves layout come in pairs.  What bounds it is reading and writing every element once.
 #include "mq_rotary.hpp"
 
 namespace mq {
@@ -26,54 +26,72 @@ template <int D, bool INTER, bool VEC>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a) {
     constexpr int V = VEC ? kVec<D> : 1;
     __shared__ __attribute__((aligned(16))) f32x2_t cs[kRotaryTurns];
-    __shared__ int64_t from[2][kRotaryTokens];
     const int64_t token0 = a.first + (int64_t)blockIdx.x * a.per;
     const int here = (int)(a.total - token0 < a.per ? a.total - token0 : a.per), pairs = a.turn.pairs;
-    for (int i = threadIdx.x; i < here * pairs; i += kRotaryThreads) {
-        const int t = i / pairs;
-        const int64_t b = (token0 + t) / a.tokens;
-        cs[i] = turn_of(a.turn, index_at(a.turn.positions, b * a.position_batch_stride + token0 + t - b * a.tokens, a.turn.positions64), i - t * pairs);
-    }
-    if ((int)threadIdx.x < 2 * here) {
-        const int t = threadIdx.x >> 1, w = threadIdx.x & 1;
-        const int64_t b = (token0 + t) / a.tokens;
-        from[w][t] = b * a.batch_stride[w] + (token0 + t - b * a.tokens) * a.token_stride[w];
-    }
-    __syncthreads();
-    const uint32_t units = (uint32_t)a.by_token.d, n = (uint32_t)here * units;
-    const int turned = VEC ? (INTER ? 2 * pairs / V : pairs / V) : pairs;
-    for (uint32_t i = threadIdx.x; i < n; i += kRotaryThreads) {
+    const uint32_t units = a.by_token.d, n = (uint32_t)here * units;
+    const int turned = VEC ? (INTER ? 2 * pairs / V : pairs / V) : pairs, half = pairs * kElem<D>;
+    auto batch_of = [&](uint32_t token) { return a.total == a.tokens ? 0u : token / (uint32_t)a.tokens; };       // (all of them: fewer than 2^31)
+    struct Unit {
+        const char* x;
+        char* y;
+        int at, token;                                    // number within the vector, and of the token within the workgroup
+    };
+    auto unit_of = [&](uint32_t i) {
         const uint32_t t = VEC ? divide(i, a.by_token) : i / units, in_token = i - t * units;
         uint32_t head = VEC ? divide(in_token, a.by_head) : in_token / a.by_head.d;
-        const int unit = (int)(in_token - head * a.by_head.d);
-        const int w = head >= (uint32_t)a.heads[0];
+        const int at = (int)(in_token - head * a.by_head.d), w = head >= (uint32_t)a.heads[0];
         if (w) head -= a.heads[0];
-        const char* x = a.in[w] + (from[w][t] + (int64_t)head * a.head_stride[w]) * kElem<D>;
-        char* y = a.out[w] + ((token0 + t) * a.heads[w] + head) * (int64_t)a.dim * kElem<D>;
-        const f32x2_t* turn = cs + t * pairs;
-        if (VEC) {
-            if (unit >= turned) {                                         // behind the part that is turned
-                const int at = (2 * pairs + (unit - turned) * V) * kElem<D>;
-                st16(y + at, ld16(x + at));
-            } else if (INTER) {
-                u32x4 v = ld16(x + unit * 16);
-                turn_neighbours<D>(v, turn + unit * (V / 2));
-                st16(y + unit * 16, v);
-            } else {
-                const int half = pairs * kElem<D>;
-                u32x4 u = ld16(x + unit * 16), v = ld16(x + half + unit * 16);
-                turn_halves<D>(u, v, turn + unit * V);
-                st16(y + unit * 16, u);
-                st16(y + half + unit * 16, v);
+        const uint32_t token = (uint32_t)token0 + t, b = batch_of(token);
+        return Unit{a.in[w] + ((int64_t)b * a.batch_stride[w] + (int64_t)(token - b * (uint32_t)a.tokens) * a.token_stride[w] + (int64_t)head * a.head_stride[w]) * kElem<D>,
+                    a.out[w] + ((int64_t)token * a.heads[w] + head) * a.dim * kElem<D>, at, (int)t};
+    };
+    auto angles = [&]() {
+        for (int i = threadIdx.x; i < here * pairs; i += kRotaryThreads) {
+            const int t = i / pairs;
+            const uint32_t token = (uint32_t)token0 + t, b = batch_of(token);
+            cs[i] = turn_of(a.turn, index_at(a.turn.positions, b * a.position_batch_stride + (token - b * (uint32_t)a.tokens), a.turn.positions64), i - t * pairs);
+        }
+        __syncthreads();
+    };
+    if (VEC) {
+        // The first access is on its way while the angles are computed; one at a time and plain stores measured best (4 x 4096 tokens of 40 heads of 128 in
+        // bf16 in 55 us, 6.1 TB/s; two at a time 57, non-temporal stores 58, the angles first 62; a copy of as many bytes runs at 6.2 to 6.5).
+        const bool any = threadIdx.x < n;
+        for (uint32_t i = threadIdx.x; i < n || i == threadIdx.x; i += kRotaryThreads) {
+            Unit unit = {};
+            u32x4 p, q;
+            int at = 0;
+            if (any) {
+                unit = unit_of(i);
+                at = unit.at >= turned && !INTER ? 2 * half + (unit.at - turned) * 16 : unit.at * 16;
+                p = ld16(unit.x + at);
+                if (!INTER && unit.at < turned) q = ld16(unit.x + half + at);
             }
-        } else if (unit >= turned) {
-            const int at = pairs + unit;
-            store_dtype(y, at, load_f32(x, at, D), D);
-        } else {
-            const int i0 = INTER ? 2 * unit : unit, i1 = INTER ? i0 + 1 : unit + pairs;
-            const float p = load_f32(x, i0, D), q = load_f32(x, i1, D);
-            store_dtype(y, i0, p * turn[unit].x - q * turn[unit].y, D);
-            store_dtype(y, i1, q * turn[unit].x + p * turn[unit].y, D);
+            if (i == threadIdx.x) angles();
+            if (!any) return;
+            if (unit.at < turned) {
+                const f32x2_t* turn = cs + unit.token * pairs;
+                if (INTER) turn_neighbours<D>(p, turn + unit.at * (V / 2));
+                else {
+                    turn_halves<D>(p, q, turn + unit.at * V);
+                    *(u32x4*)(unit.y + half + at) = q;
+                }
+            }
+            *(u32x4*)(unit.y + at) = p;
+        }
+    } else {
+        angles();
+        for (uint32_t i = threadIdx.x; i < n; i += kRotaryThreads) {
+            const Unit unit = unit_of(i);
+            if (unit.at >= turned) {                      // behind the part that is turned
+                store_dtype(unit.y, pairs + unit.at, load_f32(unit.x, pairs + unit.at, D), D);
+                continue;
+            }
+            const f32x2_t w = cs[unit.token * pairs + unit.at];
+            const int i0 = INTER ? 2 * unit.at : unit.at, i1 = INTER ? i0 + 1 : unit.at + pairs;
+            const float p = load_f32(unit.x, i0, D), q = load_f32(unit.x, i1, D);
+            store_dtype(unit.y, i0, p * w.x - q * w.y, D);
+            store_dtype(unit.y, i1, q * w.x + p * w.y, D);
         }
     }
 }
@@ -134,10 +152,11 @@ extern "C" int mq_rotary(const struct mq_heads* x, int n, int dtype, int64_t bat
     const int64_t units = vec ? (interleaved ? dim / v : (dim - pairs) / v) : dim - pairs;
     if (heads * units > 65535 * (vec ? 1 : 64)) return mq_fail(MQ_ERR_ARG, "mq_rotary: tensor too large");
     a.units_head = (int)units;
-    // Tokens of a workgroup: enough for all lanes to have an angle to compute, while there are workgroups for every compute unit.
+    // Tokens of a workgroup: enough for all lanes to have an angle to compute and an access or two to make, while there are workgroups for every
+    // compute unit (8192 tokens of 9 heads of 64 by eight at once 7.0 us, by one 12.9; of 40 heads of 128 by one or two 58, by four 61, by eight 70).
     int64_t per = 1;
     while (per < kRotaryTokens && per * 2 * pairs <= kRotaryTurns && per * pairs < kRotaryThreads && a.total / (per * 2) >= 1024 &&
-           per * 2 * heads * units * heads * units < (1ll << 32))
+           per * 2 * heads * units <= 512)
         per *= 2;
     a.per = (int)per;
     a.by_token = small_divisor((uint32_t)(heads * units));
