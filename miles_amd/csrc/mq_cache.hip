@@ -1,8 +1,12 @@
 // Keys and values appended to a paged cache, keys (and queries) rotated on the way.
 //
-// A workgroup has some tokens: cosines and sines into shared memory, then 16-byte accesses of the tokens' vectors.  A key's pieces are
-// written page_size x 16 bytes apart; the tokens of a workgroup, which are neighbours in a prompt, fill the lines between them, so that the
-// cache of their compute units writes whole lines back.
+// A workgroup has some tokens: cosines and sines into shared memory, then 16-byte accesses of the tokens' vectors (32 into 8 bits, of which a lane makes
+// one access of 16).  What bounds many tokens is reading and writing every element once and, into 8 bits, the arithmetic; what bounds few is the launch.
+// A wavefront has a token at a time (or a share of one), so that what depends on the token's slot is scalar work, and asks for its first
+// elements before the angles and the slot are there (8191 tokens of 32 query and 8 key heads of 128: 43 us, 4.7 TB/s; with the slot first 45).  A key's
+// pieces are written page_size x 16 bytes apart; neighbours of a prompt fill the lines between them, for which the workgroups of 16 tokens run on one
+// of the card's eight dies, behind whose cache they meet (as they come: 46 us).  Pieces gathered in shared memory and written side by side by workgroups of
+// their own took 60.  16384 tokens of 4 heads of 192 and 128 into 8 bits: 26.7 us, 2.4 TB/s (eight elements a lane 28.4).
 #include <stdio.h>
 
 #include "mq_paged.hpp"
@@ -17,129 +21,157 @@ struct AppendArgs {
     char* q_out;
     int64_t k_token, k_head, v_token, v_head, q_token, q_head;       // strides, elements
     const void* slots;
-    int64_t slot_count, tokens, first;
+    int64_t slot_count, tokens, first;          // first: token of this launch
     RotaryTurn turn;
     int slots64, page_shift, kv_heads, q_heads, key_dim, value_dim, per;
-    int key_units, query_units;                 // of a head: accesses, or pairs of them
-    int keys_end, values_end, queries_end;      // of a token's units: keys, then values, then queries, then padding to a multiple of 4
-    SmallDivisor by_token, by_key, by_value, by_query;
+    int keys_end, values_end, queries_end;      // of a token's units: keys, then values, then queries
+    int token_waves;                            // wavefronts that share a token
+    int together;                               // workgroups of 16 tokens, which run on one die; 0: as they come
+    SmallDivisor by_key, by_value, by_query;
 };
-constexpr int kAppendThreads = 256, kAppendTurns = 2048, kAppendTokens = 16;
+constexpr int kAppendThreads = 256, kAppendWaves = 4, kAppendTurns = 2048, kAppendTokens = 16;
 
-// Eight elements as e4m3 codes of their group of 32, which four neighbouring lanes hold: the arithmetic of the MXFP8 quantizer, of fp32 values
-__device__ __forceinline__ u32x2 kept_codes8(const float* f, uint32_t& e) {
+// Sixteen elements as e4m3 codes of their group of 32, which two neighbouring lanes hold: the arithmetic of the MXFP8 quantizer, of fp32 values
+__device__ __forceinline__ u32x4 kept_codes16(const float* f, uint32_t& e) {
     float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = keep_larger(m, f[i]);
-    const uint32_t top = group_max4(f2u(m));
+    for (int i = 0; i < 16; i++) m = keep_larger(m, f[i]);
+    const uint32_t top = group_max2(f2u(m));
     e = keep_exponent(top);
     const float inv = e8m0_inverse(e);
-    return u32x2{keep_codes4(f[0], f[1], f[2], f[3], inv, top == kInfinity), keep_codes4(f[4], f[5], f[6], f[7], inv, top == kInfinity)};
+    const bool infinite = top == kInfinity;
+    return u32x4{keep_codes4(f[0], f[1], f[2], f[3], inv, infinite), keep_codes4(f[4], f[5], f[6], f[7], inv, infinite),
+                 keep_codes4(f[8], f[9], f[10], f[11], inv, infinite), keep_codes4(f[12], f[13], f[14], f[15], inv, infinite)};
+}
+
+// An access: eight elements of a vector and, where they are turned in the halves layout, their partners.  In 16 bits a lane has both and writes both; in 8
+// bits it writes its own, beside which its group's other three lanes have theirs.
+struct Access {
+    const char* x;
+    int at, partner;               // bytes; partner < 0: none
+};
+// unit: of a vector, of all its pieces (OWN) or of pairs of pieces and the pieces behind them
+template <bool INTER, bool OWN>
+__device__ __forceinline__ Access access_of(const char* x, int unit, int turned, int half) {
+    if (INTER) return Access{x, unit * 16, -1};
+    if (OWN) return Access{x, unit * 16, unit >= 2 * turned ? -1 : unit * 16 + (unit >= turned ? -half : half)};
+    return unit < turned ? Access{x, unit * 16, half + unit * 16} : Access{x, half + unit * 16, -1};
+}
+// p and its partner r turned, for both to be written
+template <int D, bool INTER>
+__device__ __forceinline__ void turn_both(const Access& x, u32x4& p, u32x4& r, const f32x2_t* turn, int half) {
+    if (INTER) {
+        if (x.at < 2 * half) turn_neighbours<D>(p, turn + x.at / 4);
+    } else if (x.partner >= 0) turn_halves<D>(p, r, turn + x.at / 2);
+}
+// the eight own elements, turned, as fp32
+template <int D, bool INTER>
+__device__ __forceinline__ void turn_own(const Access& x, u32x4 p, u32x4 r, const f32x2_t* turn, int half, float* f) {
+    unpack<D>(p, f);
+    if (INTER) {
+        if (x.at >= 2 * half) return;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const f32x2_t w = turn[x.at / 4 + j / 2];
+            const float a = f[j], b = f[j + 1];
+            f[j] = a * w.x - b * w.y;
+            f[j + 1] = b * w.x + a * w.y;
+        }
+    } else if (x.partner >= 0) {
+        const bool second = x.partner < x.at;
+        float g[8];
+        unpack<D>(r, g);
+        const f32x2_t* w = turn + (second ? x.partner : x.at) / 2;
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] = f[j] * w[j].x - g[j] * (second ? -w[j].y : w[j].y);
+    }
 }
 
 template <int D, bool INTER, bool KEPT>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendArgs a) {
     __shared__ __attribute__((aligned(16))) f32x2_t cs[kAppendTurns];
-    __shared__ int64_t slot[kAppendTokens];
-    const int64_t token0 = a.first + (int64_t)blockIdx.x * a.per;
+    uint32_t nth = blockIdx.x;
+    if (a.together) {                                     // consecutive workgroups run on the eight dies in turn
+        const uint32_t all = 8 * a.together, set = nth / all, in = nth - set * all;
+        if ((set + 1) * all <= gridDim.x) nth = (set * 8 + in % 8) * a.together + in / 8;
+    }
+    const int64_t token0 = a.first + (int64_t)nth * a.per;
     const int here = (int)(a.tokens - token0 < a.per ? a.tokens - token0 : a.per), pairs = a.turn.pairs;
-    for (int i = threadIdx.x; i < here * pairs; i += kAppendThreads) {
-        const int t = i / pairs;
-        cs[i] = turn_of(a.turn, index_at(a.turn.positions, token0 + t, a.turn.positions64), i - t * pairs);
-    }
-    if ((int)threadIdx.x < here) {
-        const int64_t s = index_at(a.slots, token0 + threadIdx.x, a.slots64);
-        slot[threadIdx.x] = inside(s, a.slot_count) ? s : -1;
-    }
-    __syncthreads();
-    const int page_size = 1 << a.page_shift, half = pairs * 2;           // (bytes)
-    const int turned = INTER ? pairs / 4 : pairs / 8;                    // units
-    for (uint32_t i = threadIdx.x, n = (uint32_t)here * a.by_token.d; i < n; i += kAppendThreads) {
-        const uint32_t t = divide(i, a.by_token);
-        int unit = (int)(i - t * a.by_token.d);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int half = pairs * 2, turned = INTER ? pairs / 4 : pairs / 8;           // bytes, units
+    const int pieces = a.key_dim / (KEPT ? 16 : 8), share = wave % a.token_waves;
+    const uint32_t key_head = (uint32_t)(pieces * 16) << a.page_shift, value_head = (uint32_t)(a.value_dim * (KEPT ? 1 : 2)) << a.page_shift;       // bytes
+    const uint32_t key_groups = (uint32_t)(a.key_dim / 32) << a.page_shift, value_groups = (uint32_t)(a.value_dim / 32) << a.page_shift;
+    bool prepared = false;
+    for (int t = wave / a.token_waves; t < here || !prepared; t += kAppendWaves / a.token_waves) {
+        const int64_t token = token0 + (t < here ? t : 0), given = index_at(a.slots, token, a.slots64);
+        const char *const k = a.k + token * a.k_token * 2, *const v = a.v + token * a.v_token * 2, *const q = a.q + token * a.q_token * 2;
+        char* const q_out = a.q_out + token * ((int64_t)a.q_heads * a.key_dim * 2);
         const f32x2_t* turn = cs + t * pairs;
-        const bool is_key = unit < a.keys_end;
-        if (is_key || unit < a.values_end) {
-            const int64_t s = slot[t];
-            if (s < 0) continue;                                         // (of all lanes of a group alike)
-            if (!is_key) unit -= a.keys_end;
-            const int h = (int)divide(unit, is_key ? a.by_key : a.by_value);
-            unit -= h * (int)(is_key ? a.by_key.d : a.by_value.d);
-            const int64_t at = (s >> a.page_shift) * a.kv_heads + h;     // page and head
-            const int place = (int)(s & (page_size - 1));
-            if (!is_key) {
-                const u32x4 v = ld16(a.v + ((token0 + t) * a.v_token + (int64_t)h * a.v_head + unit * 8) * 2);
-                const int64_t to = ((at << a.page_shift) + place) * a.value_dim + unit * 8;
-                if (KEPT) {
-                    float f[8];
-                    uint32_t e;
-                    unpack<D>(v, f);
-                    *(u32x2*)(a.values + to) = kept_codes8(f, e);
-                    if (unit % 4 == 0) a.value_scales[((at * (a.value_dim / 32) + unit / 4) << a.page_shift) + place] = (uint8_t)e;
-                } else *(u32x4*)(a.values + to * 2) = v;
-                continue;
+        const int n = t < here ? a.queries_end : 0, step = a.token_waves * kWave;
+        for (int i = share * kWave + lane; i < n || !prepared; i += step) {
+            // the first access is on its way while the angles are computed and the slot is asked for
+            const bool is_key = i < a.keys_end, is_value = !is_key && i < a.values_end;
+            const SmallDivisor by = is_key ? a.by_key : is_value ? a.by_value : a.by_query;
+            uint32_t unit = (uint32_t)i - (is_key ? 0 : is_value ? a.keys_end : a.values_end);
+            const uint32_t head = divide(unit, by);
+            unit -= __umul24(head, by.d);
+            const char* from = (is_key ? k : is_value ? v : q) + (int64_t)head * (is_key ? a.k_head : is_value ? a.v_head : a.q_head) * 2;
+            Access x, x2;                                 // x2: the second eight of sixteen elements that go into 8 bits
+            if (KEPT && is_key) {
+                x = access_of<INTER, true>(from, 2 * unit, turned, half);
+                x2 = access_of<INTER, true>(from, 2 * unit + 1, turned, half);
+            } else if (KEPT && is_value) {
+                x = Access{from, (int)unit * 32, -1};
+                x2 = Access{from, (int)unit * 32 + 16, -1};
+            } else x = is_value ? Access{from, (int)unit * 16, -1} : access_of<INTER, false>(from, unit, turned, half);
+            const bool two = KEPT && (is_key || is_value);
+            u32x4 p = {}, r = {}, p2 = {}, r2 = {};
+            if (i < n) {
+                p = ld16_keep(x.x + x.at);
+                if (two) p2 = ld16_keep(x2.x + x2.at);
+                if (x.partner >= 0) r = ld16_keep(x.x + x.partner);
+                if (two && x2.partner >= 0) r2 = ld16_keep(x2.x + x2.partner);
             }
-            const char* x = a.k + ((token0 + t) * a.k_token + (int64_t)h * a.k_head) * 2;
-            if (KEPT) {
-                // a lane has the eight elements that it writes, and their partners
-                float f[8];
-                const u32x4 own = ld16_keep(x + unit * 16);
-                unpack<D>(own, f);
-                if (INTER) {
-                    if (unit < turned) {
-#pragma unroll
-                        for (int j = 0; j < 8; j += 2) {
-                            const f32x2_t w = turn[unit * 4 + j / 2];
-                            const float p = f[j], r = f[j + 1];
-                            f[j] = p * w.x - r * w.y;
-                            f[j + 1] = r * w.x + p * w.y;
-                        }
-                    }
-                } else if (unit < 2 * turned) {
-                    const bool second = unit >= turned;
-                    float g[8];
-                    unpack<D>(ld16_keep(x + unit * 16 + (second ? -half : half)), g);
-                    const f32x2_t* w = turn + (second ? unit - turned : unit) * 8;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) f[j] = f[j] * w[j].x - g[j] * (second ? -w[j].y : w[j].y);
+            if (!prepared) {
+                for (int j = threadIdx.x; j < here * pairs; j += kAppendThreads) {
+                    const int tj = j / pairs;
+                    cs[j] = turn_of(a.turn, index_at(a.turn.positions, token0 + tj, a.turn.positions64), j - tj * pairs);
                 }
+                __syncthreads();
+                prepared = true;
+            }
+            const uint64_t slot = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(given >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)given);
+            const bool stored = inside((int64_t)slot, a.slot_count);
+            const uint64_t page = (stored ? slot : 0) >> a.page_shift;
+            const uint32_t place = (uint32_t)slot & ((1u << a.page_shift) - 1);
+            if (i >= n || (!stored && (is_key || is_value))) continue;                    // (a token that is left out has its queries)
+            char* const keys = a.keys + page * ((uint64_t)key_head * a.kv_heads) + place * 16;
+            char* const values = a.values + page * ((uint64_t)value_head * a.kv_heads) + place * (uint32_t)(a.value_dim * (KEPT ? 1 : 2));
+            if (two) {
+                float f[16];
                 uint32_t e;
-                *(u32x2*)(a.keys + ((((at * (a.key_dim / 16) + unit / 2) << a.page_shift) + place) * 16 + (unit & 1) * 8)) = kept_codes8(f, e);
-                if (unit % 4 == 0) a.key_scales[((at * (a.key_dim / 32) + unit / 4) << a.page_shift) + place] = (uint8_t)e;
-                continue;
-            }
-            char* y = a.keys + (((at * (a.key_dim / 8)) << a.page_shift) + place) * 16;         // its first piece
-            if (unit >= turned) {
-                const int piece = (INTER ? 0 : turned) + unit;
-                *(u32x4*)(y + ((int64_t)piece << a.page_shift) * 16) = ld16(x + piece * 16);
-            } else if (INTER) {
-                u32x4 p = ld16(x + unit * 16);
-                turn_neighbours<D>(p, turn + unit * 4);
-                *(u32x4*)(y + ((int64_t)unit << a.page_shift) * 16) = p;
-            } else {
-                u32x4 p = ld16(x + unit * 16), r = ld16(x + half + unit * 16);
-                turn_halves<D>(p, r, turn + unit * 8);
-                *(u32x4*)(y + ((int64_t)unit << a.page_shift) * 16) = p;
-                *(u32x4*)(y + ((int64_t)(unit + turned) << a.page_shift) * 16) = r;
-            }
-        } else if (unit < a.queries_end) {
-            unit -= a.values_end;
-            const int h = (int)divide(unit, a.by_query);
-            unit -= h * (int)a.by_query.d;
-            const char* x = a.q + ((token0 + t) * a.q_token + (int64_t)h * a.q_head) * 2;
-            char* y = a.q_out + ((token0 + t) * a.q_heads + h) * (int64_t)a.key_dim * 2;
-            if (unit >= turned) {
-                const int piece = (INTER ? 0 : turned) + unit;
-                *(u32x4*)(y + piece * 16) = ld16(x + piece * 16);
-            } else if (INTER) {
-                u32x4 p = ld16(x + unit * 16);
-                turn_neighbours<D>(p, turn + unit * 4);
-                *(u32x4*)(y + unit * 16) = p;
-            } else {
-                u32x4 p = ld16(x + unit * 16), r = ld16(x + half + unit * 16);
-                turn_halves<D>(p, r, turn + unit * 8);
-                *(u32x4*)(y + unit * 16) = p;
-                *(u32x4*)(y + half + unit * 16) = r;
+                if (is_key) {
+                    turn_own<D, INTER>(x, p, r, turn, half, f);
+                    turn_own<D, INTER>(x2, p2, r2, turn, half, f + 8);
+                } else {
+                    unpack<D>(p, f);
+                    unpack<D>(p2, f + 8);
+                }
+                const u32x4 codes = kept_codes16(f, e);
+                *(u32x4*)(is_key ? keys + head * key_head + ((unit << a.page_shift) * 16) : values + head * value_head + unit * 16) = codes;
+                if (unit % 2 == 0) {
+                    uint8_t* const scales = is_key ? a.key_scales + page * ((uint64_t)key_groups * a.kv_heads) + head * key_groups
+                                                   : a.value_scales + page * ((uint64_t)value_groups * a.kv_heads) + head * value_groups;
+                    scales[place + ((unit / 2) << a.page_shift)] = (uint8_t)e;
+                }
+            } else if (is_value) *(u32x4*)(values + head * value_head + unit * 16) = p;
+            else {
+                turn_both<D, INTER>(x, p, r, turn, half);
+                char* y = is_key ? keys + head * key_head : q_out + __umul24(head, (uint32_t)a.key_dim * 2);
+                const int spread = is_key ? a.page_shift : 0;
+                *(u32x4*)(y + ((uint32_t)x.at << spread)) = p;
+                if (x.partner >= 0) *(u32x4*)(y + ((uint32_t)x.partner << spread)) = r;
             }
         }
     }
@@ -195,22 +227,26 @@ extern "C" int mq_cache_append(const mq_paged_cache* c, const mq_heads* k, const
     a.turn = RotaryTurn{positions, inv_freq, scale, (int)pairs, positions64, freq64, 0};
     a.kv_heads = (int)c->kv_heads, a.key_dim = (int)c->key_dim, a.value_dim = (int)c->value_dim;
     const bool kept = c->key_scales;
-    a.query_units = (int)(interleaved ? c->key_dim / 8 : (c->key_dim - pairs) / 8);
-    a.key_units = kept ? (int)c->key_dim / 8 : a.query_units;
-    const int64_t keys = c->kv_heads * a.key_units, values = c->kv_heads * (c->value_dim / 8), queries = a.q_heads * (int64_t)a.query_units;
-    const int64_t units = (keys + values + queries + 3) / 4 * 4;
-    if (units > 65532) return mq_fail(MQ_ERR_ARG, "mq_cache_append: tensor too large");
-    a.keys_end = (int)keys, a.values_end = (int)(keys + values), a.queries_end = (int)(keys + values + queries);
-    a.by_token = small_divisor((uint32_t)units);
-    a.by_key = small_divisor((uint32_t)a.key_units), a.by_value = small_divisor((uint32_t)c->value_dim / 8), a.by_query = small_divisor((uint32_t)a.query_units);
+    const int query_units = (int)(interleaved ? c->key_dim / 8 : (c->key_dim - pairs) / 8), key_units = kept ? (int)c->key_dim / 16 : query_units;
+    const int value_units = (int)c->value_dim / (kept ? 16 : 8);
+    const int64_t keys = c->kv_heads * key_units, values = c->kv_heads * value_units, queries = a.q_heads * (int64_t)query_units, units = keys + values + queries;
+    if (units > 65535) return mq_fail(MQ_ERR_ARG, "mq_cache_append: tensor too large");
+    a.keys_end = (int)keys, a.values_end = (int)(keys + values), a.queries_end = (int)units;
+    a.by_key = small_divisor((uint32_t)key_units), a.by_value = small_divisor((uint32_t)value_units), a.by_query = small_divisor((uint32_t)query_units);
+    // tokens of a workgroup: for few accesses a lane, while there are workgroups for every compute unit (the 8191 tokens above by one or two 43, by four
+    // 52; the 16384 by one 50, by two 32, by four 27.4, by eight 26.7)
     int64_t per = 1;
-    while (per < kAppendTokens && per * 2 * pairs <= kAppendTurns && tokens / (per * 2) >= 512 && per * 2 * units * units < (1ll << 32)) per *= 2;
+    while (per < kAppendTokens && per * 2 * pairs <= kAppendTurns && tokens / (per * 2) >= 1024 && per * 2 * units <= 640) per *= 2;
     a.per = (int)per;
-    constexpr int64_t kMost = 1 << 23;                    // workgroups of a launch, which has fewer than 2^32 lanes
+    a.token_waves = per >= kAppendWaves ? 1 : kAppendWaves / (int)per;
+    a.together = tokens >= 1024 ? kAppendTokens / (int)per : 0;
+    constexpr int64_t kMost = 1 << 22;                    // tokens of a launch, which has fewer than 2^32 lanes
     const hipStream_t st = (hipStream_t)stream;
-    for (; a.first < tokens; a.first += kMost * per) {
-        const int64_t left = (tokens - a.first + per - 1) / per;
-        const dim3 grid((unsigned)(left < kMost ? left : kMost));
+    const int64_t end = tokens;
+    for (; a.first < end; a.first += kMost) {
+        const int64_t left = end - a.first < kMost ? end - a.first : kMost;
+        a.tokens = a.first + left;
+        const dim3 grid((unsigned)((left + per - 1) / per));
         auto launch = [&](auto type, auto inter, auto in8) {
             append_kernel<decltype(type)::value, decltype(inter)::value, decltype(in8)::value><<<grid, kAppendThreads, 0, st>>>(a);
         };
