@@ -49,63 +49,72 @@ __global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendA
 #pragma unroll
         for (int i = 0; i < kJoinWaves; i++) top = __builtin_fmaxf(top, tops[i]);
     }
+    float all = 0.0f, f[NV][8];
 #pragma unroll
-    for (int nv = 0; nv < NV; nv++) {
-        float all = 0.0f, f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t i0 = 0; i0 < mine; i0 += 64) {
-            if (mine > 64) {                              // (else they are here already)
-                m = kLowest;
-                l = 0.0f;
-                if (i0 + lane < mine) {
-                    const f32x2 x = *(const f32x2*)(nth_part(i0 + lane) + ml);
-                    m = x.x;
-                    l = x.y;
-                }
-            }
-            const float times = i0 + lane < mine ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
-            all += l * times;
-            const int here = mine - i0 < 64 ? (int)(mine - i0) : 64;
-            constexpr int kAtOnce = WAVES > 1 ? 4 : 2;    // loads on their way
-            for (int k0 = 0; k0 < here; k0 += 4 * kAtOnce) {
-                f32x4 x[kAtOnce], y[kAtOnce];
-                float w[kAtOnce];
+    for (int nv = 0; nv < NV; nv++)
 #pragma unroll
-                for (int u = 0; u < kAtOnce; u++) {
-                    const int k = k0 + 4 * u + sub, last = here - 1;
-                    const float of_k = __shfl(times, k & 63);             // (of all lanes: 0 behind the last)
-                    w[u] = k < here ? of_k : 0.0f;
-                    const float* from = nth_part(i0 + (k < here ? k : last)) + row_at + nv * 128;
-                    x[u] = *(const f32x4*)from;
-                    y[u] = *(const f32x4*)(from + 4);
-                }
-#pragma unroll
-                for (int u = 0; u < kAtOnce; u++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        f[i] += x[u][i] * w[u];
-                        f[4 + i] += y[u][i] * w[u];
-                    }
+        for (int i = 0; i < 8; i++) f[nv][i] = 0.0f;
+    for (uint32_t i0 = 0; i0 < mine; i0 += 64) {
+        if (mine > 64) {                                  // (else they are here already)
+            m = kLowest;
+            l = 0.0f;
+            if (i0 + lane < mine) {
+                const f32x2 x = *(const f32x2*)(nth_part(i0 + lane) + ml);
+                m = x.x;
+                l = x.y;
             }
         }
+        const float times = i0 + lane < mine ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
+        all += l * times;
+        const int here = mine - i0 < 64 ? (int)(mine - i0) : 64;
+        constexpr int kAtOnce = (WAVES > 1 ? 4 : 3) / NV + 1;         // loads on their way
+        for (int k0 = 0; k0 < here; k0 += 4 * kAtOnce) {
+            f32x4 x[kAtOnce][NV], y[kAtOnce][NV];
+            float w[kAtOnce];
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+            for (int u = 0; u < kAtOnce; u++) {
+                const int k = k0 + 4 * u + sub, last = here - 1;
+                const float of_k = __shfl(times, k & 63);             // (of all lanes: 0 behind the last)
+                w[u] = k < here ? of_k : 0.0f;
+                const float* from = nth_part(i0 + (k < here ? k : last)) + row_at;
 #pragma unroll
-        for (int i = 0; i < 8; i++) f[i] = sum_of_head(f[i]);
+                for (int nv = 0; nv < NV; nv++) {
+                    x[u][nv] = *(const f32x4*)(from + nv * 128);
+                    y[u][nv] = *(const f32x4*)(from + nv * 128 + 4);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; u++)
+#pragma unroll
+                for (int nv = 0; nv < NV; nv++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        f[nv][i] += x[u][nv][i] * w[u];
+                        f[nv][4 + i] += y[u][nv][i] * w[u];
+                    }
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+#pragma unroll
+    for (int nv = 0; nv < NV; nv++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[nv][i] = sum_of_head(f[nv][i]);
         if (WAVES > 1) {
             if (lane < 16) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) sums[wave][piece][i] = f[i];
+                for (int i = 0; i < 8; i++) sums[wave][piece][i] = f[nv][i];
                 sums[wave][piece][8] = all;
             }
             __syncthreads();
-            all = 0.0f;
+            if (nv == 0) all = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[i] = 0.0f;
+            for (int i = 0; i < 8; i++) f[nv][i] = 0.0f;
 #pragma unroll
             for (int w = 0; w < kJoinWaves; w++) {
-                all += sums[w][piece][8];
+                if (nv == 0) all += sums[w][piece][8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) f[i] += sums[w][piece][i];
+                for (int i = 0; i < 8; i++) f[nv][i] += sums[w][piece][i];
             }
             __syncthreads();
         }
@@ -113,8 +122,8 @@ __global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendA
         if (lane < 16 && nth_wave == 0 && at < a.value_dim) {
             const float times = finish_factor(a, head, top, all);
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[i] *= times;
-            store8<D>(a.out + (nth * a.value_dim + at) * 2, f);
+            for (int i = 0; i < 8; i++) f[nv][i] *= times;
+            store8<D>(a.out + (nth * a.value_dim + at) * 2, f[nv]);
         }
     }
 }

@@ -2,11 +2,11 @@
 //
 // A workgroup has some tokens: cosines and sines into shared memory, then 16-byte accesses of the tokens' vectors (32 into 8 bits, of which a lane makes
 // one access of 16).  What bounds many tokens is reading and writing every element once and, into 8 bits, the arithmetic; what bounds few is the launch.
-// A wavefront has a token at a time (or a share of one), so that what depends on the token's slot is scalar work, and asks for its first
-// elements before the angles and the slot are there (8191 tokens of 32 query and 8 key heads of 128: 43 us, 4.7 TB/s; with the slot first 45).  A key's
-// pieces are written page_size x 16 bytes apart; neighbours of a prompt fill the lines between them, for which the workgroups of 16 tokens run on one
-// of the card's eight dies, behind whose cache they meet (as they come: 46 us).  Pieces gathered in shared memory and written side by side by workgroups of
-// their own took 60.  16384 tokens of 4 heads of 192 and 128 into 8 bits: 26.7 us, 2.4 TB/s (eight elements a lane 28.4).
+// What depends on a token alone, its slot's address above all, one lane computes into shared memory (every lane for itself: 16384 tokens of 4 heads of
+// 192 and 128 into 8 bits 28 us; this takes 23.5, 2.7 TB/s, and a wavefront to a token 26.7), and the first elements are asked for before the angles and the slots are there.  A
+// key's pieces are written page_size x 16 bytes apart; neighbours of a prompt fill the lines between them, for which the workgroups of 16 tokens run on
+// one of the card's eight dies, behind whose cache they meet (8191 tokens of 32 query and 8 key heads of 128: 45 us, 4.5 TB/s, and 47 as they come).
+// Pieces gathered in shared memory and written side by side by workgroups of their own took 60.
 #include <stdio.h>
 
 #include "mq_paged.hpp"
@@ -24,12 +24,11 @@ struct AppendArgs {
     int64_t slot_count, tokens, first;          // first: token of this launch
     RotaryTurn turn;
     int slots64, page_shift, kv_heads, q_heads, key_dim, value_dim, per;
-    int keys_end, values_end, queries_end;      // of a token's units: keys, then values, then queries
-    int token_waves;                            // wavefronts that share a token
+    int keys_end, values_end, queries_end;      // of a token's units: keys, then values, then queries, then none up to a multiple of 2
     int together;                               // workgroups of 16 tokens, which run on one die; 0: as they come
-    SmallDivisor by_key, by_value, by_query;
+    SmallDivisor by_token, by_key, by_value, by_query;
 };
-constexpr int kAppendThreads = 256, kAppendWaves = 4, kAppendTurns = 2048, kAppendTokens = 16;
+constexpr int kAppendThreads = 256, kAppendTurns = 2048, kAppendTokens = 16;
 
 // Sixteen elements as e4m3 codes of their group of 32, which two neighbouring lanes hold: the arithmetic of the MXFP8 quantizer, of fp32 values
 __device__ __forceinline__ u32x4 kept_codes16(const float* f, uint32_t& e) {
@@ -90,89 +89,100 @@ __device__ __forceinline__ void turn_own(const Access& x, u32x4 p, u32x4 r, cons
 template <int D, bool INTER, bool KEPT>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendArgs a) {
     __shared__ __attribute__((aligned(16))) f32x2_t cs[kAppendTurns];
+    __shared__ const char* from[3][kAppendTokens];        // a token's keys, values and queries,
+    __shared__ char* to[3][kAppendTokens];                // its place in the first head's keys and values, and its turned queries
+    __shared__ uint8_t* scales_to[2][KEPT ? kAppendTokens : 1];
+    __shared__ bool stored[kAppendTokens];
     uint32_t nth = blockIdx.x;
     if (a.together) {                                     // consecutive workgroups run on the eight dies in turn
         const uint32_t all = 8 * a.together, set = nth / all, in = nth - set * all;
         if ((set + 1) * all <= gridDim.x) nth = (set * 8 + in % 8) * a.together + in / 8;
     }
     const int64_t token0 = a.first + (int64_t)nth * a.per;
-    const int here = (int)(a.tokens - token0 < a.per ? a.tokens - token0 : a.per), pairs = a.turn.pairs;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int here = (int)(a.tokens - token0 < a.per ? a.tokens - token0 : a.per), pairs = a.turn.pairs, mine = threadIdx.x;
     const int half = pairs * 2, turned = INTER ? pairs / 4 : pairs / 8;           // bytes, units
-    const int pieces = a.key_dim / (KEPT ? 16 : 8), share = wave % a.token_waves;
+    const int pieces = a.key_dim / (KEPT ? 16 : 8);
     const uint32_t key_head = (uint32_t)(pieces * 16) << a.page_shift, value_head = (uint32_t)(a.value_dim * (KEPT ? 1 : 2)) << a.page_shift;       // bytes
     const uint32_t key_groups = (uint32_t)(a.key_dim / 32) << a.page_shift, value_groups = (uint32_t)(a.value_dim / 32) << a.page_shift;
-    bool prepared = false;
-    for (int t = wave / a.token_waves; t < here || !prepared; t += kAppendWaves / a.token_waves) {
-        const int64_t token = token0 + (t < here ? t : 0), given = index_at(a.slots, token, a.slots64);
-        const char *const k = a.k + token * a.k_token * 2, *const v = a.v + token * a.v_token * 2, *const q = a.q + token * a.q_token * 2;
-        char* const q_out = a.q_out + token * ((int64_t)a.q_heads * a.key_dim * 2);
+    int64_t slot = 0;
+    const char *const k = a.k + token0 * a.k_token * 2, *const v = a.v + token0 * a.v_token * 2, *const q = a.q + token0 * a.q_token * 2;
+    if (mine < here) {
+        slot = index_at(a.slots, token0 + mine, a.slots64);
+        from[0][mine] = k + mine * a.k_token * 2;
+        from[1][mine] = v + mine * a.v_token * 2;
+        from[2][mine] = q + mine * a.q_token * 2;
+    }
+    if (a.per > 1) __syncthreads();
+    const uint32_t n = (uint32_t)here * a.by_token.d;
+    for (uint32_t i = mine; i < n || i == (uint32_t)mine; i += kAppendThreads) {
+        // the first access is on its way while the angles are computed and the slots are asked for
+        const bool some = i < n;
+        const uint32_t t = a.per > 1 && some ? divide(i, a.by_token) : 0u, in_token = i - t * a.by_token.d;
+        const int kind = (int)in_token < a.keys_end ? 0 : (int)in_token < a.values_end ? 1 : 2;
+        const SmallDivisor by = kind == 0 ? a.by_key : kind == 1 ? a.by_value : a.by_query;
+        uint32_t unit = in_token - (kind == 0 ? 0 : kind == 1 ? a.keys_end : a.values_end);
+        const uint32_t head = divide(unit, by);
+        unit -= __umul24(head, by.d);
+        const bool two = KEPT && kind < 2, read = some && (int)in_token < a.queries_end;
+        const char* const x0 = (a.per > 1 ? from[kind][t] : kind == 0 ? k : kind == 1 ? v : q) + (int64_t)head * (kind == 0 ? a.k_head : kind == 1 ? a.v_head : a.q_head) * 2;
+        Access x, x2;                                     // x2: the second eight of sixteen elements that go into 8 bits
+        if (KEPT && kind == 0) {
+            x = access_of<INTER, true>(x0, 2 * unit, turned, half);
+            x2 = access_of<INTER, true>(x0, 2 * unit + 1, turned, half);
+        } else if (KEPT && kind == 1) {
+            x = Access{x0, (int)unit * 32, -1};
+            x2 = Access{x0, (int)unit * 32 + 16, -1};
+        } else x = kind == 1 ? Access{x0, (int)unit * 16, -1} : access_of<INTER, false>(x0, unit, turned, half);
+        u32x4 p = {}, r = {}, p2 = {}, r2 = {};
+        if (read) {
+            p = ld16_keep(x.x + x.at);
+            if (two) p2 = ld16_keep(x2.x + x2.at);
+            if (x.partner >= 0) r = ld16_keep(x.x + x.partner);
+            if (two && x2.partner >= 0) r2 = ld16_keep(x2.x + x2.partner);
+        }
+        if (i == (uint32_t)mine) {
+            for (int j = mine; j < here * pairs; j += kAppendThreads) {
+                const int tj = j / pairs;
+                cs[j] = turn_of(a.turn, index_at(a.turn.positions, token0 + tj, a.turn.positions64), j - tj * pairs);
+            }
+            if (mine < here) {
+                const bool ok = inside(slot, a.slot_count);
+                const uint64_t page = (uint64_t)(ok ? slot : 0) >> a.page_shift;
+                const uint32_t place = (uint32_t)slot & ((1u << a.page_shift) - 1);
+                stored[mine] = ok;
+                to[0][mine] = a.keys + page * ((uint64_t)key_head * a.kv_heads) + place * 16;
+                to[1][mine] = a.values + page * ((uint64_t)value_head * a.kv_heads) + place * (uint32_t)(a.value_dim * (KEPT ? 1 : 2));
+                to[2][mine] = a.q_out + (token0 + mine) * ((int64_t)a.q_heads * a.key_dim * 2);
+                if (KEPT) {
+                    scales_to[0][mine] = a.key_scales + page * ((uint64_t)key_groups * a.kv_heads) + place;
+                    scales_to[1][mine] = a.value_scales + page * ((uint64_t)value_groups * a.kv_heads) + place;
+                }
+            }
+            __syncthreads();
+        }
+        if (!read || (kind < 2 && !stored[t])) continue;  // (a token that is left out has its queries)
         const f32x2_t* turn = cs + t * pairs;
-        const int n = t < here ? a.queries_end : 0, step = a.token_waves * kWave;
-        for (int i = share * kWave + lane; i < n || !prepared; i += step) {
-            // the first access is on its way while the angles are computed and the slot is asked for
-            const bool is_key = i < a.keys_end, is_value = !is_key && i < a.values_end;
-            const SmallDivisor by = is_key ? a.by_key : is_value ? a.by_value : a.by_query;
-            uint32_t unit = (uint32_t)i - (is_key ? 0 : is_value ? a.keys_end : a.values_end);
-            const uint32_t head = divide(unit, by);
-            unit -= __umul24(head, by.d);
-            const char* from = (is_key ? k : is_value ? v : q) + (int64_t)head * (is_key ? a.k_head : is_value ? a.v_head : a.q_head) * 2;
-            Access x, x2;                                 // x2: the second eight of sixteen elements that go into 8 bits
-            if (KEPT && is_key) {
-                x = access_of<INTER, true>(from, 2 * unit, turned, half);
-                x2 = access_of<INTER, true>(from, 2 * unit + 1, turned, half);
-            } else if (KEPT && is_value) {
-                x = Access{from, (int)unit * 32, -1};
-                x2 = Access{from, (int)unit * 32 + 16, -1};
-            } else x = is_value ? Access{from, (int)unit * 16, -1} : access_of<INTER, false>(from, unit, turned, half);
-            const bool two = KEPT && (is_key || is_value);
-            u32x4 p = {}, r = {}, p2 = {}, r2 = {};
-            if (i < n) {
-                p = ld16_keep(x.x + x.at);
-                if (two) p2 = ld16_keep(x2.x + x2.at);
-                if (x.partner >= 0) r = ld16_keep(x.x + x.partner);
-                if (two && x2.partner >= 0) r2 = ld16_keep(x2.x + x2.partner);
+        char* const y = to[kind][t];
+        if (two) {
+            float f[16];
+            uint32_t e;
+            if (kind == 0) {
+                turn_own<D, INTER>(x, p, r, turn, half, f);
+                turn_own<D, INTER>(x2, p2, r2, turn, half, f + 8);
+            } else {
+                unpack<D>(p, f);
+                unpack<D>(p2, f + 8);
             }
-            if (!prepared) {
-                for (int j = threadIdx.x; j < here * pairs; j += kAppendThreads) {
-                    const int tj = j / pairs;
-                    cs[j] = turn_of(a.turn, index_at(a.turn.positions, token0 + tj, a.turn.positions64), j - tj * pairs);
-                }
-                __syncthreads();
-                prepared = true;
-            }
-            const uint64_t slot = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(given >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)given);
-            const bool stored = inside((int64_t)slot, a.slot_count);
-            const uint64_t page = (stored ? slot : 0) >> a.page_shift;
-            const uint32_t place = (uint32_t)slot & ((1u << a.page_shift) - 1);
-            if (i >= n || (!stored && (is_key || is_value))) continue;                    // (a token that is left out has its queries)
-            char* const keys = a.keys + page * ((uint64_t)key_head * a.kv_heads) + place * 16;
-            char* const values = a.values + page * ((uint64_t)value_head * a.kv_heads) + place * (uint32_t)(a.value_dim * (KEPT ? 1 : 2));
-            if (two) {
-                float f[16];
-                uint32_t e;
-                if (is_key) {
-                    turn_own<D, INTER>(x, p, r, turn, half, f);
-                    turn_own<D, INTER>(x2, p2, r2, turn, half, f + 8);
-                } else {
-                    unpack<D>(p, f);
-                    unpack<D>(p2, f + 8);
-                }
-                const u32x4 codes = kept_codes16(f, e);
-                *(u32x4*)(is_key ? keys + head * key_head + ((unit << a.page_shift) * 16) : values + head * value_head + unit * 16) = codes;
-                if (unit % 2 == 0) {
-                    uint8_t* const scales = is_key ? a.key_scales + page * ((uint64_t)key_groups * a.kv_heads) + head * key_groups
-                                                   : a.value_scales + page * ((uint64_t)value_groups * a.kv_heads) + head * value_groups;
-                    scales[place + ((unit / 2) << a.page_shift)] = (uint8_t)e;
-                }
-            } else if (is_value) *(u32x4*)(values + head * value_head + unit * 16) = p;
-            else {
-                turn_both<D, INTER>(x, p, r, turn, half);
-                char* y = is_key ? keys + head * key_head : q_out + __umul24(head, (uint32_t)a.key_dim * 2);
-                const int spread = is_key ? a.page_shift : 0;
-                *(u32x4*)(y + ((uint32_t)x.at << spread)) = p;
-                if (x.partner >= 0) *(u32x4*)(y + ((uint32_t)x.partner << spread)) = r;
-            }
+            const u32x4 codes = kept_codes16(f, e);
+            *(u32x4*)(y + head * (kind == 0 ? key_head : value_head) + (kind == 0 ? (unit << a.page_shift) * 16 : unit * 16)) = codes;
+            if (unit % 2 == 0) scales_to[kind][t][head * (kind == 0 ? key_groups : value_groups) + ((unit / 2) << a.page_shift)] = (uint8_t)e;
+        } else if (kind == 1) *(u32x4*)(y + head * value_head + unit * 16) = p;
+        else {
+            turn_both<D, INTER>(x, p, r, turn, half);
+            const uint32_t at_head = kind == 0 ? head * key_head : __umul24(head, (uint32_t)a.key_dim * 2);
+            const int spread = kind == 0 ? a.page_shift : 0;
+            *(u32x4*)(y + at_head + ((uint32_t)x.at << spread)) = p;
+            if (x.partner >= 0) *(u32x4*)(y + at_head + ((uint32_t)x.partner << spread)) = r;
         }
     }
 }
@@ -229,16 +239,16 @@ extern "C" int mq_cache_append(const mq_paged_cache* c, const mq_heads* k, const
     const bool kept = c->key_scales;
     const int query_units = (int)(interleaved ? c->key_dim / 8 : (c->key_dim - pairs) / 8), key_units = kept ? (int)c->key_dim / 16 : query_units;
     const int value_units = (int)c->value_dim / (kept ? 16 : 8);
-    const int64_t keys = c->kv_heads * key_units, values = c->kv_heads * value_units, queries = a.q_heads * (int64_t)query_units, units = keys + values + queries;
-    if (units > 65535) return mq_fail(MQ_ERR_ARG, "mq_cache_append: tensor too large");
-    a.keys_end = (int)keys, a.values_end = (int)(keys + values), a.queries_end = (int)units;
+    const int64_t keys = c->kv_heads * key_units, values = c->kv_heads * value_units, queries = a.q_heads * (int64_t)query_units, units = (keys + values + queries + 1) / 2 * 2;
+    if (units > 65534) return mq_fail(MQ_ERR_ARG, "mq_cache_append: tensor too large");
+    a.keys_end = (int)keys, a.values_end = (int)(keys + values), a.queries_end = (int)(keys + values + queries);
+    a.by_token = small_divisor((uint32_t)units);
     a.by_key = small_divisor((uint32_t)key_units), a.by_value = small_divisor((uint32_t)value_units), a.by_query = small_divisor((uint32_t)query_units);
-    // tokens of a workgroup: for few accesses a lane, while there are workgroups for every compute unit (the 8191 tokens above by one or two 43, by four
-    // 52; the 16384 by one 50, by two 32, by four 27.4, by eight 26.7)
+    // tokens of a workgroup: for few accesses a lane, while there are workgroups for every compute unit (the 8191 tokens above by one or two 45, by four
+    // 54; the 16384 by one 49, by two 31, by four 25.5, by eight 23.5)
     int64_t per = 1;
     while (per < kAppendTokens && per * 2 * pairs <= kAppendTurns && tokens / (per * 2) >= 1024 && per * 2 * units <= 640) per *= 2;
     a.per = (int)per;
-    a.token_waves = per >= kAppendWaves ? 1 : kAppendWaves / (int)per;
     a.together = tokens >= 1024 ? kAppendTokens / (int)per : 0;
     constexpr int64_t kMost = 1 << 22;                    // tokens of a launch, which has fewer than 2^32 lanes
     const hipStream_t st = (hipStream_t)stream;
