@@ -86,7 +86,8 @@ __device__ __forceinline__ void turn_own(const Access& x, u32x4 p, u32x4 r, cons
     }
 }
 
-template <int D, bool INTER, bool KEPT>
+// PAST: queries and values go past the caches (keys stay, until their neighbours have come)
+template <int D, bool INTER, bool KEPT, bool PAST>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendArgs a) {
     __shared__ __attribute__((aligned(16))) f32x2_t cs[kAppendTurns];
     __shared__ const char* from[3][kAppendTokens];        // a token's keys, values and queries,
@@ -176,13 +177,18 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendArgs
             const u32x4 codes = kept_codes16(f, e);
             *(u32x4*)(y + head * (kind == 0 ? key_head : value_head) + (kind == 0 ? (unit << a.page_shift) * 16 : unit * 16)) = codes;
             if (unit % 2 == 0) scales_to[kind][t][head * (kind == 0 ? key_groups : value_groups) + ((unit / 2) << a.page_shift)] = (uint8_t)e;
-        } else if (kind == 1) *(u32x4*)(y + head * value_head + unit * 16) = p;
+        } else if (kind == 1) store16<PAST>(y + head * value_head + unit * 16, p);
         else {
             turn_both<D, INTER>(x, p, r, turn, half);
-            const uint32_t at_head = kind == 0 ? head * key_head : __umul24(head, (uint32_t)a.key_dim * 2);
-            const int spread = kind == 0 ? a.page_shift : 0;
-            *(u32x4*)(y + at_head + ((uint32_t)x.at << spread)) = p;
-            if (x.partner >= 0) *(u32x4*)(y + at_head + ((uint32_t)x.partner << spread)) = r;
+            if (kind == 0) {
+                char* const z = y + head * key_head;
+                *(u32x4*)(z + ((uint32_t)x.at << a.page_shift)) = p;
+                if (x.partner >= 0) *(u32x4*)(z + ((uint32_t)x.partner << a.page_shift)) = r;
+            } else {
+                char* const z = y + __umul24(head, (uint32_t)a.key_dim * 2);
+                store16<PAST>(z + x.at, p);
+                if (x.partner >= 0) store16<PAST>(z + x.partner, r);
+            }
         }
     }
 }
@@ -250,6 +256,7 @@ extern "C" int mq_cache_append(const mq_paged_cache* c, const mq_heads* k, const
     while (per < kAppendTokens && per * 2 * pairs <= kAppendTurns && tokens / (per * 2) >= 1024 && per * 2 * units <= 640) per *= 2;
     a.per = (int)per;
     a.together = tokens >= 1024 ? kAppendTokens / (int)per : 0;
+    const bool past = tokens * (a.q_heads * c->key_dim + c->kv_heads * c->value_dim) * 2 >= kPastCaches;
     constexpr int64_t kMost = 1 << 22;                    // tokens of a launch, which has fewer than 2^32 lanes
     const hipStream_t st = (hipStream_t)stream;
     const int64_t end = tokens;
@@ -258,7 +265,10 @@ extern "C" int mq_cache_append(const mq_paged_cache* c, const mq_heads* k, const
         a.tokens = a.first + left;
         const dim3 grid((unsigned)((left + per - 1) / per));
         auto launch = [&](auto type, auto inter, auto in8) {
-            append_kernel<decltype(type)::value, decltype(inter)::value, decltype(in8)::value><<<grid, kAppendThreads, 0, st>>>(a);
+            constexpr int D = decltype(type)::value;
+            constexpr bool kInter = decltype(inter)::value, kKept = decltype(in8)::value;
+            if (past) append_kernel<D, kInter, kKept, true><<<grid, kAppendThreads, 0, st>>>(a);
+            else append_kernel<D, kInter, kKept, false><<<grid, kAppendThreads, 0, st>>>(a);
         };
         auto by_kept = [&](auto type, auto inter) { kept ? launch(type, inter, std::true_type{}) : launch(type, inter, std::false_type{}); };
         auto by_layout = [&](auto type) { interleaved ? by_kept(type, std::true_type{}) : by_kept(type, std::false_type{}); };

@@ -22,7 +22,8 @@ struct RotaryArgs {
 constexpr int kRotaryThreads = 256, kRotaryTurns = 2048, kRotaryTokens = 16;
 
 // VEC: every vector begins at a multiple of 16 bytes, and so does its second half; else element by element
-template <int D, bool INTER, bool VEC>
+// PAST: results go past the caches
+template <int D, bool INTER, bool VEC, bool PAST>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs a) {
     constexpr int V = VEC ? kVec<D> : 1;
     __shared__ __attribute__((aligned(16))) f32x2_t cs[kRotaryTurns];
@@ -54,8 +55,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
         __syncthreads();
     };
     if (VEC) {
-        // The first access is on its way while the angles are computed; one at a time and plain stores measured best (4 x 4096 tokens of 40 heads of 128 in
-        // bf16 in 55 us, 6.1 TB/s; two at a time 57, non-temporal stores 58, the angles first 62; a copy of as many bytes runs at 6.2 to 6.5).
+        // The first access is on its way while the angles are computed, one at a time: 16384 tokens of 40 heads of 128 in bf16 in 56 us, 6.0 TB/s (the
+        // angles first 62; two accesses at a time were 2 us slower; a copy of as many bytes runs at 6.2 to 6.5).
         const bool any = threadIdx.x < n;
         for (uint32_t i = threadIdx.x; i < n || i == threadIdx.x; i += kRotaryThreads) {
             Unit unit = {};
@@ -74,10 +75,10 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
                 if (INTER) turn_neighbours<D>(p, turn + unit.at * (V / 2));
                 else {
                     turn_halves<D>(p, q, turn + unit.at * V);
-                    *(u32x4*)(unit.y + half + at) = q;
+                    store16<PAST>(unit.y + half + at, q);
                 }
             }
-            *(u32x4*)(unit.y + at) = p;
+            store16<PAST>(unit.y + at, p);
         }
     } else {
         angles();
@@ -97,15 +98,18 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryArgs
 }
 
 template <int D>
-int rotary_launch(RotaryArgs a, bool inter, bool vec, hipStream_t st) {
+int rotary_launch(RotaryArgs a, bool inter, bool vec, bool past, hipStream_t st) {
     constexpr int64_t kMost = 1 << 23;                    // workgroups of a launch, which has fewer than 2^32 lanes
     for (; a.first < a.total; a.first += kMost * a.per) {
         const int64_t left = (a.total - a.first + a.per - 1) / a.per;
         const dim3 grid((unsigned)(left < kMost ? left : kMost));
-        if (vec && inter) rotary_kernel<D, true, true><<<grid, kRotaryThreads, 0, st>>>(a);
-        else if (vec) rotary_kernel<D, false, true><<<grid, kRotaryThreads, 0, st>>>(a);
-        else if (inter) rotary_kernel<D, true, false><<<grid, kRotaryThreads, 0, st>>>(a);
-        else rotary_kernel<D, false, false><<<grid, kRotaryThreads, 0, st>>>(a);
+        auto launch = [&](auto kind, auto far) {
+            constexpr bool kInter = decltype(kind)::value, kPast = decltype(far)::value;
+            if (vec) rotary_kernel<D, kInter, true, kPast><<<grid, kRotaryThreads, 0, st>>>(a);
+            else rotary_kernel<D, kInter, false, false><<<grid, kRotaryThreads, 0, st>>>(a);
+        };
+        auto by_past = [&](auto kind) { past ? launch(kind, std::true_type{}) : launch(kind, std::false_type{}); };
+        inter ? by_past(std::true_type{}) : by_past(std::false_type{});
         const int rc = mq_check_launch("mq_rotary");
         if (rc != MQ_OK) return rc;
     }
@@ -159,10 +163,11 @@ extern "C" int mq_rotary(const struct mq_heads* x, int n, int dtype, int64_t bat
            per * 2 * heads * units <= 512)
         per *= 2;
     a.per = (int)per;
+    const bool past = a.total * heads * dim * elem >= kPastCaches;
     a.by_token = small_divisor((uint32_t)(heads * units));
     a.by_head = small_divisor((uint32_t)units);
     const hipStream_t st = (hipStream_t)stream;
-    if (dtype == MQ_BF16) return rotary_launch<MQ_BF16>(a, interleaved, vec, st);
-    if (dtype == MQ_F16) return rotary_launch<MQ_F16>(a, interleaved, vec, st);
-    return rotary_launch<MQ_F32>(a, interleaved, vec, st);
+    if (dtype == MQ_BF16) return rotary_launch<MQ_BF16>(a, interleaved, vec, past, st);
+    if (dtype == MQ_F16) return rotary_launch<MQ_F16>(a, interleaved, vec, past, st);
+    return rotary_launch<MQ_F32>(a, interleaved, vec, past, st);
 }
