@@ -2,11 +2,11 @@
 //
 // A workgroup has some tokens: cosines and sines into shared memory, then 16-byte accesses of the tokens' vectors (32 into 8 bits, of which a lane makes
 // one access of 16).  What bounds many tokens is reading and writing every element once and, into 8 bits, the arithmetic; what bounds few is the launch.
-// What depends on a token alone, its slot's address above all, one lane computes into shared memory (every lane for itself: 16384 tokens of 4 heads of
-// 192 and 128 into 8 bits 28 us; this takes 23.5, 2.7 TB/s, and a wavefront to a token 26.7), and the first elements are asked for before the angles and the slots are there.  A
-// key's pieces are written page_size x 16 bytes apart; neighbours of a prompt fill the lines between them, for which the workgroups of 16 tokens run on
-// one of the card's eight dies, behind whose cache they meet (8191 tokens of 32 query and 8 key heads of 128: 45 us, 4.5 TB/s, and 47 as they come).
-// Pieces gathered in shared memory and written side by side by workgroups of their own took 60.
+// A key's pieces are written page_size x 16 bytes apart; neighbours of a prompt fill the lines between them, for which the workgroups of 16 tokens run on
+// one of the card's eight dies, behind whose cache they meet, and everything that is read once is read past it.
+// 8191 tokens of 32 query and 8 key heads of 128: 36.2 us, 5.6 TB/s (as they come 42.5, read through the cache 46, queries and values past it 38.3, two
+// tokens to a workgroup 37, four 42; pieces gathered in shared memory and written side by side by workgroups of their own 60).  16384 tokens of 4 heads
+// of 192 and 128 into 8 bits: 25.7 us, 2.5 TB/s.
 #include <stdio.h>
 
 #include "mq_paged.hpp"
@@ -21,10 +21,10 @@ struct AppendArgs {
     char* q_out;
     int64_t k_token, k_head, v_token, v_head, q_token, q_head;       // strides, elements
     const void* slots;
-    int64_t slot_count, tokens, first;          // first: token of this launch
+    int64_t slot_count, tokens, first;
     RotaryTurn turn;
     int slots64, page_shift, kv_heads, q_heads, key_dim, value_dim, per;
-    int keys_end, values_end, queries_end;      // of a token's units: keys, then values, then queries, then none up to a multiple of 2
+    int keys_end, values_end, queries_end;      // of a token's units: keys, then values, then queries, then padding to a multiple of 2
     int together;                               // workgroups of 16 tokens, which run on one die; 0: as they come
     SmallDivisor by_token, by_key, by_value, by_query;
 };
@@ -43,151 +43,128 @@ __device__ __forceinline__ u32x4 kept_codes16(const float* f, uint32_t& e) {
                  keep_codes4(f[8], f[9], f[10], f[11], inv, infinite), keep_codes4(f[12], f[13], f[14], f[15], inv, infinite)};
 }
 
-// An access: eight elements of a vector and, where they are turned in the halves layout, their partners.  In 16 bits a lane has both and writes both; in 8
-// bits it writes its own, beside which its group's other three lanes have theirs.
-struct Access {
-    const char* x;
-    int at, partner;               // bytes; partner < 0: none
-};
-// unit: of a vector, of all its pieces (OWN) or of pairs of pieces and the pieces behind them
-template <bool INTER, bool OWN>
-__device__ __forceinline__ Access access_of(const char* x, int unit, int turned, int half) {
-    if (INTER) return Access{x, unit * 16, -1};
-    if (OWN) return Access{x, unit * 16, unit >= 2 * turned ? -1 : unit * 16 + (unit >= turned ? -half : half)};
-    return unit < turned ? Access{x, unit * 16, half + unit * 16} : Access{x, half + unit * 16, -1};
-}
-// p and its partner r turned, for both to be written
+// The eight elements of a key's piece, turned, as fp32: with their partners in the other half where pairs are i and i + pairs
 template <int D, bool INTER>
-__device__ __forceinline__ void turn_both(const Access& x, u32x4& p, u32x4& r, const f32x2_t* turn, int half) {
+__device__ __forceinline__ void turned8(const char* x, int piece, int turned, int half, const f32x2_t* turn, float* f) {
+    const u32x4 own = ld16_keep(x + piece * 16);          // (two lanes read it)
     if (INTER) {
-        if (x.at < 2 * half) turn_neighbours<D>(p, turn + x.at / 4);
-    } else if (x.partner >= 0) turn_halves<D>(p, r, turn + x.at / 2);
-}
-// the eight own elements, turned, as fp32
-template <int D, bool INTER>
-__device__ __forceinline__ void turn_own(const Access& x, u32x4 p, u32x4 r, const f32x2_t* turn, int half, float* f) {
-    unpack<D>(p, f);
-    if (INTER) {
-        if (x.at >= 2 * half) return;
+        unpack<D>(own, f);
+        if (piece >= turned) return;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
-            const f32x2_t w = turn[x.at / 4 + j / 2];
-            const float a = f[j], b = f[j + 1];
-            f[j] = a * w.x - b * w.y;
-            f[j + 1] = b * w.x + a * w.y;
+            const f32x2_t w = turn[piece * 4 + j / 2];
+            const float p = f[j], r = f[j + 1];
+            f[j] = p * w.x - r * w.y;
+            f[j + 1] = r * w.x + p * w.y;
         }
-    } else if (x.partner >= 0) {
-        const bool second = x.partner < x.at;
+    } else if (piece >= 2 * turned) {
+        unpack<D>(own, f);
+    } else {
+        const bool second = piece >= turned;
+        const u32x4 other = ld16_keep(x + piece * 16 + (second ? -half : half));
         float g[8];
-        unpack<D>(r, g);
-        const f32x2_t* w = turn + (second ? x.partner : x.at) / 2;
+        unpack<D>(own, f);
+        unpack<D>(other, g);
+        const f32x2_t* w = turn + (second ? piece - turned : piece) * 8;
 #pragma unroll
         for (int j = 0; j < 8; j++) f[j] = f[j] * w[j].x - g[j] * (second ? -w[j].y : w[j].y);
     }
 }
 
-// PAST: queries and values go past the caches (keys stay, until their neighbours have come)
-template <int D, bool INTER, bool KEPT, bool PAST>
+template <int D, bool INTER, bool KEPT>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(const AppendArgs a) {
     __shared__ __attribute__((aligned(16))) f32x2_t cs[kAppendTurns];
-    __shared__ const char* from[3][kAppendTokens];        // a token's keys, values and queries,
-    __shared__ char* to[3][kAppendTokens];                // its place in the first head's keys and values, and its turned queries
-    __shared__ uint8_t* scales_to[2][KEPT ? kAppendTokens : 1];
-    __shared__ bool stored[kAppendTokens];
+    __shared__ int64_t slot[kAppendTokens];
     uint32_t nth = blockIdx.x;
     if (a.together) {                                     // consecutive workgroups run on the eight dies in turn
         const uint32_t all = 8 * a.together, set = nth / all, in = nth - set * all;
         if ((set + 1) * all <= gridDim.x) nth = (set * 8 + in % 8) * a.together + in / 8;
     }
     const int64_t token0 = a.first + (int64_t)nth * a.per;
-    const int here = (int)(a.tokens - token0 < a.per ? a.tokens - token0 : a.per), pairs = a.turn.pairs, mine = threadIdx.x;
-    const int half = pairs * 2, turned = INTER ? pairs / 4 : pairs / 8;           // bytes, units
-    const int pieces = a.key_dim / (KEPT ? 16 : 8);
-    const uint32_t key_head = (uint32_t)(pieces * 16) << a.page_shift, value_head = (uint32_t)(a.value_dim * (KEPT ? 1 : 2)) << a.page_shift;       // bytes
-    const uint32_t key_groups = (uint32_t)(a.key_dim / 32) << a.page_shift, value_groups = (uint32_t)(a.value_dim / 32) << a.page_shift;
-    int64_t slot = 0;
-    const char *const k = a.k + token0 * a.k_token * 2, *const v = a.v + token0 * a.v_token * 2, *const q = a.q + token0 * a.q_token * 2;
-    if (mine < here) {
-        slot = index_at(a.slots, token0 + mine, a.slots64);
-        from[0][mine] = k + mine * a.k_token * 2;
-        from[1][mine] = v + mine * a.v_token * 2;
-        from[2][mine] = q + mine * a.q_token * 2;
+    const int here = (int)(a.tokens - token0 < a.per ? a.tokens - token0 : a.per), pairs = a.turn.pairs;
+    for (int i = threadIdx.x; i < here * pairs; i += kAppendThreads) {
+        const int t = i / pairs;
+        cs[i] = turn_of(a.turn, index_at(a.turn.positions, token0 + t, a.turn.positions64), i - t * pairs);
     }
-    if (a.per > 1) __syncthreads();
-    const uint32_t n = (uint32_t)here * a.by_token.d;
-    for (uint32_t i = mine; i < n || i == (uint32_t)mine; i += kAppendThreads) {
-        // the first access is on its way while the angles are computed and the slots are asked for
-        const bool some = i < n;
-        const uint32_t t = a.per > 1 && some ? divide(i, a.by_token) : 0u, in_token = i - t * a.by_token.d;
-        const int kind = (int)in_token < a.keys_end ? 0 : (int)in_token < a.values_end ? 1 : 2;
-        const SmallDivisor by = kind == 0 ? a.by_key : kind == 1 ? a.by_value : a.by_query;
-        uint32_t unit = in_token - (kind == 0 ? 0 : kind == 1 ? a.keys_end : a.values_end);
-        const uint32_t head = divide(unit, by);
-        unit -= __umul24(head, by.d);
-        const bool two = KEPT && kind < 2, read = some && (int)in_token < a.queries_end;
-        const char* const x0 = (a.per > 1 ? from[kind][t] : kind == 0 ? k : kind == 1 ? v : q) + (int64_t)head * (kind == 0 ? a.k_head : kind == 1 ? a.v_head : a.q_head) * 2;
-        Access x, x2;                                     // x2: the second eight of sixteen elements that go into 8 bits
-        if (KEPT && kind == 0) {
-            x = access_of<INTER, true>(x0, 2 * unit, turned, half);
-            x2 = access_of<INTER, true>(x0, 2 * unit + 1, turned, half);
-        } else if (KEPT && kind == 1) {
-            x = Access{x0, (int)unit * 32, -1};
-            x2 = Access{x0, (int)unit * 32 + 16, -1};
-        } else x = kind == 1 ? Access{x0, (int)unit * 16, -1} : access_of<INTER, false>(x0, unit, turned, half);
-        u32x4 p = {}, r = {}, p2 = {}, r2 = {};
-        if (read) {
-            p = ld16_keep(x.x + x.at);
-            if (two) p2 = ld16_keep(x2.x + x2.at);
-            if (x.partner >= 0) r = ld16_keep(x.x + x.partner);
-            if (two && x2.partner >= 0) r2 = ld16_keep(x2.x + x2.partner);
-        }
-        if (i == (uint32_t)mine) {
-            for (int j = mine; j < here * pairs; j += kAppendThreads) {
-                const int tj = j / pairs;
-                cs[j] = turn_of(a.turn, index_at(a.turn.positions, token0 + tj, a.turn.positions64), j - tj * pairs);
-            }
-            if (mine < here) {
-                const bool ok = inside(slot, a.slot_count);
-                const uint64_t page = (uint64_t)(ok ? slot : 0) >> a.page_shift;
-                const uint32_t place = (uint32_t)slot & ((1u << a.page_shift) - 1);
-                stored[mine] = ok;
-                to[0][mine] = a.keys + page * ((uint64_t)key_head * a.kv_heads) + place * 16;
-                to[1][mine] = a.values + page * ((uint64_t)value_head * a.kv_heads) + place * (uint32_t)(a.value_dim * (KEPT ? 1 : 2));
-                to[2][mine] = a.q_out + (token0 + mine) * ((int64_t)a.q_heads * a.key_dim * 2);
-                if (KEPT) {
-                    scales_to[0][mine] = a.key_scales + page * ((uint64_t)key_groups * a.kv_heads) + place;
-                    scales_to[1][mine] = a.value_scales + page * ((uint64_t)value_groups * a.kv_heads) + place;
-                }
-            }
-            __syncthreads();
-        }
-        if (!read || (kind < 2 && !stored[t])) continue;  // (a token that is left out has its queries)
+    if ((int)threadIdx.x < here) {
+        const int64_t s = index_at(a.slots, token0 + threadIdx.x, a.slots64);
+        slot[threadIdx.x] = inside(s, a.slot_count) ? s : -1;
+    }
+    __syncthreads();
+    const int page_size = 1 << a.page_shift, half = pairs * 2;           // (bytes)
+    const int turned = INTER ? pairs / 4 : pairs / 8;                    // units
+    for (uint32_t i = threadIdx.x, n = (uint32_t)here * a.by_token.d; i < n; i += kAppendThreads) {
+        const uint32_t t = divide(i, a.by_token);
+        int unit = (int)(i - t * a.by_token.d);
         const f32x2_t* turn = cs + t * pairs;
-        char* const y = to[kind][t];
-        if (two) {
-            float f[16];
-            uint32_t e;
-            if (kind == 0) {
-                turn_own<D, INTER>(x, p, r, turn, half, f);
-                turn_own<D, INTER>(x2, p2, r2, turn, half, f + 8);
-            } else {
-                unpack<D>(p, f);
-                unpack<D>(p2, f + 8);
+        const bool is_key = unit < a.keys_end;
+        if (is_key || unit < a.values_end) {
+            const int64_t s = slot[t];
+            if (s < 0) continue;                                         // (of all lanes of a group alike)
+            if (!is_key) unit -= a.keys_end;
+            const int h = (int)divide(unit, is_key ? a.by_key : a.by_value);
+            unit -= h * (int)(is_key ? a.by_key.d : a.by_value.d);
+            const int64_t at = (s >> a.page_shift) * a.kv_heads + h;     // page and head
+            const int place = (int)(s & (page_size - 1));
+            if (KEPT) {                                                  // sixteen elements
+                float f[16];
+                uint32_t e;
+                if (is_key) {
+                    const char* x = a.k + ((token0 + t) * a.k_token + (int64_t)h * a.k_head) * 2;
+                    turned8<D, INTER>(x, 2 * unit, turned, half, turn, f);
+                    turned8<D, INTER>(x, 2 * unit + 1, turned, half, turn, f + 8);
+                } else {
+                    const char* x = a.v + ((token0 + t) * a.v_token + (int64_t)h * a.v_head + unit * 16) * 2;
+                    unpack<D>(ld16(x), f);
+                    unpack<D>(ld16(x + 16), f + 8);
+                }
+                const u32x4 codes = kept_codes16(f, e);
+                if (is_key) *(u32x4*)(a.keys + (((at * (a.key_dim / 16) + unit) << a.page_shift) + place) * 16) = codes;
+                else *(u32x4*)(a.values + ((at << a.page_shift) + place) * a.value_dim + unit * 16) = codes;
+                if (unit % 2 == 0) {
+                    uint8_t* const scales = is_key ? a.key_scales : a.value_scales;
+                    scales[((at * ((is_key ? a.key_dim : a.value_dim) / 32) + unit / 2) << a.page_shift) + place] = (uint8_t)e;
+                }
+                continue;
             }
-            const u32x4 codes = kept_codes16(f, e);
-            *(u32x4*)(y + head * (kind == 0 ? key_head : value_head) + (kind == 0 ? (unit << a.page_shift) * 16 : unit * 16)) = codes;
-            if (unit % 2 == 0) scales_to[kind][t][head * (kind == 0 ? key_groups : value_groups) + ((unit / 2) << a.page_shift)] = (uint8_t)e;
-        } else if (kind == 1) store16<PAST>(y + head * value_head + unit * 16, p);
-        else {
-            turn_both<D, INTER>(x, p, r, turn, half);
-            if (kind == 0) {
-                char* const z = y + head * key_head;
-                *(u32x4*)(z + ((uint32_t)x.at << a.page_shift)) = p;
-                if (x.partner >= 0) *(u32x4*)(z + ((uint32_t)x.partner << a.page_shift)) = r;
+            if (!is_key) {
+                *(u32x4*)(a.values + (((at << a.page_shift) + place) * a.value_dim + unit * 8) * 2) =
+                    ld16(a.v + ((token0 + t) * a.v_token + (int64_t)h * a.v_head + unit * 8) * 2);
+                continue;
+            }
+            const char* x = a.k + ((token0 + t) * a.k_token + (int64_t)h * a.k_head) * 2;
+            char* y = a.keys + (((at * (a.key_dim / 8)) << a.page_shift) + place) * 16;         // its first piece
+            if (unit >= turned) {
+                const int piece = (INTER ? 0 : turned) + unit;
+                *(u32x4*)(y + ((int64_t)piece << a.page_shift) * 16) = ld16(x + piece * 16);
+            } else if (INTER) {
+                u32x4 p = ld16(x + unit * 16);
+                turn_neighbours<D>(p, turn + unit * 4);
+                *(u32x4*)(y + ((int64_t)unit << a.page_shift) * 16) = p;
             } else {
-                char* const z = y + __umul24(head, (uint32_t)a.key_dim * 2);
-                store16<PAST>(z + x.at, p);
-                if (x.partner >= 0) store16<PAST>(z + x.partner, r);
+                u32x4 p = ld16(x + unit * 16), r = ld16(x + half + unit * 16);
+                turn_halves<D>(p, r, turn + unit * 8);
+                *(u32x4*)(y + ((int64_t)unit << a.page_shift) * 16) = p;
+                *(u32x4*)(y + ((int64_t)(unit + turned) << a.page_shift) * 16) = r;
+            }
+        } else if (unit < a.queries_end) {
+            unit -= a.values_end;
+            const int h = (int)divide(unit, a.by_query);
+            unit -= h * (int)a.by_query.d;
+            const char* x = a.q + ((token0 + t) * a.q_token + (int64_t)h * a.q_head) * 2;
+            char* y = a.q_out + ((token0 + t) * a.q_heads + h) * (int64_t)a.key_dim * 2;
+            if (unit >= turned) {
+                const int piece = (INTER ? 0 : turned) + unit;
+                *(u32x4*)(y + piece * 16) = ld16(x + piece * 16);
+            } else if (INTER) {
+                u32x4 p = ld16(x + unit * 16);
+                turn_neighbours<D>(p, turn + unit * 4);
+                *(u32x4*)(y + unit * 16) = p;
+            } else {
+                u32x4 p = ld16(x + unit * 16), r = ld16(x + half + unit * 16);
+                turn_halves<D>(p, r, turn + unit * 8);
+                *(u32x4*)(y + unit * 16) = p;
+                *(u32x4*)(y + half + unit * 16) = r;
             }
         }
     }
@@ -250,13 +227,12 @@ extern "C" int mq_cache_append(const mq_paged_cache* c, const mq_heads* k, const
     a.keys_end = (int)keys, a.values_end = (int)(keys + values), a.queries_end = (int)(keys + values + queries);
     a.by_token = small_divisor((uint32_t)units);
     a.by_key = small_divisor((uint32_t)key_units), a.by_value = small_divisor((uint32_t)value_units), a.by_query = small_divisor((uint32_t)query_units);
-    // tokens of a workgroup: for few accesses a lane, while there are workgroups for every compute unit (the 8191 tokens above by one or two 45, by four
-    // 54; the 16384 by one 49, by two 31, by four 25.5, by eight 23.5)
+    // tokens of a workgroup: for an access or two a lane, while there are workgroups for every compute unit (the 16384 above by one 35, by two or four
+    // 25.7, by eight 29.7)
     int64_t per = 1;
-    while (per < kAppendTokens && per * 2 * pairs <= kAppendTurns && tokens / (per * 2) >= 1024 && per * 2 * units <= 640) per *= 2;
+    while (per < kAppendTokens && per * 2 * pairs <= kAppendTurns && tokens / (per * 2) >= 1024 && per * 2 * units <= 384) per *= 2;
     a.per = (int)per;
     a.together = tokens >= 1024 ? kAppendTokens / (int)per : 0;
-    const bool past = tokens * (a.q_heads * c->key_dim + c->kv_heads * c->value_dim) * 2 >= kPastCaches;
     constexpr int64_t kMost = 1 << 22;                    // tokens of a launch, which has fewer than 2^32 lanes
     const hipStream_t st = (hipStream_t)stream;
     const int64_t end = tokens;
@@ -267,8 +243,7 @@ extern "C" int mq_cache_append(const mq_paged_cache* c, const mq_heads* k, const
         auto launch = [&](auto type, auto inter, auto in8) {
             constexpr int D = decltype(type)::value;
             constexpr bool kInter = decltype(inter)::value, kKept = decltype(in8)::value;
-            if (past) append_kernel<D, kInter, kKept, true><<<grid, kAppendThreads, 0, st>>>(a);
-            else append_kernel<D, kInter, kKept, false><<<grid, kAppendThreads, 0, st>>>(a);
+            append_kernel<D, kInter, kKept><<<grid, kAppendThreads, 0, st>>>(a);
         };
         auto by_kept = [&](auto type, auto inter) { kept ? launch(type, inter, std::true_type{}) : launch(type, inter, std::false_type{}); };
         auto by_layout = [&](auto type) { interleaved ? by_kept(type, std::true_type{}) : by_kept(type, std::false_type{}); };

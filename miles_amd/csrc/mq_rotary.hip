@@ -6,6 +6,16 @@
 
 namespace mq {
 
+// Results of this many bytes and more go past the caches (non-temporal stores: 16384 tokens of 40 heads of 128 in 56 us instead of 61, 4096 in 17.4 instead of
+// 18.8); fewer may be there still when the next kernel reads them.  A template's argument of the kernel, since stores of both kinds behind one branch
+// become one plain store.
+constexpr int64_t kPastCaches = 16 << 20;
+template <bool PAST>
+__device__ __forceinline__ void store16(char* p, u32x4 v) {
+    if (PAST) st16(p, v);
+    else *(u32x4*)p = v;
+}
+
 struct RotaryArgs {
     const char* in[2];
     char* out[2];
