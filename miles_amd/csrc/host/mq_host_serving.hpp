@@ -175,6 +175,8 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         for (const at::Tensor* t : {k, v, slots, positions, inv_freq, q})
             if (t && t->device() != device) Py_RETURN_NONE;
         at::Tensor turned;
+        for (int i = 0; i < 4; i++)                           // written in place: a graph that saved them before says so
+            if (a[i] != Py_None && !THPVariable_Unpack(a[i]).is_inference()) THPVariable_Unpack(a[i]).unsafeGetTensorImpl()->bump_version();
         {
             pybind11::gil_scoped_release no_gil;
             at::NoGradGuard no_grad;

@@ -14,11 +14,11 @@ namespace mq {
 // totals its lanes hold, and goes through them four at once with 16 lanes of eight elements each.
 constexpr int kJoinThreads = 256, kJoinWaves = 4;
 template <int D, int NV, int WAVES>
-__global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendArgs a, uint32_t workers) {
+__global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendArgs a, uint32_t workers, int64_t first) {
     __shared__ float tops[kJoinWaves];
     __shared__ __attribute__((aligned(16))) float sums[kJoinWaves][16][12];
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x / kWave), piece = lane & 15, sub = lane >> 4, nth_wave = WAVES > 1 ? wave : 0;
-    const int64_t nth = WAVES > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kJoinWaves + wave;
+    const int64_t nth = first + (WAVES > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kJoinWaves + wave);
     if (nth >= (int64_t)a.batch * a.heads) return;        // (with WAVES > 1: never)
     const int b = (int)(nth / a.heads), head = (int)(nth - (int64_t)b * a.heads);
     const uint32_t before = a.starts[b], units = a.starts[b + 1] - before, total = a.starts[a.batch];
@@ -190,14 +190,19 @@ int join_launch(const AttendArgs& a, const AttendPlan& p, hipStream_t st) {
     const uint32_t workers = p.grid * attend_workers(p.head_waves);
     // few heads: many parts each, a workgroup for a head; else a wavefront
     if (rows <= 1024) {
-        if (p.nv == 2) attend_join_kernel<D, 2, 4><<<(unsigned)rows, kJoinThreads, 0, st>>>(a, workers);
-        else attend_join_kernel<D, 1, 4><<<(unsigned)rows, kJoinThreads, 0, st>>>(a, workers);
+        if (p.nv == 2) attend_join_kernel<D, 2, 4><<<(unsigned)rows, kJoinThreads, 0, st>>>(a, workers, 0);
+        else attend_join_kernel<D, 1, 4><<<(unsigned)rows, kJoinThreads, 0, st>>>(a, workers, 0);
         return mq_check_launch("mq_paged_attention");
     }
-    const unsigned grid = (unsigned)((rows + kJoinWaves - 1) / kJoinWaves);
-    if (p.nv == 2) attend_join_kernel<D, 2, 1><<<grid, kJoinThreads, 0, st>>>(a, workers);
-    else attend_join_kernel<D, 1, 1><<<grid, kJoinThreads, 0, st>>>(a, workers);
-    return mq_check_launch("mq_paged_attention");
+    for (int64_t first = 0; first < rows; first += (int64_t)kMostGrid * kJoinWaves) {       // (a launch has fewer than 2^32 lanes)
+        const int64_t groups = (rows - first + kJoinWaves - 1) / kJoinWaves;
+        const unsigned grid = (unsigned)(groups < kMostGrid ? groups : kMostGrid);
+        if (p.nv == 2) attend_join_kernel<D, 2, 1><<<grid, kJoinThreads, 0, st>>>(a, workers, first);
+        else attend_join_kernel<D, 1, 1><<<grid, kJoinThreads, 0, st>>>(a, workers, first);
+        const int rc = mq_check_launch("mq_paged_attention");
+        if (rc != MQ_OK) return rc;
+    }
+    return MQ_OK;
 }
 
 }  // namespace mq

@@ -53,7 +53,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, len
         pages = pages.contiguous()
     lengths = lengths.contiguous()
     sinks = None if sinks is None else sinks.contiguous()
-    window = 0 if window is None else int(window)
+    window = 0 if window is None else min(int(window), 1 << 62)
     scale = 1.0 / math.sqrt(cache.key_dim) if scale is None else float(scale)
     struct, size = cache.struct(q.dtype), ctypes.c_int64()
     out = torch.empty((batch, heads, cache.value_dim), dtype=q.dtype, device=q.device)

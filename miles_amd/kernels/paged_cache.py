@@ -181,6 +181,9 @@ def append_tokens(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, slots: to
     is64 = lambda t, wide: int(t is not None and t.dtype == wide)  # noqa: E731
     address = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     launch.note_direct_call()
+    for t in (cache.keys, cache.values, cache.key_scales, cache.value_scales):
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)         # written in place: a graph that saved it before says so
     with _lib.on_device(k.device):
         _lib.check(_lib.load().mq_cache_append(
             *(None if a is None else ctypes.addressof(a) for a in args), tokens, slots.data_ptr(), is64(slots, torch.int64), address(positions),
