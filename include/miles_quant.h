@@ -196,7 +196,7 @@ int mq_cache_append(const mq_paged_cache* cache, const mq_heads* k, const mq_hea
  * t from max(0, length - window) (window 0: from 0) to length - 1; no such t: zeros.  Head h reads key head h / (heads / kv_heads).
  * Token t of sequence b is place t % page_size of page table[b, t / page_size] (rows table_stride apart, `width` of them); tokens on a page that
  * the cache has not, or behind the table's width, are left out.  A negative length is 0.  sinks [heads] fp32 or NULL.
- * q: element (b, h, i) at b q_batch_stride + h q_head_stride + i, 16-byte aligned, strides multiples of 8; out [batch, heads, value_dim] contiguous, 16-byte aligned.
+ * q: element (b, h, i) at b q_batch_stride + h q_head_stride + i, 16-byte aligned, strides multiples of 8; out [batch, heads, value_dim] contiguous, 16-byte aligned, none of the inputs.
  * ws: mq_paged_attention_workspace's bytes (0: may be NULL), 16-byte aligned.  The work is split by lengths that the device reads, the launch by
  * sizes alone: a captured call holds for other lengths and tables.  Sums are added in an order that depends on the lengths and sizes. */
 int mq_paged_attention_workspace(const mq_paged_cache* cache, int64_t batch, int64_t heads, int64_t width, int64_t window, int64_t* bytes);

@@ -101,7 +101,11 @@ class PagedCache:
 
     def gather(self, slots: torch.Tensor, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """(keys [..., heads, key_dim], values [..., heads, value_dim]) that lie in these slots, restored to `dtype` from 8 bits (bf16 by default).
-        Slots outside of the cache raise, as indices do."""
+        Slots outside of the cache raise; to see them, this waits for the device."""
+        if slots.dtype not in (torch.int64, torch.int32):
+            raise ValueError(f"PagedCache.gather: slots are {slots.dtype}, not int64 or int32")
+        if bool(((slots < 0) | (slots >= self.pages * self.page_size)).any()):
+            raise IndexError(f"PagedCache.gather: a slot outside of the cache's {self.pages * self.page_size}")
         page, place = torch.div(slots, self.page_size, rounding_mode="floor"), slots % self.page_size
         n, flat = slots.shape, lambda t: t.reshape(-1)  # noqa: E731
         page, place = flat(page).long(), flat(place).long()

@@ -145,3 +145,16 @@ def test_refusals():
     with torch.no_grad():
         append_tokens(cache, leaf, v, slots)
     assert torch.equal(cache.gather(slots)[0], k)
+
+
+@pytest.mark.parametrize("kept8", [False, True], ids=["16 bits", "8 bits"])
+def test_more_tokens_than_a_launch_has(kept8):
+    tokens, dim = (1 << 22) + 1013, 32 if kept8 else 8
+    g = torch.Generator(device=DEV).manual_seed(0)
+    cache = PagedCache.empty((tokens + 1023) // 1024, 1024, 1, dim, kept8=kept8)
+    slots = torch.randperm(tokens, generator=g, device=DEV)
+    k, v = (torch.randint(-8, 9, (tokens, 1, dim), generator=g, device=DEV).bfloat16() for _ in range(2))       # (exact in 8 bits)
+    append_tokens(cache, k, v, slots)
+    for part in (slice(0, 70000), slice(tokens - 70000, None)):
+        got = cache.gather(slots[part])
+        assert torch.equal(got[0], k[part]) and torch.equal(got[1], v[part])

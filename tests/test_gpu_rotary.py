@@ -156,3 +156,33 @@ def test_refusals():
         rotary(q.double(), None, positions, freq)
     with pytest.raises(_lib.MilesQuantError, match="1024"):
         rotary(torch.zeros(4, 1, 1032, device=DEV), None, positions, freq)
+
+
+def test_gradients_that_are_broadcast_unused_or_added_up():
+    q, k = (_randn(2, 19, n, 64, dtype=torch.bfloat16, seed=n).requires_grad_(True) for n in (4, 2))
+    positions, freq = torch.arange(19, device=DEV) * 11, rotary_frequencies(64, device=DEV)[0]
+    y, z = rotary(q, k, positions, freq)
+    y.sum().backward()                                     # of ones that share one address; nothing for k
+    assert k.grad is None and torch.equal(q.grad, rotary(torch.ones_like(q), None, positions, freq, inverse=True))
+    y, z = rotary(q, q[:, :, :2], positions, freq)         # the same leaf as both
+    dq = torch.autograd.grad((y.float().sum() + 2 * z.float().sum()), q)[0]
+    ones = rotary(torch.ones_like(q), None, positions, freq, inverse=True).detach()
+    assert torch.equal(dq[:, :, 2:], ones[:, :, 2:]) and torch.equal(dq[:, :, :2], 3 * ones[:, :, :2])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "neighbours"])
+def test_results_that_go_past_the_caches(interleaved, dtype):
+    q, k = (_randn(1, 4099, n, 128, dtype=dtype, seed=n) for n in (12, 4))
+    positions, freq = torch.arange(4099, device=DEV) * 31, rotary_frequencies(96, device=DEV)[0]
+    for x, y in zip((q, k), rotary(q, k, positions, freq, interleaved=interleaved)):
+        _check(x, y, positions, freq, 1.0, interleaved)
+
+
+def test_more_tokens_than_a_launch_has():
+    tokens = 16 * (1 << 23) + 4321
+    x = torch.arange(tokens * 8, dtype=torch.int32, device=DEV).bfloat16().view(tokens, 1, 8)
+    positions, freq = torch.arange(tokens, dtype=torch.int32, device=DEV) % 4096, rotary_frequencies(8, device=DEV)[0]
+    y = rotary(x, None, positions, freq, interleaved=True)
+    for part in (slice(0, 3000), slice(tokens - 6000, None)):
+        assert torch.equal(y[part], rotary(x[part], None, positions[part].clone(), freq, interleaved=True))

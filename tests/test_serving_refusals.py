@@ -51,6 +51,20 @@ def test_tensors_that_are_no_cache():
             PagedCache(*tensors).check("a cache", BF16)
 
 
+def test_gathered_slots():
+    cache = PagedCache.empty(3, 16, 2, 8, device="cpu")
+    cache.keys.copy_(torch.arange(48).view(3, 1, 1, 16, 1).expand_as(cache.keys))
+    cache.values.copy_(torch.arange(48).view(3, 1, 16, 1).expand_as(cache.values))
+    slots = torch.tensor([[0, 47], [16, 31]], dtype=torch.int32)
+    k, v = cache.gather(slots)
+    assert k.shape == v.shape == (2, 2, 2, 8) and torch.equal(k[..., 0, 0].int(), slots) and torch.equal(v[..., 1, 7].int(), slots)
+    for bad in (-1, 48, 1 << 40):
+        with pytest.raises(IndexError, match="outside"):
+            cache.gather(torch.tensor([0, bad]))
+    with pytest.raises(ValueError, match="int64 or int32"):
+        cache.gather(torch.zeros(2))
+
+
 def test_frequencies():
     f, scale = rotary_frequencies(128, 1e6, device="cpu")
     assert f.dtype == torch.float64 and scale == 1.0 and f[0] == 1.0 and abs(f[-1].item() - 1e6 ** (-126 / 128)) < 1e-18
