@@ -27,7 +27,7 @@ __global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendA
     const uint32_t row = units / (uint32_t)(a.kv_heads * a.blocks), u0 = before + (uint32_t)(kv * a.blocks + block) * row, per = units_of_worker(total, workers, a.least);
     // workers that have tiles of the row, which begin behind its first units: the first may have the end of other rows before it
     const uint32_t w0 = (u0 + kRowUnits) / per, w1 = (u0 + row - 1) / per, parts = w1 - w0 + 1;
-    if (parts == 1) return;                               // one worker had it all
+    if (parts == 1 || w1 >= workers) return;              // one worker had it all (or the lengths changed under the first kernel)
     const bool inside_first = u0 > w0 * per;              // the first part is the last of its worker's
     auto part = [&](uint32_t i) { return a.parts + ((int64_t)(w0 + i) * 2 + (i == 0 && inside_first ? 1 : 0)) * part_floats(a.block_heads, NV); };
     const int64_t ml = (int64_t)a.block_heads * (128 * NV) + in_block * 2, row_at = (int64_t)in_block * (128 * NV) + piece * 8;

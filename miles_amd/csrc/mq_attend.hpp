@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 
             }
             before = end;
         }
-        if (u0 >= total) return;
+        if (u0 >= total || b < 0) return;
     }
 
     const int token_wave = DIRECT ? wave / a.head_waves : 0, token_waves = DIRECT ? (int)blockDim.x / kWave / a.head_waves : 1;
@@ -185,7 +185,10 @@ __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 
     for (;;) {                                            // a row, or the part of it that is this worker's
         const Seen seen = seen_uniform(a, b);
         const int tiles = tiles_of(seen);
-        const uint32_t units = units_of(tiles), row = rest / units, from = rest - row * units, to = units - from < left ? units : from + left;
+        const uint32_t units = units_of(tiles);
+        // (as the lengths were read above; should they change meanwhile, results are open, but nothing is read or written out of range)
+        if (units == 0 || rest >= units * rows) return;
+        const uint32_t row = rest / units, from = rest - row * units, to = units - from < left ? units : from + left;
         const int tile0 = from > kRowUnits ? (int)(from - kRowUnits) : 0, tile1 = to > kRowUnits ? (int)(to - kRowUnits) : 0;
         const int kv = (int)row / a.blocks, block = (int)row - kv * a.blocks, head0 = block * a.block_heads + head_wave * 16;      // within the group
         const int heads_here = a.group - head0 < 16 ? a.group - head0 : 16;
@@ -463,7 +466,8 @@ __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 
         first_of_worker = false;
         if (rest == units * rows) {
             rest = 0;
-            do b++;
+            do
+                if (++b == a.batch) return;
             while (tiles_of(seen_uniform(a, b)) == 0);
         }
     }
