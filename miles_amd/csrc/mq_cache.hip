@@ -2,11 +2,11 @@
 //
 // A workgroup has some tokens: cosines and sines into shared memory, then 16-byte accesses of the tokens' vectors (32 into 8 bits, of which a lane makes
 // one access of 16).  What bounds many tokens is reading and writing every element once and, into 8 bits, the arithmetic; what bounds few is the launch.
-// A key's pieces are written page_size x 16 bytes apart; neighbours of a prompt fill the lines between them, for which the workgroups of 16 tokens run on
+// A key's pieces are written page_size x 16 bytes apart; neighbours of a prompt fill the lines between them, for which the workgroups of 64 tokens run on
 // one of the card's eight dies, behind whose cache they meet, and everything that is read once is read past it.
-// 8191 tokens of 32 query and 8 key heads of 128: 36.2 us, 5.6 TB/s (as they come 42.5, read through the cache 46, queries and values past it 38.3, two
+// 8191 tokens of 32 query and 8 key heads of 128: 35.9 us, 5.6 TB/s (as they come 42.5, read through the cache 46, queries and values past it 38.3, two
 // tokens to a workgroup 37, four 42; pieces gathered in shared memory and written side by side by workgroups of their own 60).  16384 tokens of 4 heads
-// of 192 and 128 into 8 bits: 25.7 us, 2.5 TB/s.
+// of 192 and 128 into 8 bits: 24.4 us, 2.6 TB/s (16 tokens on a die 25.6, and 36.2 above; 128 24.3 and 37.6).
 #include <stdio.h>
 
 #include "mq_paged.hpp"
@@ -25,10 +25,10 @@ struct AppendArgs {
     RotaryTurn turn;
     int slots64, page_shift, kv_heads, q_heads, key_dim, value_dim, per;
     int keys_end, values_end, queries_end;      // of a token's units: keys, then values, then queries, then padding to a multiple of 2
-    int together;                               // workgroups of 16 tokens, which run on one die; 0: as they come
+    int together;                               // workgroups of kAppendTogether tokens, which run on one die; 0: as they come
     SmallDivisor by_token, by_key, by_value, by_query;
 };
-constexpr int kAppendThreads = 256, kAppendTurns = 2048, kAppendTokens = 16;
+constexpr int kAppendThreads = 256, kAppendTurns = 2048, kAppendTokens = 16, kAppendTogether = 64;
 
 // Sixteen elements as e4m3 codes of their group of 32, which two neighbouring lanes hold: the arithmetic of the MXFP8 quantizer, of fp32 values
 __device__ __forceinline__ u32x4 kept_codes16(const float* f, uint32_t& e) {
@@ -227,12 +227,12 @@ extern "C" int mq_cache_append(const mq_paged_cache* c, const mq_heads* k, const
     a.keys_end = (int)keys, a.values_end = (int)(keys + values), a.queries_end = (int)(keys + values + queries);
     a.by_token = small_divisor((uint32_t)units);
     a.by_key = small_divisor((uint32_t)key_units), a.by_value = small_divisor((uint32_t)value_units), a.by_query = small_divisor((uint32_t)query_units);
-    // tokens of a workgroup: for an access or two a lane, while there are workgroups for every compute unit (the 16384 above by one 35, by two or four
+    // tokens of a workgroup: for an access or two a lane, while there are workgroups for every compute unit (the 16384 above, 16 on a die, by one 35, by two or four
     // 25.7, by eight 29.7)
     int64_t per = 1;
     while (per < kAppendTokens && per * 2 * pairs <= kAppendTurns && tokens / (per * 2) >= 1024 && per * 2 * units <= 384) per *= 2;
     a.per = (int)per;
-    a.together = tokens >= 1024 ? kAppendTokens / (int)per : 0;
+    a.together = tokens >= 1024 ? kAppendTogether / (int)per : 0;
     constexpr int64_t kMost = 1 << 22;                    // tokens of a launch, which has fewer than 2^32 lanes
     const hipStream_t st = (hipStream_t)stream;
     const int64_t end = tokens;
