@@ -17,38 +17,72 @@ from miles_amd import _lib, launch
 from miles_amd._host import native
 from miles_amd.kernels._rows import unpacked, wants_graph
 
+# names that a kind of scaling needs and those that it may have; names that repeat what is known or change nothing
+_SCALINGS = {"default": (set(), {"factor"}), "linear": ({"factor"}, set()),
+             "yarn": ({"factor", "original_max_position_embeddings"}, {"beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate"})}
+_ANY_SCALING = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "original_max_position_embeddings", "max_position_embeddings"}
+
 
 def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: dict | None = None, device="cuda") -> tuple[torch.Tensor, float]:
     """(inv_freq [dim/2] fp64, scale): the radians that each pair of `dim` elements turns by from one position to the next, `base`^(-2i/dim),
     and what cosines and sines are multiplied with, for `rotary(..., inv_freq, scale=scale)`.
 
-    `scaling` stretches a context, with the names of a checkpoint's configuration: {"rope_type": "linear", "factor"} divides every
-    frequency by the factor; {"rope_type": "yarn", "factor", "original_max_position_embeddings"[, "beta_fast", "beta_slow", "attention_factor"]}
-    keeps pairs that turn more than beta_fast (32) times in the original context, divides those that turn less than beta_slow (1) times, with
-    a ramp between (Peng et al., "YaRN: Efficient context window extension of large language models", 2023)."""
+    `scaling` stretches a context, with the names of a checkpoint's configuration (`rope_type` or `type`): {"rope_type": "linear", "factor"} divides every
+    frequency by the factor; {"rope_type": "yarn", "factor", "original_max_position_embeddings"} keeps pairs that turn more than `beta_fast` (32) times in
+    the original context, divides those that turn less than `beta_slow` (1) times, with a ramp between, whose ends are whole pairs unless `truncate` is
+    False (Peng et al., "YaRN: Efficient context window extension of large language models", 2023).  YaRN's scale is `attention_factor`; without it
+    m(`mscale`) / m(`mscale_all_dim`) where both are given, else m(1), with m(x) = 0.1 x ln(factor) + 1.  (Where a model multiplies its attention's scale
+    by m(mscale_all_dim)^2 as well, that is the attention's argument.)  `rope_theta` has to be the base that is given, and `partial_rotary_factor` 1:
+    `dim` is what turns.  Other names are refused, since they would change the result."""
     if dim < 2 or dim % 2:
         raise ValueError(f"rotary_frequencies: an even number of elements, got {dim}")
     inv_freq = base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
-    kind = None if scaling is None else scaling.get("rope_type", scaling.get("type"))
-    if kind in (None, "default"):
-        return inv_freq.to(device), 1.0
-    if kind not in ("linear", "yarn"):
+    given = {} if scaling is None else {k: v for k, v in scaling.items() if v is not None}
+    kind = given.get("rope_type", given.get("type", "default"))
+    if kind not in _SCALINGS:
         raise ValueError(f"rotary_frequencies: unknown rope_type {kind!r}: linear or yarn (or an inv_freq of one's own)")
-    factor = float(scaling["factor"])
+    needed, optional = _SCALINGS[kind]
+    unknown = given.keys() - _ANY_SCALING - needed - optional
+    if unknown or not needed <= given.keys():
+        raise ValueError(f"rotary_frequencies: rope_type {kind!r} with {', '.join(sorted(map(str, unknown)))}, which is not known" if unknown else
+                         f"rotary_frequencies: rope_type {kind!r} without {', '.join(sorted(needed - given.keys()))}")
+    if given.get("rope_theta", base) != base or given.get("partial_rotary_factor", 1) != 1:
+        raise ValueError(f"rotary_frequencies: a base of {base} and {dim} elements that turn, beside a rope_theta of {given.get('rope_theta')} and a partial_rotary_factor "
+                         f"of {given.get('partial_rotary_factor')}; give them as base and dim")
+    if kind == "default":
+        return inv_freq.to(device), 1.0
+    factor = float(given["factor"])
     if kind == "linear":
         return (inv_freq / factor).to(device), 1.0
-    length = scaling["original_max_position_embeddings"]
+    length, truncate = given["original_max_position_embeddings"], given.get("truncate", True)
+    if not isinstance(truncate, bool):
+        raise ValueError(f"rotary_frequencies: truncate is {truncate!r}, neither True nor False")
 
     def pair_that_turns(times: float) -> float:
         return dim * math.log(length / (times * 2 * math.pi)) / (2 * math.log(base))
 
-    low = max(math.floor(pair_that_turns(scaling.get("beta_fast") or 32)), 0)
-    high = min(math.ceil(pair_that_turns(scaling.get("beta_slow") or 1)), dim - 1)
+    low, high = pair_that_turns(given.get("beta_fast") or 32), pair_that_turns(given.get("beta_slow") or 1)
+    if truncate:
+        low, high = math.floor(low), math.ceil(high)
+    low, high = max(low, 0), min(high, dim - 1)
     slowed = ((torch.arange(dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
-    scale = scaling.get("attention_factor")
-    if scale is None:
-        scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
-    return (inv_freq * (1 - slowed) + inv_freq / factor * slowed).to(device), float(scale)
+    return (inv_freq * (1 - slowed) + inv_freq / factor * slowed).to(device), _yarn_scale(factor, given)
+
+
+def _yarn_scale(factor: float, given: dict) -> float:
+    if "attention_factor" in given:
+        return float(given["attention_factor"])
+
+    def m(x: float) -> float:
+        return 0.1 * x * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+    over, under = given.get("mscale", 1.0), given.get("mscale_all_dim", 0.0)
+    if "mscale" in given and over and under:
+        return m(over) / m(under)
+    if over == 1 and not under or factor <= 1:
+        return m(1.0)
+    raise ValueError(f"rotary_frequencies: mscale {given.get('mscale')} with mscale_all_dim {given.get('mscale_all_dim')}: one of the two alone has no meaning that programs "
+                     "agree on; give both or an attention_factor")
 
 
 def check_frequencies(inv_freq: torch.Tensor, device: torch.device, dim: int, what: str) -> None:
