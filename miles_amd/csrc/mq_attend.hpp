@@ -331,15 +331,17 @@ __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 
                     }
                 }
             }
+            // (times the scale before the maximum is taken from them: a fused operation would round one of the two and not the other, which beyond 2^24 is whole
+            // powers of two, and a weight of 0 or an infinity for the largest score itself)
             float p[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) p[i] = s[i / 4][i & 3];
+            for (int i = 0; i < 8; i++) p[i] = s[i / 4][i & 3] * a.scale;
             float most = p[0];
 #pragma unroll
             for (int i = 1; i < 8; i++) most = __builtin_fmaxf(most, p[i]);
             // The running maximum need not be the largest: weights up to 2^kSlack of it are numbers as good.  Sums are rescaled when it is passed by
             // more, which after a row's first tile hardly ever is.
-            const float higher = max_of_head(most) * a.scale;
+            const float higher = max_of_head(most);
             if (__any(higher > top + kSlack)) {
                 const float now = __builtin_fmaxf(top, higher), f = __builtin_amdgcn_exp2f(top - now);
                 total *= f;
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 
                 top = now;
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], a.scale, -top));
+            for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(p[i] - top);
 #pragma unroll
             for (int i = 0; i < 8; i++) total += p[i];
             uint32_t big[4], small[4];
