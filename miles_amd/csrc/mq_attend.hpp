@@ -7,8 +7,8 @@
 //   output   O^T += V^T P^T: the same lane needs, for element 8 c + e of the values, the weights and values of eight tokens.  Which
 //            eight is free as long as both operands agree: 4 g + r of both halves of the 32, whose weights it has, and
 //            whose values it reads as rows of 16 bytes; eight such rows are rearranged in its own registers, one instruction for two elements.
-// Weights enter as the sum of two 16-bit numbers, so that they are as good as the 32-bit ones (one alone would be off by as much as the
-// result's own rounding); the matrix cores have the time (6 % of the cycles in 16 bits, 10 in 8).  What bounds it is reading keys and values
+// Weights enter as the sum of two 16-bit numbers (one alone would be off by as much as the result's own rounding), which hold 16 bits of them in bf16; in
+// fp16 22, and whatever is above 2^-40 of the largest weight in the same tile.  The matrix cores have the time (6 % of the cycles in 16 bits, 10 in 8).  What bounds it is reading keys and values
 // once: a tile's keys are asked for when the last tile's have been used, its values likewise, so that a wavefront always has one of the two on its way, and two wavefronts on a
 // SIMD keep 64 KB a compute unit in flight.  32 query heads over 8 key heads of 128, bf16: 64 sequences of 8192 tokens 332 us, 6.5 TB/s; 64 of 1 to
 // 8192 in 122, 5.9 TB/s (in 8 bits 125, 6.0 TB/s: half the bytes for twice the tokens); one of 131072 in 93, 5.8 TB/s; one of 1024 in 8.
@@ -117,6 +117,7 @@ template <int D, bool KEPT, int NK, int NV, bool DIRECT, bool SHARED>
 __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 2) void attend_kernel(const AttendArgs a) {
     constexpr int kPolicy = SHARED ? 0 : 2;               // (2: non-temporal)
     constexpr int kLoads = KEPT ? NK / 2 : NK;            // of a tile's half's keys
+    constexpr bool kOwnTop = D == MQ_F16;                 // a tile's weights are relative to its own maximum
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x / kWave), c = lane & 15, g = lane >> 4;
     const int rows = a.kv_heads * a.blocks;               // of a sequence
     const int head_wave = SHARED ? wave % a.head_waves : 0;
@@ -349,17 +350,34 @@ __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 
                 for (int i = 0; i < NV * 8; i++) acc[i] *= f;
                 top = now;
             }
+            // What the weights of this tile are relative to: fp16 ends at 2^-24, so that beside a weight of 1 all that is 2^25 times as small would be lost, which is the
+            // result itself where the first token takes nearly all weight and its value is zero.  So fp16 weights are relative to their own tile's maximum, which
+            // is 2^15 and its sums' factor makes up for; what is lost is below 2^-40 of that, of 32 tokens at most.
+            const float of = kOwnTop ? __builtin_fmaxf(higher, kLowest) : top;
 #pragma unroll
-            for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(p[i] - top);
+            for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(p[i] - of);
+            float times = 1.0f;
+            if (kOwnTop) {
+                times = __builtin_amdgcn_exp2f(of - top);
+                float here = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) total += p[i];
+                for (int i = 0; i < 8; i++) {
+                    here += p[i];
+                    p[i] *= 0x1p15f;
+                }
+                total = __builtin_fmaf(here, times, total);
+                times *= 0x1p-15f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) total += p[i];
+            }
             uint32_t big[4], small[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 big[i] = pack2<D>(p[2 * i], p[2 * i + 1]);
                 small[i] = pack2<D>(p[2 * i] - elem_lo<D == MQ_F16>(big[i]), p[2 * i + 1] - elem_hi<D == MQ_F16>(big[i]));
             }
-            const u32x4 weights = {big[0], big[1], big[2], big[3]}, remainders = {small[0], small[1], small[2], small[3]};
+            const u32x4 weights[2] = {{big[0], big[1], big[2], big[3]}, {small[0], small[1], small[2], small[3]}};
             // ---- values
 #pragma unroll
             for (int nv = 0; nv < NV; nv++) {
@@ -372,13 +390,31 @@ __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 
                         x[i] = u32x4{lo.x, lo.y, hi.x, hi.y};
                     } else x[i] = v[nv][i];
                 }
+                constexpr int kAtOnce = 4;                // products that do not wait for each other
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const uint32_t pick = e & 1 ? 0x07060302u : 0x05040100u;
-                    const u32x4 row8 = {__builtin_amdgcn_perm(x[1][e / 2], x[0][e / 2], pick), __builtin_amdgcn_perm(x[3][e / 2], x[2][e / 2], pick),
+                for (int e0 = 0; e0 < 8; e0 += kAtOnce) {
+                    u32x4 row8[kAtOnce];
+                    f32x4 sum[kAtOnce];
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; i++) {
+                        const int e = e0 + i;
+                        const uint32_t pick = e & 1 ? 0x07060302u : 0x05040100u;
+                        row8[i] = u32x4{__builtin_amdgcn_perm(x[1][e / 2], x[0][e / 2], pick), __builtin_amdgcn_perm(x[3][e / 2], x[2][e / 2], pick),
                                         __builtin_amdgcn_perm(x[5][e / 2], x[4][e / 2], pick), __builtin_amdgcn_perm(x[7][e / 2], x[6][e / 2], pick)};
-                    acc[nv * 8 + e] = mfma<D>(row8, weights, acc[nv * 8 + e]);
-                    acc[nv * 8 + e] = mfma<D>(row8, remainders, acc[nv * 8 + e]);
+                        sum[i] = kOwnTop ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc[nv * 8 + e];
+                    }
+#pragma unroll
+                    for (int part = 0; part < 2; part++)
+#pragma unroll
+                        for (int i = 0; i < kAtOnce; i++) sum[i] = mfma<D>(row8[i], weights[part], sum[i]);
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; i++) {
+                        f32x4& all = acc[nv * 8 + e0 + i];
+                        if (!kOwnTop) all = sum[i];
+                        else
+#pragma unroll
+                            for (int r = 0; r < 4; r++) all[r] = __builtin_fmaf(sum[i][r], times, all[r]);
+                    }
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -394,16 +430,19 @@ __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 
         total = sum_of_head(total);
         if (!DIRECT) {
             const bool whole = tile0 == 0 && tile1 == tiles;
-            const int in_block = head_wave * 16 + c, head = kv * a.group + head0 + c;
+            // the lane's numbers anew, which keeps the addresses below from being computed before the rows and held in up to 30 registers
+            int c1 = c, g1 = g;
+            asm("" : "+v"(c1), "+v"(g1));
+            const int in_block = head_wave * 16 + c1, head = kv * a.group + head0 + c1;
             float* part = a.parts + ((int64_t)worker * 2 + (first_of_worker ? 0 : 1)) * part_floats(a.block_heads, NV);
-            if (c < heads_here) {
+            if (c1 < heads_here) {
                 const float times = whole ? finish_factor(a, head, top, total) : 1.0f;
-                if (!whole && g == 0) *(f32x2*)(part + a.block_heads * (128 * NV) + in_block * 2) = f32x2{top, total};
+                if (!whole && g1 == 0) *(f32x2*)(part + a.block_heads * (128 * NV) + in_block * 2) = f32x2{top, total};
 #pragma unroll
                 for (int nv = 0; nv < NV; nv++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const int at_dim = nv * 128 + 8 * (4 * g + r);
+                        const int at_dim = nv * 128 + 8 * (4 * g1 + r);
                         if (at_dim >= a.value_dim) continue;
                         float f[8];
 #pragma unroll

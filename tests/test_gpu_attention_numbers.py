@@ -1,4 +1,6 @@
-"""Attention over a paged cache where numbers are large, against the formula in 64 bits."""
+"""Attention over a paged cache where numbers are large or small, against the formula in 64 bits."""
+
+import math
 
 import pytest
 import torch
@@ -11,6 +13,10 @@ from tests.serving_checks import DEV
 pytestmark = pytest.mark.gpu
 HALVES = [torch.bfloat16, torch.float16]
 PAGE = 16
+# What a weight is off by as two 16-bit numbers, the second the rounded rest: of itself, and of the largest among the same 32 tokens, which is 2^15 where fp16's
+# smallest steps are 2^-24
+WEIGHT = {torch.bfloat16: 2.0**-17, torch.float16: 2.0**-22}
+SMALLEST = {torch.bfloat16: 0.0, torch.float16: 2.0**-40}
 
 
 def _cache_of(sequences, dtype):
@@ -35,6 +41,32 @@ def _widened(table, tokens):
     return torch.nn.functional.pad(table, (0, max(0, tokens // PAGE - table.shape[1])), value=-1)
 
 
+def formula(q, k, v, scale=None):
+    """(out [heads, value_dim] in 64 bits, a bound on what comes before its rounding) of q [heads, key_dim], k [tokens, key heads, key_dim], v.
+
+    A score is a sum of key_dim products in fp32, off by (key_dim + 4) 2^-23 of their magnitudes, and is rounded twice more (times the scale, less the
+    maximum), with the maximum and the exponential 2^-22 (1 + |score| + |maximum|); sums of n tokens are off by (n / 32 + 64) 2^-23 of the magnitudes.  These are errors of
+    each token's own weight and of the total.  What a weight loses as 16-bit numbers is WEIGHT of itself and SMALLEST of the largest weight of its 32 tokens."""
+    dtype = q.dtype
+    q, k, v = f64(q), f64(k), f64(v)
+    group, n = q.shape[0] // k.shape[1], k.shape[0]
+    k, v = (t.repeat_interleave(group, 1).transpose(0, 1).contiguous() for t in (k, v))
+    scale = 1 / math.sqrt(q.shape[1]) if scale is None else scale
+    scores = torch.matmul(k, q[:, :, None])[:, :, 0] * scale
+    size = torch.matmul(k.abs(), q.abs()[:, :, None])[:, :, 0] * abs(scale)
+    top = scores.amax(1, keepdim=True)
+    w = torch.exp(scores - top)
+    w = w / w.sum(1, keepdim=True)
+    off = (q.shape[1] + 4) * 2.0**-23 * size + 2.0**-22 * (1 + scores.abs() + top.abs())
+    of_sums = (n / 32 + 64) * 2.0**-23
+    padded = torch.nn.functional.pad(w, (0, -n % 32)).view(q.shape[0], -1, 32)
+    beside = padded.amax(2, keepdim=True).expand_as(padded).reshape(q.shape[0], -1)[:, :n]
+    apart = w * (off + WEIGHT[dtype] + of_sums) + SMALLEST[dtype] * beside
+    out = torch.matmul(w[:, None], v)[:, 0]
+    of_total = (w * off).sum(1, keepdim=True) + of_sums
+    return out, torch.matmul(apart[:, None], v.abs())[:, 0] + of_total * out.abs()
+
+
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("shared", [False, True], ids=["whole", "shared"])
 @pytest.mark.parametrize("n", [1, 30, 700])
@@ -53,3 +85,27 @@ def test_scores_that_have_no_fraction(n, shared, dtype):
         out = paged_attention(q, cache, table, lengths)
         want = f64(v[first:first + winners, 0]).mean(0).expand(2, 64)
         within(out[0], want, (winners / 32 + 64) * 2.0**-23 * f64(v[first:first + winners, 0]).abs().mean(0), f"{winners} of {n}")
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("shared", [False, True], ids=["whole", "shared"])
+@pytest.mark.parametrize("spread", [0.0, 1.0])
+@pytest.mark.parametrize("gap", [8.0, 14.0, 16.0, 18.0, 22.0])
+def test_a_first_token_that_has_nearly_all_weight(gap, spread, shared, dtype):
+    """Its value is 0, so that a result is made of the others' small weights: none of them may be lost, however small, outside of its own step of 32."""
+    g = torch.Generator().manual_seed(int(gap))
+    heads, kv_heads, dim = 8, 2, 64
+    sequences = []
+    for n in (40, 64, 300, 2000):
+        k, v = torch.zeros(n, kv_heads, dim), 200 * (2 + torch.randn(n, kv_heads, dim, generator=g))
+        k[:, :, 0] = spread * torch.randn(n, kv_heads, generator=g)
+        k[0, :, 0] = gap
+        v[0] = 0
+        sequences.append((k, v))
+    cache, table, lengths = _cache_of(sequences, dtype)
+    q = torch.zeros(len(sequences), heads, dim, dtype=dtype, device=DEV)
+    q[:, :, 0] = 8                                         # times 1 / sqrt(64): a score is the key's first element
+    out = paged_attention(q, cache, _widened(table, 6000) if shared else table, lengths)
+    for i, (k, v) in enumerate(sequences):
+        want, off = formula(q[i], k.to(DEV).to(dtype), v.to(DEV).to(dtype))
+        within(out[i], want, off, f"{k.shape[0]} tokens")
