@@ -74,8 +74,7 @@ __global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendA
 #pragma unroll
             for (int u = 0; u < kAtOnce; u++) {
                 const int k = k0 + 4 * u + sub, last = here - 1;
-                const float of_k = __shfl(times, k & 63);             // (of all lanes: 0 behind the last)
-                w[u] = k < here ? of_k : 0.0f;
+                w[u] = __shfl(times, k & 63);                         // (of all lanes)
                 const float* from = nth_part(i0 + (k < here ? k : last)) + row_at;
 #pragma unroll
                 for (int nv = 0; nv < NV; nv++) {
@@ -84,7 +83,8 @@ __global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendA
                 }
             }
 #pragma unroll
-            for (int u = 0; u < kAtOnce; u++)
+            for (int u = 0; u < kAtOnce; u++) {
+                if (k0 + 4 * u + sub >= here) continue;               // (the last part again, whose sums may be infinite)
 #pragma unroll
                 for (int nv = 0; nv < NV; nv++)
 #pragma unroll
@@ -92,6 +92,7 @@ __global__ __launch_bounds__(kJoinThreads) void attend_join_kernel(const AttendA
                         f[nv][i] += x[u][nv][i] * w[u];
                         f[nv][4 + i] += y[u][nv][i] * w[u];
                     }
+            }
         }
     }
 #pragma unroll

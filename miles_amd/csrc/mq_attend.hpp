@@ -7,8 +7,9 @@
 //   output   O^T += V^T P^T: the same lane needs, for element 8 c + e of the values, the weights and values of eight tokens.  Which
 //            eight is free as long as both operands agree: 4 g + r of both halves of the 32, whose weights it has, and
 //            whose values it reads as rows of 16 bytes; eight such rows are rearranged in its own registers, one instruction for two elements.
-// Weights enter as the sum of two 16-bit numbers (one alone would be off by as much as the result's own rounding), which hold 16 bits of them in bf16; in
-// fp16 22, and whatever is above 2^-40 of the largest weight in the same tile.  The matrix cores have the time (6 % of the cycles in 16 bits, 10 in 8).  What bounds it is reading keys and values
+// Weights enter as sums of 16-bit numbers (one alone would be off by as much as the result's own rounding): three in bf16, which hold all their bits (two
+// would leave 2 in 1000 results on the other side of a rounding, where these leave 4 in 10000), two in fp16, which hold 21, and whatever is above 2^-39 of the
+// largest weight in the same tile.  The matrix cores have the time.  What bounds it is reading keys and values
 // once: a tile's keys are asked for when the last tile's have been used, its values likewise, so that a wavefront always has one of the two on its way, and two wavefronts on a
 // SIMD keep 64 KB a compute unit in flight.  32 query heads over 8 key heads of 128, bf16: 64 sequences of 8192 tokens 332 us, 6.5 TB/s; 64 of 1 to
 // 8192 in 122, 5.9 TB/s (in 8 bits 125, 6.0 TB/s: half the bytes for twice the tokens); one of 131072 in 93, 5.8 TB/s; one of 1024 in 8.
@@ -97,6 +98,36 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {           // inclusi
 template <int D>
 __device__ __forceinline__ void store8(char* to, const float* f) {
     *(u32x4*)to = pack<D>(f);
+}
+// Two weights as sums of 16-bit numbers, all of them positive where the weight is: a value that is infinite times a part of 0, or times parts of both signs,
+// would be a NaN, where its product with the weight is that infinity.  Each part but the last is what is left without its last bits, and where nothing is left
+// the smallest number that the matrix instructions count (bf16: the smallest normal one, which is below 2^-100 of any weight that matters; fp16: 2^-24 of 2^15).
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t smaller2(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+}
+template <int D>
+constexpr int kWeightParts = D == MQ_F16 ? 2 : 3;
+template <int D>
+__device__ __forceinline__ void split_weights(float p, float q, u32x4* parts, int i) {
+    if (D == MQ_F16) {
+        const uint32_t big = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p, q));
+        parts[0][i] = big;
+        parts[1][i] = larger2(pack2<D>(p - elem_lo<true>(big), q - elem_hi<true>(big)), smaller2(big, 0x00010001u));
+        return;
+    }
+    uint32_t least = 0u;
+#pragma unroll
+    for (int part = 0; part < kWeightParts<D>; part++) {
+        const uint32_t high = __builtin_amdgcn_perm(f2u(q), f2u(p), 0x07060302u);
+        if (part == 0) least = smaller2(high, 0x00800080u);
+        parts[part][i] = part == 0 ? high : larger2(high, least);
+        p -= u2f(f2u(p) & 0xFFFF0000u);
+        q -= u2f(f2u(q) & 0xFFFF0000u);
+    }
 }
 // what a row of sums is multiplied with at the end, with the sink in its total; no weight at all: zeros
 __device__ __forceinline__ float finish_factor(const AttendArgs& a, int head, float m, float l) {
@@ -371,13 +402,9 @@ __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 
 #pragma unroll
                 for (int i = 0; i < 8; i++) total += p[i];
             }
-            uint32_t big[4], small[4];
+            u32x4 weights[kWeightParts<D>];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                big[i] = pack2<D>(p[2 * i], p[2 * i + 1]);
-                small[i] = pack2<D>(p[2 * i] - elem_lo<D == MQ_F16>(big[i]), p[2 * i + 1] - elem_hi<D == MQ_F16>(big[i]));
-            }
-            const u32x4 weights[2] = {{big[0], big[1], big[2], big[3]}, {small[0], small[1], small[2], small[3]}};
+            for (int i = 0; i < 4; i++) split_weights<D>(p[2 * i], p[2 * i + 1], weights, i);
             // ---- values
 #pragma unroll
             for (int nv = 0; nv < NV; nv++) {
@@ -390,7 +417,9 @@ __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 
                         x[i] = u32x4{lo.x, lo.y, hi.x, hi.y};
                     } else x[i] = v[nv][i];
                 }
-                constexpr int kAtOnce = 4;                // products that do not wait for each other
+                // products that do not wait for each other, while two wavefronts' registers suffice (one after the other: 33 sequences of up to 9001 tokens, 40 heads over one of 256: 39.9 us instead of
+                // 38.5)
+                constexpr int kAtOnce = kOwnTop && NV == 2 && !attend_is_wide(NK, NV) ? 2 : 4;
 #pragma unroll
                 for (int e0 = 0; e0 < 8; e0 += kAtOnce) {
                     u32x4 row8[kAtOnce];
@@ -404,7 +433,7 @@ __global__ __launch_bounds__(kAttendWaves * kWave, attend_is_wide(NK, NV) ? 1 : 
                         sum[i] = kOwnTop ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc[nv * 8 + e];
                     }
 #pragma unroll
-                    for (int part = 0; part < 2; part++)
+                    for (int part = 0; part < kWeightParts<D>; part++)
 #pragma unroll
                         for (int i = 0; i < kAtOnce; i++) sum[i] = mfma<D>(row8[i], weights[part], sum[i]);
 #pragma unroll

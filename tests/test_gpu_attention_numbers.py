@@ -1,4 +1,4 @@
-"""Attention over a paged cache where numbers are large or small, against the formula in 64 bits."""
+"""Attention over a paged cache where numbers are large, small or infinite, against the formula in 64 bits."""
 
 import math
 
@@ -13,10 +13,10 @@ from tests.serving_checks import DEV
 pytestmark = pytest.mark.gpu
 HALVES = [torch.bfloat16, torch.float16]
 PAGE = 16
-# What a weight is off by as two 16-bit numbers, the second the rounded rest: of itself, and of the largest among the same 32 tokens, which is 2^15 where fp16's
-# smallest steps are 2^-24
-WEIGHT = {torch.bfloat16: 2.0**-17, torch.float16: 2.0**-22}
-SMALLEST = {torch.bfloat16: 0.0, torch.float16: 2.0**-40}
+# What a weight is off by as a sum of 16-bit numbers.  bf16: nothing, three of them hold all its bits.  fp16: what is left without the last bits is below 2^-10 of it and
+# rounded to 2^-11 of itself; and, of the largest among the same 32 tokens, which is 2^15, half of fp16's smallest steps of 2^-24, or one of them where nothing is left
+WEIGHT = {torch.bfloat16: 0.0, torch.float16: 2.0**-21}
+SMALLEST = {torch.bfloat16: 0.0, torch.float16: 2.0**-39}
 
 
 def _cache_of(sequences, dtype):
@@ -109,3 +109,41 @@ def test_a_first_token_that_has_nearly_all_weight(gap, spread, shared, dtype):
     for i, (k, v) in enumerate(sequences):
         want, off = formula(q[i], k.to(DEV).to(dtype), v.to(DEV).to(dtype))
         within(out[i], want, off, f"{k.shape[0]} tokens")
+
+
+def _random(lengths, heads, kv_heads, key_dim, value_dim, dtype, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    randn = lambda *shape: torch.randn(shape, generator=g, device=DEV).to(dtype)  # noqa: E731
+    return randn(len(lengths), heads, key_dim), [(randn(n, kv_heads, key_dim), randn(n, kv_heads, value_dim)) for n in lengths]
+
+
+def _check(out, q, sequences, which=None):
+    for i in range(len(sequences)) if which is None else which:
+        k, v = sequences[i]
+        if k.shape[0] == 0:
+            assert (out[i] == 0).all()
+            continue
+        want, off = formula(q[i], k, v)
+        far = ~torch.isfinite(want)
+        assert torch.equal(torch.nan_to_num(f64(out[i])[far], 7.0), torch.nan_to_num(want[far], 7.0)), f"sequence {i} of {k.shape[0]} tokens"
+        within(out[i].masked_fill(far, 0), want.masked_fill(far, 0), off.masked_fill(far, 0), f"sequence {i} of {k.shape[0]} tokens")
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("lengths,heads,kv_heads,key_dim,value_dim,width", [
+    ([1, 2, 33, 100], 4, 2, 64, 64, 0), ([1, 2, 33, 600], 4, 2, 64, 64, 6000), ([40, 500], 20, 1, 128, 256, 0), ([9000, 3, 700], 40, 1, 256, 256, 0), ([9000, 20], 8, 2, 128, 128, 0),
+    ([0] * 299 + [5000], 4, 2, 64, 256, 0)], ids=["whole", "shared", "wide", "many heads", "long", "many sequences"])
+def test_infinite_values_that_are_seen(lengths, heads, kv_heads, key_dim, value_dim, width, dtype):
+    """One infinity among the values of an element makes its result that infinity, two of different signs a NaN; the other elements do not notice.
+    All scores are within e^12 of each other, so that every token has a weight."""
+    q, sequences = _random(lengths, heads, kv_heads, key_dim, value_dim, dtype)
+    for k, v in sequences:
+        n = v.shape[0]
+        if n == 0:
+            continue
+        v[0, :, 3], v[n - 1, :, 5], v[n // 2, :, value_dim - 1] = math.inf, -math.inf, math.inf
+        v[0, :, 9], v[n - 1, :, 10] = math.inf, math.inf
+        if n > 1:
+            v[n - 1, :, 9] = -math.inf
+    cache, table, n = _cache_of(sequences, dtype)
+    _check(paged_attention(q, cache, _widened(table, width), n), q, sequences)
