@@ -147,3 +147,14 @@ def test_infinite_values_that_are_seen(lengths, heads, kv_heads, key_dim, value_
             v[n - 1, :, 9] = -math.inf
     cache, table, n = _cache_of(sequences, dtype)
     _check(paged_attention(q, cache, _widened(table, width), n), q, sequences)
+
+
+@pytest.mark.parametrize("lengths,heads,kv_heads,key_dim,value_dim", [([130007], 2, 1, 64, 64), ([130007], 5, 1, 64, 256), ([0] * 150 + [40001] + [0] * 149, 4, 1, 64, 64), (
+    [3] * 9 + [40001] + [0] * 290, 4, 1, 64, 256)])
+def test_a_row_of_more_than_64_parts_a_wavefront_of_the_join(lengths, heads, kv_heads, key_dim, value_dim):
+    """About a thousand parts for four wavefronts of a workgroup, and some 300 for one wavefront."""
+    q, sequences = _random(lengths, heads, kv_heads, key_dim, value_dim, torch.bfloat16)
+    cache, table, n = _cache_of(sequences, torch.bfloat16)
+    out = paged_attention(q, cache, table, n)
+    _check(out, q, sequences)
+    assert torch.equal(out, paged_attention(q, cache, table, n))
