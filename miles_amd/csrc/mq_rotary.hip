@@ -26,8 +26,7 @@ struct RotaryArgs {
     int64_t tokens, total;         // of a batch entry, and of all
     int64_t first;                 // token of this launch
     int dim, per;                  // elements of a vector; tokens of a workgroup
-    int units_head;                // of a vector: accesses (pairs of them in the halves layout), or single elements
-    SmallDivisor by_token, by_head;
+    SmallDivisor by_token, by_head;        // units of a token and of a vector: accesses (pairs of them in the halves layout), or single elements
 };
 constexpr int kRotaryThreads = 256, kRotaryTurns = 2048, kRotaryTokens = 16;
 
@@ -165,7 +164,6 @@ extern "C" int mq_rotary(const struct mq_heads* x, int n, int dtype, int64_t bat
     a.dim = (int)dim;
     const int64_t units = vec ? (interleaved ? dim / v : (dim - pairs) / v) : dim - pairs;
     if (heads * units > 65535 * (vec ? 1 : 64)) return mq_fail(MQ_ERR_ARG, "mq_rotary: tensor too large");
-    a.units_head = (int)units;
     // Tokens of a workgroup: enough for all lanes to have an angle to compute and an access or two to make, while there are workgroups for every
     // compute unit (8192 tokens of 9 heads of 64 by eight at once 7.0 us, by one 12.9; of 40 heads of 128 by one or two 58, by four 61, by eight 70).
     int64_t per = 1;

@@ -14,7 +14,7 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 // cos and sin of x, |x| < 2^50 or so: x less the nearest multiple n of pi/2, which two 53-bit pieces of pi/2 give to 2^-53 of
 // a radian while n < 2^52, then the Taylor series on [-pi/4, pi/4], whose first terms left out are (pi/4)^17 / 17! = 5e-17 and
-// (pi/4)^16 / 16! = 1e-15.  Some 30 operations of 64 bits, at the rate of 32-bit ones here, for each pair and token, not for each head.
+// (pi/4)^18 / 18! = 2e-18.  Some 30 operations of 64 bits, at the rate of 32-bit ones here, for each pair and token, not for each head.
 __device__ __forceinline__ void cos_sin(double x, double& c, double& s) {
     const double n = __builtin_rint(x * 0.63661977236758134308);                  // 2 / pi
     const double r = __builtin_fma(-n, 6.1232339957367659e-17, __builtin_fma(-n, 1.5707963267948966, x));
