@@ -137,8 +137,9 @@ struct AttendPlan {
     int64_t bytes, starts_bytes;
 };
 // Tiles that a wavefront goes through at most where every workgroup has a row of its own: half as many where there are few rows, of which a long one
-// would keep the others waiting.  32 query heads over 8 of 128, from 1 to the given number of tokens (us, rows of their own / shared out): 8 sequences
-// to 1024 13.1 / 14.1, to 2048 21.7 / 14.9; 24 to 2048 23.5 / 23.7 (all of 2048: 33 / 41), to 4096 43 / 32; 64 to 2048 36 / 39, to 4096 69 / 66.
+// would keep the others waiting.  32 query heads over 8 of 128, random lengths up to the given number of tokens, in brackets all of it (us, rows of their own / shared out):
+// 8 sequences to 1024 13.0 / 14.8 (15.0 / 15.8), to 2048 21.8 / 16.9 (25.2 / 25.1); 24 to 2048 29.6 / 31.4 (37 / 43), to 4096 55 / 47 (64 / 75); 64 to 1024
+// 31 / 33 (46 / 51), to 2048 62 / 61 (89 / 92), to 4096 109 / 100 (173 / 177).
 constexpr int64_t kDirectSteps = 16, kManyRows = 128, kMostGrid = 1 << 22;
 
 // false: too large

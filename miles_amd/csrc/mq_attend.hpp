@@ -9,10 +9,10 @@
 //            whose values it reads as rows of 16 bytes; eight such rows are rearranged in its own registers, one instruction for two elements.
 // Weights enter as sums of 16-bit numbers (one alone would be off by as much as the result's own rounding): three in bf16, which hold all their bits (two
 // would leave 2 in 1000 results on the other side of a rounding, where these leave 4 in 10000), two in fp16, which hold 21, and whatever is above 2^-39 of the
-// largest weight in the same tile.  The matrix cores have the time.  What bounds it is reading keys and values
+// largest weight in the same tile.  The matrix cores have the time (7 % of the cycles in 16 bits, 13 in 8).  What bounds it is reading keys and values
 // once: a tile's keys are asked for when the last tile's have been used, its values likewise, so that a wavefront always has one of the two on its way, and two wavefronts on a
-// SIMD keep 64 KB a compute unit in flight.  32 query heads over 8 key heads of 128, bf16: 64 sequences of 8192 tokens 332 us, 6.5 TB/s; 64 of 1 to
-// 8192 in 122, 5.9 TB/s (in 8 bits 125, 6.0 TB/s: half the bytes for twice the tokens); one of 131072 in 93, 5.8 TB/s; one of 1024 in 8.
+// SIMD keep 64 KB a compute unit in flight.  32 query heads over 8 key heads of 128, bf16: 64 sequences of 8192 tokens 330 us, 6.5 TB/s; 64 of 1 to
+// 8192 in 122, 5.9 TB/s (in 8 bits 125, 6.0 TB/s: half the bytes for twice the tokens); one of 131072 in fp16 in 94, 5.7 TB/s; one of 1024 in 12.5.
 #pragma once
 #include "mq_gemm.hpp"
 #include "mq_paged.hpp"
