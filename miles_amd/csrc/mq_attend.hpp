@@ -101,7 +101,7 @@ __device__ __forceinline__ void store8(char* to, const float* f) {
 }
 // Two weights as sums of 16-bit numbers, all of them positive where the weight is: a value that is infinite times a part of 0, or times parts of both signs,
 // would be a NaN, where its product with the weight is that infinity.  Each part but the last is what is left without its last bits, and where nothing is left
-// the smallest number that the matrix instructions count (bf16: the smallest normal one, which is below 2^-100 of any weight that matters; fp16: 2^-24 of 2^15).
+// the smallest number of the type, which the matrix instructions count like any other (bf16: 2^-133; fp16: 2^-24, of 2^15).
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t smaller2(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
@@ -123,7 +123,7 @@ __device__ __forceinline__ void split_weights(float p, float q, u32x4* parts, in
 #pragma unroll
     for (int part = 0; part < kWeightParts<D>; part++) {
         const uint32_t high = __builtin_amdgcn_perm(f2u(q), f2u(p), 0x07060302u);
-        if (part == 0) least = smaller2(high, 0x00800080u);
+        if (part == 0) least = smaller2(high, 0x00010001u);
         parts[part][i] = part == 0 ? high : larger2(high, least);
         p -= u2f(f2u(p) & 0xFFFF0000u);
         q -= u2f(f2u(q) & 0xFFFF0000u);

@@ -17,6 +17,8 @@ PAGE = 16
 # rounded to 2^-11 of itself; and, of the largest among the same 32 tokens, which is 2^15, half of fp16's smallest steps of 2^-24, or one of them where nothing is left
 WEIGHT = {torch.bfloat16: 0.0, torch.float16: 2.0**-21}
 SMALLEST = {torch.bfloat16: 0.0, torch.float16: 2.0**-39}
+# bf16: two parts may be the smallest number where nothing is left, 2^-133, of weights whose largest in the sequence is 1 at least
+LEAST = {torch.bfloat16: 2.0**-132, torch.float16: 0.0}
 
 
 def _cache_of(sequences, dtype):
@@ -46,7 +48,8 @@ def formula(q, k, v, scale=None):
 
     A score is a sum of key_dim products in fp32, off by (key_dim + 4) 2^-23 of their magnitudes, and is rounded twice more (times the scale, less the
     maximum), with the maximum and the exponential 2^-22 (1 + |score| + |maximum|); sums of n tokens are off by (n / 32 + 64) 2^-23 of the magnitudes.  These are errors of
-    each token's own weight and of the total.  What a weight loses as 16-bit numbers is WEIGHT of itself and SMALLEST of the largest weight of its 32 tokens."""
+    each token's own weight and of the total.  What a weight loses as 16-bit numbers is WEIGHT of itself and SMALLEST of the largest weight of its 32 tokens, LEAST of the
+    largest of all."""
     dtype = q.dtype
     q, k, v = f64(q), f64(k), f64(v)
     group, n = q.shape[0] // k.shape[1], k.shape[0]
@@ -61,7 +64,7 @@ def formula(q, k, v, scale=None):
     of_sums = (n / 32 + 64) * 2.0**-23
     padded = torch.nn.functional.pad(w, (0, -n % 32)).view(q.shape[0], -1, 32)
     beside = padded.amax(2, keepdim=True).expand_as(padded).reshape(q.shape[0], -1)[:, :n]
-    apart = w * (off + WEIGHT[dtype] + of_sums) + SMALLEST[dtype] * beside
+    apart = w * (off + WEIGHT[dtype] + of_sums) + SMALLEST[dtype] * beside + LEAST[dtype] * w.amax(1, keepdim=True)
     out = torch.matmul(w[:, None], v)[:, 0]
     of_total = (w * off).sum(1, keepdim=True) + of_sums
     return out, torch.matmul(apart[:, None], v.abs())[:, 0] + of_total * out.abs()
@@ -90,7 +93,7 @@ def test_scores_that_have_no_fraction(n, shared, dtype):
 @pytest.mark.parametrize("dtype", HALVES)
 @pytest.mark.parametrize("shared", [False, True], ids=["whole", "shared"])
 @pytest.mark.parametrize("spread", [0.0, 1.0])
-@pytest.mark.parametrize("gap", [8.0, 14.0, 16.0, 18.0, 22.0])
+@pytest.mark.parametrize("gap", [8.0, 14.0, 16.0, 18.0, 22.0, 81.0])
 def test_a_first_token_that_has_nearly_all_weight(gap, spread, shared, dtype):
     """Its value is 0, so that a result is made of the others' small weights: none of them may be lost, however small, outside of its own step of 32."""
     g = torch.Generator().manual_seed(int(gap))
